@@ -381,6 +381,48 @@ int oasr_gemm_fp8_pw(const uint8_t* a, const uint8_t* w_packed, const float* sca
                      const float* bias, const float* resid, void* c, int64_t m, int64_t n, int64_t k,
                      float alpha, int32_t epilogue, void* stream);
 
+/* 8-bit integer path.  None of these has a counterpart in the reference.
+ *
+ * Rows of bf16 to int8 codes with one scale each (a token's scale):
+ *   scale[r] = max|x[r]| / 127 (1 for an all-zero row), y[r][c] = rint(127 x[r][c] / max|x[r]|), ties to even.
+ * x: rows of k values, `ldx` apart (any k, any alignment of a row's start); y: rows `ldy` apart (a multiple of 16, at
+ * least k rounded up to 64; y 16-byte aligned), columns k .. round_up(k, 64) - 1 are written as zeros, the rest of the
+ * pitch is left alone.  A row that holds a NaN or an infinity gets a scale that is NaN or infinite, and every output
+ * made from it is NaN.  rows may be 0. */
+int oasr_quant_i8_rows(const uint16_t* x, int64_t ldx, int64_t rows, int64_t k, int8_t* y, int64_t ldy, float* scale,
+                       void* stream);
+
+/* LayerNorm (optionally followed by Swish) of float32 rows straight to int8 codes and scales: the codes are made from
+ * the float32 result (rint(v * (127 / max|v|))).  oasr_layernorm2_i8 is the double form of a block boundary (x is
+ * overwritten with its first LayerNorm).  d as for oasr_layernorm_fp8; all pointers but scale 16-byte aligned. */
+int oasr_layernorm_i8(const float* x, const float* w, const float* b, int8_t* y, float* scale, int64_t rows, int32_t d,
+                      float eps, int32_t swish, void* stream);
+int oasr_layernorm2_i8(float* x, const float* w1, const float* b1, const float* w2, const float* b2, int8_t* y,
+                       float* scale, int64_t rows, int32_t d, float eps, void* stream);
+
+/* Weights of the 8-bit product, laid out once: int8 codes w[n][k] (rows `ldw` apart) to pieces of 16 rows x 64 k,
+ * padded with zeros; out holds oasr_gemm_i8_packed_bytes(n, k) bytes and is 16-byte aligned.  Any n, k <= 131072. */
+int64_t oasr_gemm_i8_packed_bytes(int64_t n, int64_t k);
+int oasr_gemm_pack_w_i8(const int8_t* w, int64_t ldw, int64_t n, int64_t k, int8_t* out, void* stream);
+
+/* C[m][n] = epilogue(scale_a[m] * scale_w[n] * sum_k A8[m][k] * W8[n][k]): sums in 32-bit integers, exact (k <= 131072).
+ * Any m (0: nothing is done), n, k; epilogues of oasr_epilogue, bias float32[n] or NULL with each of them
+ * (OASR_EPI_GLU_BF16: n a multiple of 32, bias interleaved as the rows are, C of n / 2 columns).
+ * a: rows `lda` apart as oasr_quant_i8_rows writes them - 16-byte aligned, lda a multiple of 16 and at least k rounded up to
+ * 64, zeros from k up to there.  c, resid: rows `ldc`, `ldr` elements apart; resid may be c (with ldr = ldc), apart from
+ * that no operand may overlap c.  Rows and columns of the pitch outside m x n are neither read nor written. */
+int oasr_gemm_i8(const int8_t* a, int64_t lda, const int8_t* w_packed, const float* scale_a, const float* scale_w,
+                 const float* bias, const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k,
+                 float alpha, int32_t epilogue, void* stream);
+
+/* Both steps: the bf16 rows x (ldx apart) are quantised and multiplied.  The same bits as oasr_quant_i8_rows followed by
+ * oasr_gemm_i8.  workspace: device, oasr_linear_i8_workspace_bytes(m, k), 256-byte aligned, contents on entry do not
+ * matter; calls that may overlap need one each. */
+int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t k);
+int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const float* scale_w, const float* bias,
+                   const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, float alpha,
+                   int32_t epilogue, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Multi-head self-attention with clamped relative-key bias and key-length masking.
  * qkv bf16 [rows][3*d] (q | k | v), ctx bf16 [rows][d], d = n_heads * head_dim; head_dim 64
  * or 128; dist_emb bf16 [96][head_dim] (rows past left_max + right_max zero).  The kernel works in

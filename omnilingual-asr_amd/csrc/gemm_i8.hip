@@ -1,0 +1,500 @@
+// 8-bit integer products with a scale for each row of A (a token) and each row of W (an output channel):
+//   C[m][n] = epi( sa[m] * sw[n] * sum_k A8[m][k] * W8[n][k] )
+// The sums are exact 32-bit integers (k <= 131072), so neither the order of summation nor a split of K over waves
+// changes a bit of the result; the only roundings are the integer's conversion to float32, the two scales' products,
+// the epilogue and the output type.
+//
+// Weights are packed once (oasr_gemm_pack_w_i8): pieces of 16 rows x 64 k, 1 KiB each, ordered [row group][K slice],
+// rows and k padded with zeros; chunk c (16 bytes) of row r of a piece sits at chunk c ^ ((r >> 2) & 3).  That is the
+// LDS image of a piece, and it makes the fragment reads (lane = (row r = lane & 15, chunk lane >> 4)) free of bank
+// conflicts; A's rows are brought into the same image by the copies' source addresses.
+// The weight fragment is the matrix instruction's A operand (v_mfma_i32_16x16x64_i8), so a lane ends up with four
+// consecutive n of one row m: C[m = lane & 15][n = 4 (lane >> 4) + e].
+#include "oasr_common.h"
+#include "quant_i8.h"
+
+namespace oasr {
+namespace i8 {
+
+constexpr int kSlice = 64;                 // k per slice: one MFMA step
+constexpr int kPiece = 16 * kSlice;        // bytes of 16 rows of a slice
+constexpr int64_t kMaxK = 131072;          // 128 * 127 * k < 2^31
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void gbl_void;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+struct GemmArgs {
+    const int8_t* a;        // [m][lda], zeros from k to round_up(k, 64)
+    const int8_t* w;        // packed
+    const float* scale_a;
+    const float* scale_w;
+    const float* bias;      // may be null
+    const float* resid;     // residual epilogue only
+    void* c;
+    int64_t lda, ldr, ldc, m, n;
+    int ks;                 // K slices
+    int ng;                 // groups of 16 rows of W
+    float alpha;
+    int vec;                // c and resid rows start on 16-byte boundaries
+};
+
+__device__ __forceinline__ uint32_t cvt_pk_bf16(float a, float b) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf2;
+    bf2 v;
+    v[0] = (__bf16)a;
+    v[1] = (__bf16)b;
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+#define OASR_I8_BARRIER()                     \
+    do {                                      \
+        asm volatile("" ::: "memory");        \
+        __builtin_amdgcn_sched_barrier(0);    \
+        __builtin_amdgcn_s_barrier();         \
+        __builtin_amdgcn_sched_barrier(0);    \
+        asm volatile("" ::: "memory");        \
+    } while (0)
+
+// Four consecutive entries of a per-column vector, guarded at n.
+__device__ __forceinline__ f32x4 load_cols(const float* __restrict__ p, int64_t col, int64_t n, float missing) {
+    f32x4 v = {missing, missing, missing, missing};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (p && col + e < n) v[e] = p[col + e];
+    return v;
+}
+
+// Four consecutive outputs, of which the first `count` exist.
+__device__ __forceinline__ void store_f32(float* p, f32x4 v, int64_t count, bool vec) {
+    if (vec && count >= 4) {
+        *reinterpret_cast<f32x4*>(p) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < count) p[e] = v[e];
+    }
+}
+__device__ __forceinline__ void store_bf16(uint16_t* p, u32x2 v, int64_t count) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < count) p[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+}
+
+// Two neighbouring 16-column tiles of bf16 results, four columns of each per lane: lanes 16 apart trade halves, so
+// that a lane holds eight consecutive columns and a row leaves as 64 consecutive bytes.
+__device__ __forceinline__ void store_bf16_pair(uint16_t* row, int64_t col, u32x2 t0, u32x2 t1, int64_t n, bool vec, int g) {
+    if (vec && col + 32 <= n) {
+        const auto p = __builtin_amdgcn_permlane16_swap(t0[0], t1[0], false, false);
+        const auto q = __builtin_amdgcn_permlane16_swap(t0[1], t1[1], false, false);
+        // even lane rows hold tile 0, odd ones tile 1; lane rows 0, 1 its columns 0..7, lane rows 2, 3 columns 8..15
+        const u32x4 v = {p[0], q[0], p[1], q[1]};
+        *reinterpret_cast<u32x4*>(row + col + 16 * (g & 1) + 8 * (g >> 1)) = v;
+    } else {
+        store_bf16(row + col + 4 * g, t0, n - (col + 4 * g));
+        store_bf16(row + col + 16 + 4 * g, t1, n - (col + 16 + 4 * g));
+    }
+}
+
+// A wave's MT x NT tiles of 16 x 16, the first at (m0, n0): scales, bias, epilogue, guarded stores.
+template <int EPI, int MT, int NT>
+__device__ __forceinline__ void epilogue(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane) {
+    static_assert(NT % 2 == 0, "columns are stored in pairs of tiles");
+    const int r = lane & 15, g = lane >> 4;
+    f32x4 sw[NT], bv[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        sw[j] = load_cols(p.scale_w, n0 + 16 * j + 4 * g, p.n, 0.f);
+        bv[j] = load_cols(p.bias, n0 + 16 * j + 4 * g, p.n, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t row = m0 + 16 * i + r;
+        if (row >= p.m) continue;
+        const float s = p.scale_a[row];
+        f32x4 o[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] = fmaf((float)acc[i][j][e] * sw[j][e], s, bv[j][e]);   // the weight's scale first: a token's may be as large as float32 goes
+        if (EPI == OASR_EPI_BIAS_F32 || EPI == OASR_EPI_RESIDUAL_F32) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int64_t col = n0 + 16 * j + 4 * g, count = p.n - col;
+                if (EPI == OASR_EPI_RESIDUAL_F32) {
+                    const float* from = p.resid + row * p.ldr + col;
+                    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                    if (p.vec && count >= 4) {
+                        x = *reinterpret_cast<const f32x4*>(from);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (e < count) x[e] = from[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] = fmaf(p.alpha, o[j][e], x[e]);
+                }
+                store_f32(reinterpret_cast<float*>(p.c) + row * p.ldc + col, o[j], count, p.vec);
+            }
+        } else {
+            uint16_t* crow = reinterpret_cast<uint16_t*>(p.c) + row * p.ldc;
+            if (EPI == OASR_EPI_GLU_BF16) {      // tile 2 q = 16 value columns, tile 2 q + 1 = their gates (n % 32 == 0)
+                u32x2 t[NT / 2];
+#pragma unroll
+                for (int q = 0; q < NT / 2; ++q) {
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = o[2 * q][e] * sigmoidf(o[2 * q + 1][e]);
+                    t[q] = (u32x2){cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
+                }
+                if (NT == 2) {
+                    store_bf16(crow + n0 / 2 + 4 * g, t[0], p.n / 2 - (n0 / 2 + 4 * g));
+                } else {
+#pragma unroll
+                    for (int q = 0; q + 1 < NT / 2; q += 2)
+                        store_bf16_pair(crow, n0 / 2 + 16 * q, t[q], t[q + 1], p.n / 2, p.vec, g);
+                }
+            } else {
+                u32x2 t[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if (EPI == OASR_EPI_BIAS_SWISH_BF16)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[j][e] = swishf(o[j][e]);
+                    t[j] = (u32x2){cvt_pk_bf16(o[j][0], o[j][1]), cvt_pk_bf16(o[j][2], o[j][3])};
+                }
+#pragma unroll
+                for (int j = 0; j < NT; j += 2) store_bf16_pair(crow, n0 + 16 * j, t[j], t[j + 1], p.n, p.vec, g);
+            }
+        }
+    }
+}
+
+// One work-group of WM x WN waves computes a tile of (16 MT WM) x (16 NT WN).  K runs through a ring of RING slices in
+// LDS, filled by direct copies RING - 1 slices ahead, one barrier per slice: behind the barrier of slice p every wave
+// has seen its own copies of slice p land and has read slice p - 1, so the slot of p - 1 may be filled again.
+// Rows of A past m repeat row m - 1 and row groups of W past the last repeat the last: read, multiplied, never stored.
+template <int EPI, int WM, int WN, int MT, int NT, int RING>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmArgs p, int tiles_n) {
+    constexpr int kWaves = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
+    constexpr int kPieces = (BM + BN) / 16, kCopies = kPieces / kWaves, kSlot = kPieces * kPiece;
+    static_assert(kPieces % kWaves == 0, "every wave issues the same number of copies");
+    __shared__ __attribute__((aligned(1024))) char ring[RING * kSlot];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * BM, n0 = (int64_t)(blockIdx.x % tiles_n) * BN;
+
+    const char* src[kCopies];
+    int step[kCopies];
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+        const int q = wave * kCopies + i;
+        if (q < BM / 16) {
+            int64_t row = m0 + 16 * q + (lane >> 2);
+            row = row < p.m ? row : p.m - 1;
+            src[i] = reinterpret_cast<const char*>(p.a) + row * p.lda + (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+            step[i] = kSlice;
+        } else {
+            int64_t grp = n0 / 16 + (q - BM / 16);
+            grp = grp < p.ng ? grp : p.ng - 1;
+            src[i] = reinterpret_cast<const char*>(p.w) + grp * p.ks * kPiece + lane * 16;
+            step[i] = kPiece;
+        }
+    }
+    auto copy_next = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            __builtin_amdgcn_global_load_lds((gbl_void*)src[i], (lds_void*)(ring + slot * kSlot + (wave * kCopies + i) * kPiece), 16, 0, 0);
+            src[i] += step[i];
+        }
+    };
+
+    i32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
+    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ ((fr >> 2) & 3)) << 4);
+
+    for (int t = 0; t < RING - 1 && t < p.ks; ++t) copy_next(t);
+    int slot = 0, fill = RING - 1;
+    for (int t = 0; t < p.ks; ++t) {
+        if (t + RING - 1 <= p.ks)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * kCopies) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last slices: fewer copies than the ring are in flight
+        OASR_I8_BARRIER();
+        if (t + RING - 1 < p.ks) {
+            copy_next(fill);
+            fill = fill + 1 == RING ? 0 : fill + 1;
+        }
+        const char* sa = ring + slot * kSlot + wm * MT * kPiece;
+        const char* sw = ring + slot * kSlot + (BM / 16 + wn * NT) * kPiece;
+        i32x4 wf[NT], xf[MT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) wf[j] = *reinterpret_cast<const i32x4*>(sw + j * kPiece + frag);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(sa + i * kPiece + frag);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[i][j], 0, 0, 0);
+        slot = slot + 1 == RING ? 0 : slot + 1;
+    }
+    epilogue<EPI, MT, NT>(p, acc, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+}
+
+// Per-row quantisation of bf16 rows.  One wavefront per row with the row in registers (k <= 512 NV: NV loads of 16
+// bytes per lane, all issued before the first use), or, for longer rows, in two sweeps of which the second reads from
+// cache.  HBM-bound: 2 bytes in, 1 byte out per element.  Row starts need no alignment; the codes' rows are whole
+// 64-byte slices, zero from k on.
+struct __attribute__((packed, aligned(2))) bf16x8_any {
+    uint32_t w[4];
+};
+
+__device__ __forceinline__ u32x4 load_row8(const uint16_t* __restrict__ xr, int64_t c, int64_t k) {
+    u32x4 v = {0, 0, 0, 0};
+    if (c + 8 <= k) {
+        const bf16x8_any t = *reinterpret_cast<const bf16x8_any*>(xr + c);
+        v = (u32x4){t.w[0], t.w[1], t.w[2], t.w[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < k) v[e >> 1] |= (uint32_t)xr[c + e] << (16 * (e & 1));
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t amax8(u32x4 v, uint32_t amax) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t lo = (v[q] << 16) & 0x7fffffffu, hi = v[q] & 0x7fff0000u;
+        amax = amax > lo ? amax : lo;
+        amax = amax > hi ? amax : hi;
+    }
+    return amax;
+}
+
+__device__ __forceinline__ u32x2 codes8(u32x4 v, const RowScale& s) {
+    uint32_t c[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        c[2 * q] = code_of_bf16(__uint_as_float(v[q] << 16), s);
+        c[2 * q + 1] = code_of_bf16(__uint_as_float(v[q] & 0xffff0000u), s);
+    }
+    return (u32x2){pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7])};
+}
+
+template <int NV>
+__global__ __launch_bounds__(256) void quant_i8_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t rows,
+                                                            int64_t k, int8_t* __restrict__ y, int64_t ldy,
+                                                            float* __restrict__ scale) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const uint16_t* xr = x + row * ldx;
+    int8_t* yr = y + row * ldy;
+    const int64_t kp = (k + kSlice - 1) / kSlice * kSlice;
+    uint32_t amax = 0;
+    u32x4 v[NV > 0 ? NV : 1];
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = load_row8(xr, 8 * lane + 512 * i, k);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) amax = amax8(v[i], amax);
+    } else {
+        for (int64_t c = 8 * lane; c < k; c += 512) amax = amax8(load_row8(xr, c, k), amax);
+    }
+    const RowScale s = row_scale(wave_umax(amax));
+    if (lane == 0) scale[row] = s.scale;
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = 8 * lane + 512 * i;
+            if (c < kp) *reinterpret_cast<u32x2*>(yr + c) = codes8(v[i], s);
+        }
+    } else {
+        for (int64_t c = 8 * lane; c < kp; c += 512) *reinterpret_cast<u32x2*>(yr + c) = codes8(load_row8(xr, c, k), s);
+    }
+}
+
+// Row-major weight codes -> packed pieces, one 16-byte chunk per thread.
+__global__ __launch_bounds__(256) void gemm_pack_w_i8_kernel(const int8_t* __restrict__ w, int64_t ldw, int64_t n, int64_t k,
+                                                             int64_t ks, int64_t chunks, int8_t* __restrict__ out) {
+    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (idx >= chunks) return;
+    const int lane = (int)(idx & 63);
+    const int64_t piece = idx >> 6, grp = piece / ks, t = piece - grp * ks;
+    const int64_t row = grp * 16 + (lane >> 2), col = t * kSlice + (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (row < n)
+        for (int e = 0; e < 16; ++e)
+            if (col + e < k) v[e >> 2] |= (uint32_t)(uint8_t)w[row * ldw + col + e] << (8 * (e & 3));
+    *reinterpret_cast<u32x4*>(out + idx * 16) = (u32x4){v[0], v[1], v[2], v[3]};
+}
+
+static int check_gemm(const char* what, const int8_t* w, const float* scale_w, const float* bias, const float* resid,
+                      int64_t ldr, const void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, int32_t epilogue) {
+    OASR_REQUIRE(m >= 0 && n > 0 && k > 0, "%s: n and k must be positive, m not negative", what);
+    OASR_REQUIRE(k <= kMaxK, "%s: k=%lld exceeds %lld (the sums are 32-bit integers)", what, (long long)k, (long long)kMaxK);
+    OASR_REQUIRE(m < ((int64_t)1 << 31) && n < ((int64_t)1 << 31), "%s: m and n must be below 2^31", what);
+    OASR_REQUIRE(epilogue >= OASR_EPI_BIAS_BF16 && epilogue <= OASR_EPI_BIAS_F32, "%s: unknown epilogue %d", what, epilogue);
+    OASR_REQUIRE(epilogue != OASR_EPI_GLU_BF16 || n % 32 == 0, "%s: the GLU epilogue needs n=%lld to be a multiple of 32", what,
+                 (long long)n);
+    OASR_REQUIRE(ldc >= (epilogue == OASR_EPI_GLU_BF16 ? n / 2 : n), "%s: ldc=%lld is shorter than a row", what, (long long)ldc);
+    OASR_REQUIRE(epilogue != OASR_EPI_RESIDUAL_F32 || ldr >= n, "%s: ldr=%lld is shorter than a row", what, (long long)ldr);
+    if (m == 0) return OASR_OK;
+    OASR_REQUIRE(w && scale_w && c, "%s: null pointer", what);
+    OASR_REQUIRE(epilogue != OASR_EPI_RESIDUAL_F32 || resid, "%s: residual epilogue without resid", what);
+    const int elt = epilogue == OASR_EPI_RESIDUAL_F32 || epilogue == OASR_EPI_BIAS_F32 ? 4 : 2;
+    OASR_REQUIRE(((uintptr_t)w & 15) == 0, "%s: the packed weights must be 16-byte aligned", what);
+    OASR_REQUIRE(((uintptr_t)c & (elt - 1)) == 0 && ((uintptr_t)scale_w & 3) == 0 && ((uintptr_t)bias & 3) == 0 &&
+                     ((uintptr_t)resid & 3) == 0,
+                 "%s: misaligned pointer", what);
+    return OASR_OK;
+}
+
+template <int EPI>
+static void launch_tiles(const GemmArgs& p, hipStream_t st) {
+    const int64_t tiles_n = (p.n + 127) / 128, tiles = (p.m + 127) / 128 * tiles_n;
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<EPI, 2, 2, 4, 4, 4>), dim3((unsigned)tiles), dim3(256), 0, st, p, (int)tiles_n);
+}
+
+static int launch_gemm(const GemmArgs& p, int32_t epilogue, hipStream_t st) {
+    OASR_REQUIRE((p.m + 127) / 128 * ((p.n + 127) / 128) < ((int64_t)1 << 31), "gemm_i8: too many tiles");
+    switch (epilogue) {
+        case OASR_EPI_BIAS_BF16: launch_tiles<OASR_EPI_BIAS_BF16>(p, st); break;
+        case OASR_EPI_BIAS_SWISH_BF16: launch_tiles<OASR_EPI_BIAS_SWISH_BF16>(p, st); break;
+        case OASR_EPI_GLU_BF16: launch_tiles<OASR_EPI_GLU_BF16>(p, st); break;
+        case OASR_EPI_RESIDUAL_F32: launch_tiles<OASR_EPI_RESIDUAL_F32>(p, st); break;
+        default: launch_tiles<OASR_EPI_BIAS_F32>(p, st); break;
+    }
+    OASR_CHECK_LAUNCH("gemm_i8");
+    return OASR_OK;
+}
+
+static GemmArgs gemm_args(const int8_t* a, int64_t lda, const int8_t* w, const float* scale_a, const float* scale_w,
+                          const float* bias, const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k,
+                          float alpha, int32_t epilogue) {
+    GemmArgs p;
+    p.a = a;
+    p.w = w;
+    p.scale_a = scale_a;
+    p.scale_w = scale_w;
+    p.bias = bias;
+    p.resid = resid;
+    p.c = c;
+    p.lda = lda;
+    p.ldr = ldr;
+    p.ldc = ldc;
+    p.m = m;
+    p.n = n;
+    p.ks = (int)((k + kSlice - 1) / kSlice);
+    p.ng = (int)((n + 15) / 16);
+    p.alpha = alpha;
+    const int elt = epilogue == OASR_EPI_RESIDUAL_F32 || epilogue == OASR_EPI_BIAS_F32 ? 4 : 2;
+    p.vec = ((uintptr_t)c & 15) == 0 && ((uintptr_t)resid & 15) == 0 && ldc * elt % 16 == 0 && ldr % 4 == 0;
+    return p;
+}
+
+static int quant_rows(const uint16_t* x, int64_t ldx, int64_t rows, int64_t k, int8_t* y, int64_t ldy, float* scale,
+                      hipStream_t st) {
+    const dim3 grid((unsigned)((rows + 3) / 4)), blk(256);
+#define OASR_QUANT_I8(NV) hipLaunchKernelGGL(quant_i8_rows_kernel<NV>, grid, blk, 0, st, x, ldx, rows, k, y, ldy, scale)
+    // the row in registers up to 16384 columns (32 loads per lane), the smallest form that covers it
+    if (k <= 512) OASR_QUANT_I8(1);
+    else if (k <= 1024) OASR_QUANT_I8(2);
+    else if (k <= 2048) OASR_QUANT_I8(4);
+    else if (k <= 4096) OASR_QUANT_I8(8);
+    else if (k <= 8192) OASR_QUANT_I8(16);
+    else if (k <= 16384) OASR_QUANT_I8(32);
+    else OASR_QUANT_I8(0);
+#undef OASR_QUANT_I8
+    OASR_CHECK_LAUNCH("quant_i8_rows");
+    return OASR_OK;
+}
+
+}  // namespace i8
+}  // namespace oasr
+
+using namespace oasr;
+
+extern "C" {
+
+int oasr_quant_i8_rows(const uint16_t* x, int64_t ldx, int64_t rows, int64_t k, int8_t* y, int64_t ldy, float* scale,
+                       void* stream) {
+    OASR_REQUIRE(rows >= 0 && k > 0, "quant_i8_rows: k must be positive and rows not negative");
+    OASR_REQUIRE(rows < ((int64_t)1 << 31), "quant_i8_rows: too many rows");
+    OASR_REQUIRE(ldx >= k && ldy % 16 == 0 && ldy >= round_up(k, i8::kSlice),
+                 "quant_i8_rows: ldx must cover k, ldy must be a multiple of 16 and cover k rounded up to 64");
+    if (rows == 0) return OASR_OK;
+    OASR_REQUIRE(x && y && scale, "quant_i8_rows: null pointer");
+    OASR_REQUIRE(((uintptr_t)x & 1) == 0 && ((uintptr_t)y & 15) == 0 && ((uintptr_t)scale & 3) == 0,
+                 "quant_i8_rows: misaligned pointer");
+    return i8::quant_rows(x, ldx, rows, k, y, ldy, scale, (hipStream_t)stream);
+}
+
+int64_t oasr_gemm_i8_packed_bytes(int64_t n, int64_t k) {
+    if (n <= 0 || k <= 0) return 0;
+    return round_up(n, 16) * round_up(k, i8::kSlice);
+}
+
+int oasr_gemm_pack_w_i8(const int8_t* w, int64_t ldw, int64_t n, int64_t k, int8_t* out, void* stream) {
+    OASR_REQUIRE(n > 0 && k > 0 && ldw >= k, "gemm_pack_w_i8: n and k must be positive and ldw cover k");
+    OASR_REQUIRE(k <= i8::kMaxK && n < ((int64_t)1 << 31), "gemm_pack_w_i8: k must not exceed %lld and n must be below 2^31",
+                 (long long)i8::kMaxK);
+    OASR_REQUIRE(w && out && w != out, "gemm_pack_w_i8: null pointer or in-place call");
+    OASR_REQUIRE(((uintptr_t)out & 15) == 0, "gemm_pack_w_i8: out must be 16-byte aligned");
+    const int64_t chunks = oasr_gemm_i8_packed_bytes(n, k) / 16;
+    OASR_REQUIRE(chunks / 256 + 1 < ((int64_t)1 << 31), "gemm_pack_w_i8: matrix too large");
+    hipLaunchKernelGGL(i8::gemm_pack_w_i8_kernel, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, (hipStream_t)stream, w, ldw,
+                       n, k, round_up(k, i8::kSlice) / i8::kSlice, chunks, out);
+    OASR_CHECK_LAUNCH("gemm_pack_w_i8");
+    return OASR_OK;
+}
+
+int oasr_gemm_i8(const int8_t* a, int64_t lda, const int8_t* w_packed, const float* scale_a, const float* scale_w,
+                 const float* bias, const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, float alpha,
+                 int32_t epilogue, void* stream) {
+    const int rc = i8::check_gemm("gemm_i8", w_packed, scale_w, bias, resid, ldr, c, ldc, m, n, k, epilogue);
+    if (rc != OASR_OK) return rc;
+    OASR_REQUIRE(lda % 16 == 0 && lda >= round_up(k, i8::kSlice), "gemm_i8: lda must be a multiple of 16 and cover k rounded up to 64");
+    if (m == 0) return OASR_OK;
+    OASR_REQUIRE(a && scale_a, "gemm_i8: null pointer");
+    OASR_REQUIRE(((uintptr_t)a & 15) == 0 && ((uintptr_t)scale_a & 3) == 0, "gemm_i8: misaligned pointer");
+    return i8::launch_gemm(i8::gemm_args(a, lda, w_packed, scale_a, scale_w, bias, resid, ldr, c, ldc, m, n, k, alpha, epilogue), epilogue,
+                           (hipStream_t)stream);
+}
+
+int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t k) {
+    if (m <= 0 || k <= 0) return 0;
+    return round_up(m * round_up(k, i8::kSlice), 256) + round_up(m * 4, 256);
+}
+
+int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const float* scale_w, const float* bias,
+                   const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, float alpha, int32_t epilogue,
+                   void* workspace, int64_t workspace_bytes, void* stream) {
+    const int rc = i8::check_gemm("linear_i8", w_packed, scale_w, bias, resid, ldr, c, ldc, m, n, k, epilogue);
+    if (rc != OASR_OK) return rc;
+    OASR_REQUIRE(ldx >= k, "linear_i8: ldx must cover k");
+    if (m == 0) return OASR_OK;
+    OASR_REQUIRE(x && workspace, "linear_i8: null pointer");
+    OASR_REQUIRE(((uintptr_t)x & 1) == 0 && ((uintptr_t)workspace & 255) == 0, "linear_i8: misaligned pointer (workspace: 256 bytes)");
+    if (workspace_bytes < oasr_linear_i8_workspace_bytes(m, k)) {
+        set_error("linear_i8: workspace needs %lld bytes, got %lld", (long long)oasr_linear_i8_workspace_bytes(m, k),
+                  (long long)workspace_bytes);
+        return OASR_ECAPACITY;
+    }
+    const int64_t kp = round_up(k, i8::kSlice);
+    int8_t* q = static_cast<int8_t*>(workspace);
+    float* s = reinterpret_cast<float*>(q + round_up(m * kp, 256));
+    const int rq = i8::quant_rows(x, ldx, m, k, q, kp, s, (hipStream_t)stream);
+    if (rq != OASR_OK) return rq;
+    return i8::launch_gemm(i8::gemm_args(q, kp, w_packed, s, scale_w, bias, resid, ldr, c, ldc, m, n, k, alpha, epilogue), epilogue,
+                           (hipStream_t)stream);
+}
+
+}  // extern "C"

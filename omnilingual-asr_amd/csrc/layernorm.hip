@@ -3,6 +3,7 @@
 // wave reductions, and the result leaves as packed bf16 (GEMM operand) or float32.
 // HBM-bound: d*4 bytes in, d*2 (or d*4) bytes out per row, nothing re-read.
 #include "oasr_common.h"
+#include "quant_i8.h"
 #include "row_norm.h"
 
 namespace oasr {
@@ -152,6 +153,67 @@ __global__ __launch_bounds__(256) void layernorm2_fp8_kernel(float* __restrict__
     store_row_fp8<VPL>(v, y + row * D, scale, row, lane);
 }
 
+// int8 output for the 8-bit integer projections: scale = max|row| / 127 (1 for an all-zero row), codes = rint(127 v /
+// max|row|) of the float32 normalised row as it stands in registers (no 16-bit rounding in between).  Bytes as the e4m3
+// form: 4 in, 1 out per element.
+template <int VPL>
+__device__ __forceinline__ void store_row_i8(const float4 (&v)[VPL], int8_t* __restrict__ yr, float* __restrict__ scale,
+                                             int64_t row, int lane) {
+    uint32_t amax = 0;
+    auto take = [&](float x) {
+        const uint32_t b = i8::abs_bits(x);
+        amax = amax > b ? amax : b;
+    };
+#pragma unroll
+    for (int c = 0; c < VPL; ++c) {
+        take(v[c].x);
+        take(v[c].y);
+        take(v[c].z);
+        take(v[c].w);
+    }
+    const i8::RowScale s = i8::row_scale(i8::wave_umax(amax));
+    if (lane == 0) scale[row] = s.scale;
+#pragma unroll
+    for (int c = 0; c < VPL; ++c)
+        *reinterpret_cast<uint32_t*>(yr + 4 * lane + 256 * c) =
+            i8::pack4(i8::code_of_f32(v[c].x, s), i8::code_of_f32(v[c].y, s), i8::code_of_f32(v[c].z, s), i8::code_of_f32(v[c].w, s));
+}
+
+// TWO: x is overwritten with its first LayerNorm (w1, b1), and the codes are those of the second (w2, b2) of that.
+template <int VPL, bool SWISH, bool TWO>
+__global__ __launch_bounds__(256) void layernorm_i8_kernel(float* __restrict__ x, const float* __restrict__ w1,
+                                                           const float* __restrict__ b1, const float* __restrict__ w2,
+                                                           const float* __restrict__ b2, int8_t* __restrict__ y,
+                                                           float* __restrict__ scale, int64_t rows, float eps) {
+    constexpr int D = 256 * VPL;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    float* xr = x + row * D;
+    float4 v[VPL];
+#pragma unroll
+    for (int c = 0; c < VPL; ++c) v[c] = *reinterpret_cast<const float4*>(xr + 4 * lane + 256 * c);
+    float mean, rstd;
+    row_stats<VPL>(v, mean, rstd, eps);
+    row_affine<VPL>(v, mean, rstd, w1, b1, lane);
+    if (TWO) {
+#pragma unroll
+        for (int c = 0; c < VPL; ++c) *reinterpret_cast<float4*>(xr + 4 * lane + 256 * c) = v[c];
+        row_stats<VPL>(v, mean, rstd, eps);
+        row_affine<VPL>(v, mean, rstd, w2, b2, lane);
+    }
+    if (SWISH) {
+#pragma unroll
+        for (int c = 0; c < VPL; ++c) {
+            v[c].x = swishf(v[c].x);
+            v[c].y = swishf(v[c].y);
+            v[c].z = swishf(v[c].z);
+            v[c].w = swishf(v[c].w);
+        }
+    }
+    store_row_i8<VPL>(v, y + row * D, scale, row, lane);
+}
+
 // d = 160 (the stacked feature rows): 40 float4 per row on lanes 0..39; output row pitch
 // y_stride >= 160 with the tail zero-filled so it can feed a GEMM whose K is padded to 192.
 template <bool OUT_BF16>
@@ -206,6 +268,31 @@ static int launch_ln(const float* x, const float* w, const float* b, void* y, in
     else
         hipLaunchKernelGGL((layernorm_kernel<VPL, false, false>), grid, blk, 0, st, x, w, b, y, rows, y_stride, eps);
     return 0;
+}
+
+template <bool SWISH, bool TWO>
+static int launch_ln_i8(const char* what, float* x, const float* w1, const float* b1, const float* w2, const float* b2, int8_t* y,
+                        float* scale, int64_t rows, int32_t d, float eps, hipStream_t st) {
+    OASR_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 33), "%s: bad row count", what);
+    OASR_REQUIRE(d == 256 || d == 512 || d == 1024 || d == 2048 || d == 4096, "%s: unsupported width %d (256, 512, 1024, 2048, 4096)",
+                 what, d);
+    if (rows == 0) return OASR_OK;
+    OASR_REQUIRE(x && w1 && b1 && w2 && b2 && y && scale, "%s: null pointer", what);
+    OASR_REQUIRE((((uintptr_t)x | (uintptr_t)w1 | (uintptr_t)b1 | (uintptr_t)w2 | (uintptr_t)b2 | (uintptr_t)y) & 15) == 0 &&
+                     ((uintptr_t)scale & 3) == 0,
+                 "%s: misaligned pointer", what);
+    const dim3 grid((unsigned)((rows + 3) / 4)), blk(256);
+#define OASR_LNI8(V) hipLaunchKernelGGL((layernorm_i8_kernel<V, SWISH, TWO>), grid, blk, 0, st, x, w1, b1, w2, b2, y, scale, rows, eps)
+    switch (d) {
+        case 256: OASR_LNI8(1); break;
+        case 512: OASR_LNI8(2); break;
+        case 1024: OASR_LNI8(4); break;
+        case 2048: OASR_LNI8(8); break;
+        default: OASR_LNI8(16);
+    }
+#undef OASR_LNI8
+    OASR_CHECK_LAUNCH(what);
+    return OASR_OK;
 }
 
 }  // namespace oasr
@@ -295,6 +382,18 @@ int oasr_layernorm2_fp8(float* x, const float* w1, const float* b1, const float*
 #undef OASR_LN28
     OASR_CHECK_LAUNCH("layernorm2_fp8");
     return OASR_OK;
+}
+
+int oasr_layernorm_i8(const float* x, const float* w, const float* b, int8_t* y, float* scale, int64_t rows, int32_t d,
+                      float eps, int32_t swish, void* stream) {
+    float* xr = const_cast<float*>(x);   // only the double form writes x
+    return swish ? launch_ln_i8<true, false>("layernorm_i8", xr, w, b, w, b, y, scale, rows, d, eps, (hipStream_t)stream)
+                 : launch_ln_i8<false, false>("layernorm_i8", xr, w, b, w, b, y, scale, rows, d, eps, (hipStream_t)stream);
+}
+
+int oasr_layernorm2_i8(float* x, const float* w1, const float* b1, const float* w2, const float* b2, int8_t* y, float* scale,
+                       int64_t rows, int32_t d, float eps, void* stream) {
+    return launch_ln_i8<false, true>("layernorm2_i8", x, w1, b1, w2, b2, y, scale, rows, d, eps, (hipStream_t)stream);
 }
 
 int oasr_layernorm2(float* x, const float* w1, const float* b1, const float* w2, const float* b2,

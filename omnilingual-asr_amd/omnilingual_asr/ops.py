@@ -1,0 +1,178 @@
+"""Operators on torch tensors: checked arguments, buffers from torch's allocator, the tensors' own device and its current
+stream.  Each call is one or two launches of liboasr_hip.so (the C ABI takes raw pointers: include/oasr.h); nothing
+synchronises, so a call may be captured into a HIP graph.  A mistake raises ValueError before anything is launched.
+
+No counterpart in the reference, whose projections and answers are made by a remote model
+(ref:src/omnilingual_asr/models/inference/gemini_pipeline.py:512-530).
+"""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _hip
+from .weights import quantize_rows_i8
+
+EPILOGUES = {"bias": _hip.EPI_BIAS_BF16, "swish": _hip.EPI_BIAS_SWISH_BF16, "glu": _hip.EPI_GLU_BF16,
+             "residual": _hip.EPI_RESIDUAL_F32, "float": _hip.EPI_BIAS_F32}
+_NORM_WIDTHS = (256, 512, 1024, 2048, 4096)
+_NULL = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device's context, entered only where another one is current."""
+    return _NULL if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _rows(t, what: str, dtype):
+    """(tensor, rows, columns, row pitch) of a [..., columns] tensor whose rows are contiguous and evenly spaced."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        raise ValueError(f"{what} must be a {dtype} tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be on a HIP device; there is no CPU fallback")
+    if t.dim() < 1:
+        raise ValueError(f"{what} must have at least one dimension")
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.dim() > 2 else t[None, :]
+    rows, cols = t.shape
+    pitch = t.stride(0) if rows > 1 else cols
+    if cols > 1 and t.stride(1) != 1 or pitch < cols:
+        raise ValueError(f"{what} must have contiguous rows that do not overlap")
+    return t, rows, cols, pitch
+
+
+def _overlap(a, b) -> bool:
+    """Whether the memory between the first and the last element of two strided tensors meets."""
+    def span(t):
+        if t.numel() == 0:
+            return 0, 0
+        lo = t.data_ptr()
+        return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _vector(t, n: int, what: str, device) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what} must be a contiguous float32 vector of {n} on {device}")
+    return t.data_ptr()
+
+
+class LinearI8:
+    """y = epilogue(x W^T + bias) with W and x in 8-bit integers: W has one scale per output row, every row of x gets its
+    own (max|row| / 127) inside the call, and the products are summed exactly in 32-bit integers.
+
+    `epilogue`: "bias" -> bf16, "swish" -> bf16, "glu" -> bf16 of half the width (rows of W interleaved as
+    `weights.glu_interleave` does, a multiple of 32), "float" -> float32, "residual" -> resid + alpha * (...) in float32.
+    The packed weights belong to the object and must not be in use by another stream when it is dropped."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None):
+        """`weight`: float [out, in] on a HIP device; quantised per output row."""
+        if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_floating_point():
+            raise ValueError("weight must be a float tensor [out, in]")
+        self._lay_out(*quantize_rows_i8(weight), bias)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None) -> "LinearI8":
+        """From int8 codes [out, in] and float32 scales [out] (weight = codes * scale[:, None])."""
+        self = cls.__new__(cls)
+        self._lay_out(codes, scale, bias)
+        return self
+
+    def _lay_out(self, codes, scale, bias):
+        if codes.dim() != 2:
+            raise ValueError("codes must be [out, in]")
+        codes, n, k, ldw = _rows(codes, "codes", torch.int8)
+        if n < 1 or not 1 <= k <= 131072:
+            raise ValueError("a weight has at least one row and 1 to 131072 columns")
+        self.device, self.out_features, self.in_features = codes.device, n, k
+        self._scale_ptr, self._bias_ptr = _vector(scale, n, "scale", codes.device), _vector(bias, n, "bias", codes.device)
+        if scale is None:
+            raise ValueError("scale must be given")
+        self.scale, self.bias = scale, bias
+        L = _hip.lib()
+        with _on(self.device):
+            self.packed = torch.empty((int(L.oasr_gemm_i8_packed_bytes(n, k)),), dtype=torch.int8, device=self.device)
+            _hip.check(L.oasr_gemm_pack_w_i8(codes.data_ptr(), ldw, n, k, self.packed.data_ptr(), _hip.current_stream_ptr()),
+                       "oasr_gemm_pack_w_i8")
+        self._packed_ptr = self.packed.data_ptr()
+
+    def _output(self, x, epilogue, resid, out):
+        """(epilogue code, output, its row pitch, residual's pointer, its row pitch) for input x."""
+        epi = EPILOGUES.get(epilogue)
+        if epi is None:
+            raise ValueError(f"epilogue must be one of {', '.join(EPILOGUES)}")
+        n = self.out_features
+        if epi == _hip.EPI_GLU_BF16:
+            if n % 32:
+                raise ValueError("the GLU epilogue needs a multiple of 32 output rows")
+            n //= 2
+        dtype = torch.float32 if epi in (_hip.EPI_RESIDUAL_F32, _hip.EPI_BIAS_F32) else torch.bfloat16
+        shape = (*x.shape[:-1], n)
+        given = out is not None
+        if not given:
+            out = torch.empty(shape, dtype=dtype, device=self.device)
+        elif out.shape != shape or out.device != self.device:
+            raise ValueError(f"out must be of shape {shape} on {self.device}")
+        flat, _, _, ldc = _rows(out, "out", dtype)
+        if given and flat.data_ptr() != out.data_ptr():
+            raise ValueError("out must have evenly spaced rows")
+        if given and _overlap(flat, x):
+            raise ValueError("out must not overlap x")
+        if epi != _hip.EPI_RESIDUAL_F32:
+            if resid is not None:
+                raise ValueError("resid goes with the residual epilogue only")
+            return epi, out, ldc, None, 0
+        if resid is None or resid.shape != shape or resid.device != self.device:
+            raise ValueError(f"the residual epilogue needs resid of shape {shape} on {self.device}")
+        r, _, _, ldr = _rows(resid, "resid", torch.float32)
+        if given and _overlap(flat, r) and (r.data_ptr() != flat.data_ptr() or ldr != ldc):
+            raise ValueError("resid may be out itself, or must not overlap it")
+        return epi, out, ldc, r, ldr
+
+    def __call__(self, x: torch.Tensor, *, epilogue: str = "bias", resid: torch.Tensor | None = None, alpha: float = 1.0,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+        """x bf16 [..., in] -> [..., out].  `out` may be given (rows evenly spaced) and may be `resid`."""
+        x2, m, k, ldx = _rows(x, "x", torch.bfloat16)
+        if k != self.in_features or x.device != self.device:
+            raise ValueError(f"x must have {self.in_features} columns on {self.device}")
+        epi, out, ldc, resid, ldr = self._output(x, epilogue, resid, out)
+        if m == 0:
+            return out
+        L = _hip.lib()
+        with _on(self.device):
+            ws_bytes = int(L.oasr_linear_i8_workspace_bytes(m, k))
+            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=self.device)
+            _hip.check(L.oasr_linear_i8(x2.data_ptr(), ldx, self._packed_ptr, self._scale_ptr, self._bias_ptr,
+                                        None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m,
+                                        self.out_features, k, alpha, epi, ws.data_ptr(), ws_bytes, _hip.current_stream_ptr()), "oasr_linear_i8")
+        return out
+
+    def normed(self, x: torch.Tensor, gain: torch.Tensor, shift: torch.Tensor, *, eps: float = 1e-5, epilogue: str = "bias",
+               resid: torch.Tensor | None = None, alpha: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The layer on LayerNorm(x) * gain + shift: x float32 [..., in] contiguous, in 256, 512, 1024, 2048 or 4096.  The
+        normalised rows go to 8-bit integers without being stored in between."""
+        x2, m, k, ldx = _rows(x, "x", torch.float32)
+        if k != self.in_features or x.device != self.device:
+            raise ValueError(f"x must have {self.in_features} columns on {self.device}")
+        if k not in _NORM_WIDTHS or ldx != k or x2.data_ptr() % 16:
+            raise ValueError(f"normed takes contiguous, 16-byte aligned rows of {', '.join(map(str, _NORM_WIDTHS))} columns")
+        gain_ptr, shift_ptr = _vector(gain, k, "gain", self.device), _vector(shift, k, "shift", self.device)
+        epi, out, ldc, resid, ldr = self._output(x, epilogue, resid, out)
+        if m == 0:
+            return out
+        L = _hip.lib()
+        with _on(self.device):
+            st = _hip.current_stream_ptr()
+            codes = torch.empty((m, k), dtype=torch.int8, device=self.device)
+            scale = torch.empty((m,), dtype=torch.float32, device=self.device)
+            _hip.check(L.oasr_layernorm_i8(x2.data_ptr(), gain_ptr, shift_ptr, codes.data_ptr(), scale.data_ptr(), m, k, eps, 0, st),
+                       "oasr_layernorm_i8")
+            _hip.check(L.oasr_gemm_i8(codes.data_ptr(), k, self._packed_ptr, scale.data_ptr(), self._scale_ptr, self._bias_ptr,
+                                      None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m,
+                                      self.out_features, k, alpha, epi, st), "oasr_gemm_i8")
+        return out

@@ -141,6 +141,16 @@ def quantize_rows_e4m3(w: torch.Tensor):
     return codes.view(torch.uint8), scale
 
 
+def quantize_rows_i8(w: torch.Tensor):
+    """Per-row 8-bit integer quantisation: (codes int8 [out, in], scale float32 [out]) with w ~= codes * scale,
+    scale = max|row| / 127 (1 for an all-zero row), codes = rint(127 w / max|row|)."""
+    w = w.to(torch.float32)
+    amax = w.abs().amax(dim=1)
+    amax = torch.where(amax > 0, amax, torch.full_like(amax, 127.0))
+    codes = (w.to(torch.float64) * 127.0 / amax[:, None]).round().to(torch.int8)
+    return codes, amax / 127.0
+
+
 def pack_for_device(weights: dict, g: Geometry, device, fp8: bool = False) -> dict:
     """Device tensors in the layout of `oasr_layer_weights` / `oasr_top_weights` (include/oasr.h);
     with `fp8`, also the e4m3 codes and row scales of `oasr_layer_fp8_weights`."""

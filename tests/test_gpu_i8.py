@@ -1,0 +1,306 @@
+"""GPU tests of the 8-bit integer operators: codes and scales against the definition (bit for bit), products and epilogues
+against 64-bit sums of the same codes within bounds that tests/i8_tools.py derives, and the calls around them (strides,
+empty batches, aliasing, streams, graphs, offsets past 32 bits).  Parity unpinned against the reference, which has none."""
+
+import math
+
+import pytest
+import torch
+
+from omnilingual_asr import _hip as H
+from omnilingual_asr import ops
+from omnilingual_asr.weights import quantize_rows_i8
+from tests.i8_tools import assert_within, finish64, product64, quantize64, weight_codes
+
+pytestmark = pytest.mark.gpu
+
+
+def _quant(x, ldy=None, fill=77):
+    rows, k = x.shape
+    kp = (k + 63) // 64 * 64
+    y = torch.full((rows, ldy or kp), fill, dtype=torch.int8, device="cuda")
+    s = torch.full((rows,), -1.0, device="cuda")
+    H.check(H.lib().oasr_quant_i8_rows(x.data_ptr(), x.stride(0), rows, k, y.data_ptr(), y.shape[1], s.data_ptr(), H.current_stream_ptr()))
+    torch.cuda.synchronize()
+    return y, s
+
+
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 63), (5, 64), (7, 65), (4, 511), (9, 512), (6, 1000), (33, 1024), (5, 2047),
+                                    (17, 4096), (3, 8191), (5, 16384), (2, 16385), (3, 40001)])
+def test_quant_rows_bit_for_bit(rows, k):
+    g = torch.Generator().manual_seed(rows * 7 + k)
+    x = (torch.randn((rows, k), generator=g) * torch.rand((rows, 1), generator=g) * 4).to(torch.bfloat16)
+    x[rows // 2] = x[rows // 2].abs().max() * torch.tensor([1.0, 0.5, -0.5, 0.25]).repeat(k // 4 + 1)[:k]   # ties: 63.5, 31.75
+    if rows > 2:
+        x[0] = 0
+    pitch = k + 3                                       # rows that start at any alignment
+    buf = torch.zeros((rows, pitch), dtype=torch.bfloat16, device="cuda")
+    buf[:, :k] = x.cuda()
+    kp = (k + 63) // 64 * 64
+    y, s = _quant(buf[:, :k], ldy=kp + 16)
+    want, scale = quantize64(x)
+    assert torch.equal(y[:, :k].cpu().double(), want)
+    assert (y[:, k:kp] == 0).all() and (y[:, kp:] == 77).all()
+    assert torch.equal(s.cpu(), (x.float().abs().amax(1) / 127.0).masked_fill(x.abs().amax(1) == 0, 1.0))
+
+
+def test_quant_rows_at_the_ends_of_the_range():
+    """Smallest and largest rows keep their codes; NaN and infinity show in the scale, whatever else the row holds."""
+    x = torch.zeros((8, 70), dtype=torch.bfloat16)
+    x[0, :3] = torch.tensor([9.2e-41, -9.2e-41, 0.0])                   # the smallest bf16
+    x[1, :3] = torch.tensor([3.3895e38, -1.69e38, 1e30])                # the largest
+    x[2, :3] = torch.tensor([1e-38, 5e-39, -2.5e-39])
+    x[3, :3] = torch.tensor([float("nan"), 1.0, 2.0])
+    x[4, :3] = torch.tensor([float("inf"), 1.0, -2.0])
+    x[5, :3] = torch.tensor([-float("inf"), float("nan"), -2.0])
+    x[6, 69] = -5.0
+    y, s = _quant(x.cuda())
+    want, _ = quantize64(x[[0, 1, 2, 6, 7]])
+    assert torch.equal(y[[0, 1, 2, 6, 7], :70].cpu().double(), want)
+    sc = s.cpu()
+    assert torch.isnan(sc[3]) and torch.isinf(sc[4]) and torch.isnan(sc[5]) and sc[7] == 1.0
+    assert torch.allclose(sc[[0, 1, 2, 6]].double(), x[[0, 1, 2, 6]].double().abs().amax(1) / 127, rtol=1e-2, atol=0)
+    codes, scale = weight_codes(33, 70, torch.Generator().manual_seed(1))
+    out = ops.LinearI8.from_codes(codes.cuda(), scale.cuda())(x.cuda(), epilogue="float").cpu()
+    assert torch.isnan(out[3:6]).all() and torch.isfinite(out[[0, 1, 2, 6, 7]]).all()
+
+
+SHAPES = [(1, 1, 1), (1, 33, 64), (1, 1024, 512), (2, 1000, 1000), (3, 64, 65), (15, 96, 63), (16, 128, 128), (17, 130, 640),
+          (33, 4096, 256), (64, 512, 4096), (99, 2048, 1024), (127, 257, 191), (128, 128, 64), (129, 384, 320), (200, 777, 1000),
+          (256, 256, 64), (300, 96, 16448), (513, 1024, 512), (1000, 4096, 64), (1504, 1024, 1024), (2100, 640, 192),
+          (4096, 512, 512), (8200, 1056, 320)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("epilogue", ["bias", "swish", "glu", "residual", "float"])
+def test_linear_i8(m, n, k, epilogue):
+    g = torch.Generator().manual_seed(m + 3 * n + 7 * k)
+    if epilogue == "glu":
+        n = (n + 31) // 32 * 32
+    x = (torch.randn((m, k), generator=g) * (0.2 + 2 * torch.rand((m, 1), generator=g))).to(torch.bfloat16)
+    codes, scale = weight_codes(n, k, g)
+    bias = torch.randn((n,), generator=g) if n % 5 else None
+    resid = torch.randn((m, n), generator=g) if epilogue == "residual" else None
+    layer = ops.LinearI8.from_codes(codes.cuda(), scale.cuda(), None if bias is None else bias.cuda())
+    got = layer(x.cuda(), epilogue=epilogue, resid=None if resid is None else resid.cuda(), alpha=0.5)
+    qa, _ = quantize64(x)
+    sa = (x.float().abs().amax(1) / 127.0).masked_fill(x.abs().amax(1) == 0, 1.0)
+    p = product64(qa.cuda(), sa.cuda(), codes.cuda(), scale.cuda()).cpu()
+    assert_within(got, *finish64(p, bias, epilogue, resid, 0.5))
+
+
+def _norm64(x, w, b, swish=0):
+    """LayerNorm (and Swish) in 64 bits, and how far a float32 evaluation may be.  With u = 2^-24: the mean is a tree of at
+    most 24 additions deep, so it is within 24 u mean|x|, and mean|x| rstd <= sqrt(1 + mean^2 / var), below 1.1 for
+    these rows; rstd is good to 15 u; the affine map adds three roundings: |dv| <= |g| (27 u + 15 u |xhat|) + 3 u (|v| + |h|),
+    which is below 2^-19 (|g| + |g xhat| + |h|).  Swish: slope at most 1.1, and 2^-16 of the value (tests/i8_tools.py)."""
+    x, w, b = x.double(), w.double(), b.double()
+    hat = (x - x.mean(1, keepdim=True)) / torch.sqrt(x.var(1, unbiased=False, keepdim=True) + 1e-5)
+    v, off = hat * w + b, 2.0 ** -19 * (w.abs() + (hat * w).abs() + b.abs())
+    return (v * torch.sigmoid(v), 1.1 * off + 2.0 ** -16 * v.abs()) if swish else (v, off)
+
+
+@pytest.mark.parametrize("rows,d,swish", [(9, 512, 0), (130, 1024, 0), (6, 4096, 1), (5, 2048, 1), (3, 256, 0), (1, 1024, 0)])
+def test_layernorm_i8(rows, d, swish):
+    """Scales and codes against the 64-bit rows: a scale within the rows' bound / 127 (and its own rounding), a code within
+    half a step of 127 v / max|v|, plus what the bound on v is worth in steps, plus 2^-16 for the kernel's two roundings of the
+    quotient (127 * 2^-23)."""
+    g = torch.Generator().manual_seed(rows + d)
+    x = (torch.randn((rows, d), generator=g) * 3 + 0.5).cuda()
+    if rows > 1:
+        x[1] = 0.25                                   # a constant row: normalises to the bias, exactly
+    w1, b1, w2, b2 = (torch.randn((d,), generator=g).cuda() for _ in range(4))
+    L, st = H.lib(), H.current_stream_ptr()
+    xa = x.clone()
+    q = torch.full((rows, d), 99, dtype=torch.int8, device="cuda")
+    s = torch.zeros((rows,), device="cuda")
+
+    def check(v, off):
+        top = s.double()[:, None] * 127
+        assert ((top[:, 0] - v.abs().amax(1)).abs() <= off.amax(1) + 2.0 ** -22 * top[:, 0]).all()
+        assert ((q.double() - 127 * v / top).abs() <= 0.5 + 127 * off / top + 2.0 ** -16).all()
+        assert int(q.abs().max()) == 127
+
+    H.check(L.oasr_layernorm_i8(xa.data_ptr(), w1.data_ptr(), b1.data_ptr(), q.data_ptr(), s.data_ptr(), rows, d, 1e-5, swish, st))
+    torch.cuda.synchronize()
+    assert torch.equal(xa, x)
+    check(*_norm64(x, w1, b1, swish))
+    if not swish:
+        H.check(L.oasr_layernorm2_i8(xa.data_ptr(), w1.data_ptr(), b1.data_ptr(), w2.data_ptr(), b2.data_ptr(), q.data_ptr(),
+                                     s.data_ptr(), rows, d, 1e-5, st))
+        torch.cuda.synchronize()
+        v, off = _norm64(x, w1, b1)
+        assert ((xa.double() - v).abs() <= off).all()
+        check(*_norm64(xa, w2, b2))
+
+
+@pytest.mark.parametrize("m,k,epilogue", [(1, 512, "bias"), (77, 1024, "swish"), (301, 2048, "residual")])
+def test_normed_linear(m, k, epilogue):
+    """LayerNorm in 64 bits against the call: a row's normalised values differ by float32 roundings, so a code may fall on
+    the other side of a tie; the chance per value is about 2^-23 * 127 * a few, so at most a handful of the row's k codes do
+    (allowed: 4), each moving an output by one step of x times one weight."""
+    g = torch.Generator().manual_seed(m + k)
+    x = torch.randn((m, k), generator=g) * 2 + 0.3
+    gain, shift = 1 + 0.2 * torch.randn((k,), generator=g), 0.2 * torch.randn((k,), generator=g)
+    codes, scale = weight_codes(96, k, g)
+    bias = torch.randn((96,), generator=g)
+    resid = torch.randn((m, 96), generator=g) if epilogue == "residual" else None
+    layer = ops.LinearI8.from_codes(codes.cuda(), scale.cuda(), bias.cuda())
+    got = layer.normed(x.cuda(), gain.cuda(), shift.cuda(), epilogue=epilogue, alpha=2.0,
+                       resid=None if resid is None else resid.cuda())
+    x64 = x.double()
+    y = (x64 - x64.mean(1, keepdim=True)) / torch.sqrt(x64.var(1, unbiased=False, keepdim=True) + 1e-5) * gain.double() + shift.double()
+    qa, sa = quantize64(y)
+    p = product64(qa, sa, codes, scale)
+    want, bound = finish64(p, bias, epilogue, resid, 2.0)
+    step = 4 * sa[:, None] * 128 * scale.double()[None, :] + 2.0 ** -20 * p.abs()      # and the float32 scale of the row
+    assert_within(got, want, bound + 2.2 * step)
+
+
+def test_quantised_weight_constructor_and_leading_dimensions():
+    g = torch.Generator().manual_seed(5)
+    w, x = torch.randn((40, 96), generator=g) / 10, torch.randn((2, 3, 96), generator=g).to(torch.bfloat16)
+    layer = ops.LinearI8(w.cuda())
+    codes, scale = quantize_rows_i8(w)
+    got = layer(x.cuda(), epilogue="float")
+    assert got.shape == (2, 3, 40) and torch.equal(layer.scale.cpu(), scale)
+    assert torch.equal(got, ops.LinearI8.from_codes(codes.cuda(), scale.cuda())(x.cuda(), epilogue="float"))
+    assert torch.equal(layer(x[0, 0].cuda(), epilogue="float"), got[0, 0])
+    assert layer(x[:0].cuda()).shape == (0, 3, 40) and layer(x.cuda()[:, :0]).shape == (2, 0, 40)
+    # the quantised layer is close to the float one: two quantisations, each within half a step of its row's maximum
+    exact = x.double() @ w.double().t()
+    bound = 96 * (x.double().abs().amax(-1, keepdim=True) * w.double().abs().amax(1)) * (1 / 127)
+    assert ((got.double().cpu() - exact).abs() <= bound).all()
+
+
+def test_strided_rows_in_and_out_and_untouched_surroundings():
+    g = torch.Generator().manual_seed(6)
+    for n, k, pad in ((70, 100, 5), (96, 128, 32), (33, 65, 1)):
+        m = 37
+        codes, scale = weight_codes(n, k, g)
+        layer = ops.LinearI8.from_codes(codes.cuda(), scale.cuda(), torch.randn((n,), generator=g).cuda())
+        x = torch.randn((m, k + pad), generator=g).to(torch.bfloat16).cuda()
+        dense = layer(x[:, :k].contiguous())
+        assert torch.equal(layer(x[:, :k]), dense)
+        for dtype, epi in ((torch.bfloat16, "bias"), (torch.float32, "float"), (torch.float32, "residual")):
+            buf = torch.full((m + 2, n + pad), 7.0, dtype=dtype, device="cuda")
+            view = buf[1:-1, :n]
+            want = layer(x[:, :k], epilogue=epi, resid=torch.full((m, n), 7.0, device="cuda") if epi == "residual" else None)
+            layer(x[:, :k], epilogue=epi, resid=view if epi == "residual" else None, out=view)
+            assert torch.equal(view, want)
+            if epi == "residual":        # a residual with a pitch of its own
+                assert torch.equal(layer(x[:, :k], epilogue=epi, resid=torch.full((m, n + 3), 7.0, device="cuda")[:, :n]), want)
+            assert (buf[0] == 7).all() and (buf[-1] == 7).all() and (buf[:, n:] == 7).all()
+        # codes with a pitch of their own
+        wide = torch.full((n, k + pad), 55, dtype=torch.int8, device="cuda")
+        wide[:, :k] = codes.cuda()
+        assert torch.equal(ops.LinearI8.from_codes(wide[:, :k], scale.cuda(), layer.bias)(x[:, :k]), dense)
+
+
+def test_every_row_is_its_own_whatever_the_batch():
+    """A token's result does not depend on the rows around it, nor on which kernel its batch size selects: bit for bit."""
+    g = torch.Generator().manual_seed(8)
+    for n, k in ((512, 1024), (777, 1000), (1024, 4096)):
+        codes, scale = weight_codes(n, k, g)
+        layer = ops.LinearI8.from_codes(codes.cuda(), scale.cuda(), torch.randn((n,), generator=g).cuda())
+        x = torch.randn((3000, k), generator=g).to(torch.bfloat16).cuda()
+        for epi in ("bias", "swish", "float"):
+            full = layer(x, epilogue=epi)
+            for m in (1, 2, 7, 16, 31, 64, 100, 129, 300, 513, 1500):
+                assert torch.equal(layer(x[1000: 1000 + m], epilogue=epi), full[1000: 1000 + m]), (n, k, epi, m)
+
+
+def test_largest_sums_are_exact():
+    """k = 131072 with codes -128 and 127 alternating in sign: the sums reach 2^31 - 2^24 and come back exact to float32."""
+    k = 131072
+    x = torch.ones((3, k), dtype=torch.bfloat16, device="cuda")
+    x[1] = -1
+    codes = torch.full((32, k), -128, dtype=torch.int8, device="cuda")
+    codes[1] = 127
+    layer = ops.LinearI8.from_codes(codes, torch.ones((32,), device="cuda"))
+    got = layer(x, epilogue="float").double().cpu()
+    assert (got[0, 0], got[1, 0]) == (-128.0 * k, 128.0 * k)
+    assert abs(got[0, 1] - 127.0 * k) <= 2 ** -22 * 127 * k
+    with pytest.raises(ValueError, match="131072"):
+        ops.LinearI8.from_codes(torch.zeros((1, k + 1), dtype=torch.int8, device="cuda"), torch.ones((1,), device="cuda"))
+
+
+def test_offsets_past_32_bits():
+    m, n, k = 66000, 33000, 64
+    g = torch.Generator().manual_seed(9)
+    codes, scale = weight_codes(n, k, g)
+    layer = ops.LinearI8.from_codes(codes.cuda(), scale.cuda())
+    x = torch.randn((m, k), generator=g).to(torch.bfloat16).cuda()
+    out = layer(x)
+    assert out.numel() > 1 << 31
+    for lo in (0, 40000, m - 300):
+        assert torch.equal(out[lo: lo + 300], layer(x[lo: lo + 300]))
+    del out
+    far = torch.zeros(((1 << 26) * 40,), dtype=torch.bfloat16, device="cuda").view(40, 1 << 26)[:, :k]
+    far.copy_(x[:40])
+    assert torch.equal(layer(far), layer(x[:40]))
+
+
+def test_refusals_on_the_device():
+    g = torch.Generator().manual_seed(10)
+    codes, scale = weight_codes(48, 64, g)
+    c, s = codes.cuda(), scale.cuda()
+    layer = ops.LinearI8.from_codes(c, s)
+    x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    y = x.clone()
+    z = torch.zeros((5, 48), device="cuda")
+    bad = [
+        (lambda: layer(x[:, :63]), "64 columns"), (lambda: layer(x.float()), "bfloat16"), (lambda: layer(x, epilogue="gelu"), "epilogue"),
+        (lambda: layer(x, epilogue="glu"), "multiple of 32"), (lambda: layer(x, epilogue="residual"), "resid"),
+        (lambda: layer(x, resid=torch.zeros((4, 48), device="cuda")), "resid"),
+        (lambda: layer(x, epilogue="residual", resid=torch.zeros((4, 47), device="cuda")), "resid"),
+        (lambda: layer(x, out=torch.zeros((4, 47), dtype=torch.bfloat16, device="cuda")), "shape"),
+        (lambda: layer(x, out=torch.zeros((4, 48), device="cuda")), "bfloat16"),
+        (lambda: layer(x, out=torch.zeros((48, 4), dtype=torch.bfloat16, device="cuda").t()), "contiguous rows"),
+        (lambda: layer(y, out=y[:, :48]), "overlap x"),
+        (lambda: layer(x, epilogue="residual", resid=z[:4], out=z[1:]), "resid may be out"),
+        (lambda: layer(x.t()[:, :1].expand(64, 64)[:4]), "contiguous rows"),
+        (lambda: layer(torch.zeros((1, 64), dtype=torch.bfloat16, device="cuda").expand(4, 64)), "overlap"),
+        (lambda: layer.normed(x.float(), s, s), "normed"), (lambda: layer.normed(x, s, s), "float32"),
+        (lambda: ops.LinearI8.from_codes(c, s[:4]), "scale"), (lambda: ops.LinearI8.from_codes(c, None), "scale"),
+        (lambda: ops.LinearI8.from_codes(c, s, s.double()), "bias"), (lambda: ops.LinearI8.from_codes(c.t(), s), "contiguous rows"),
+    ]
+    for call, text in bad:
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_streams_and_repeated_graph_replays():
+    """Captured calls on one layer, replayed between eager calls of the same layer on another stream: each equals its eager
+    result (the workspaces belong to the calls)."""
+    g = torch.Generator().manual_seed(11)
+    codes, scale = weight_codes(512, 1024, g)
+    layer = ops.LinearI8.from_codes(codes.cuda(), scale.cuda(), torch.randn((512,), generator=g).cuda())
+    gain, shift = torch.ones((1024,), device="cuda"), torch.zeros((1024,), device="cuda")
+    for m in (1, 60, 700):
+        x = torch.randn((m, 1024), generator=g).to(torch.bfloat16).cuda()
+        other = torch.randn((m, 1024), generator=g).to(torch.bfloat16).cuda()
+        resid = torch.randn((m, 512), generator=g).cuda()
+        call = lambda t: (layer(t), layer(t, epilogue="residual", resid=resid), layer.normed(t.float(), gain, shift))  # noqa: E731
+        side = torch.cuda.Stream()
+        want_x, want_other = call(x), call(other)
+        torch.cuda.synchronize()
+        buf = x.clone()
+        graphs = []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = call(buf)
+            graphs.append((graph, out))
+        for rep in range(4):
+            src, want = ((x, want_x), (other, want_other))[rep & 1]
+            buf.copy_(src)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                eager = call(other)
+            for graph, out in graphs:
+                graph.replay()
+            torch.cuda.synchronize()
+            for graph, out in graphs:
+                assert all(torch.equal(a, b) for a, b in zip(out, want))
+            assert all(torch.equal(a, b) for a, b in zip(eager, want_other))

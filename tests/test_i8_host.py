@@ -1,0 +1,91 @@
+"""Refusals of the 8-bit integer operators, made before anything is launched (no GPU needed), and the host-side quantiser."""
+
+import pytest
+import torch
+
+from omnilingual_asr import _hip, ops
+from omnilingual_asr.weights import quantize_rows_i8
+from tests.i8_tools import quantize64
+
+A = 1 << 20        # a plausible, aligned address: every call below is refused before it would be used
+
+
+def _gemm(**kw):
+    d = dict(a=A, lda=64, w=A, sa=A, sw=A, bias=None, resid=None, ldr=64, c=A, ldc=64, m=4, n=64, k=64, alpha=1.0, epi=0)
+    d.update(kw)
+    return _hip.lib().oasr_gemm_i8(d["a"], d["lda"], d["w"], d["sa"], d["sw"], d["bias"], d["resid"], d["ldr"], d["c"], d["ldc"],
+                                   d["m"], d["n"], d["k"], d["alpha"], d["epi"], None)
+
+
+def _linear(**kw):
+    d = dict(x=A, ldx=64, w=A, sw=A, bias=None, resid=None, ldr=64, c=A, ldc=64, m=4, n=64, k=64, alpha=1.0, epi=0, ws=A, bytes=1 << 20)
+    d.update(kw)
+    return _hip.lib().oasr_linear_i8(d["x"], d["ldx"], d["w"], d["sw"], d["bias"], d["resid"], d["ldr"], d["c"], d["ldc"], d["m"],
+                                     d["n"], d["k"], d["alpha"], d["epi"], d["ws"], d["bytes"], None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(n=0), "positive"), (dict(k=0), "positive"), (dict(m=-1), "positive"), (dict(k=131073, lda=131136), "131072"),
+    (dict(epi=5), "epilogue"), (dict(epi=-1), "epilogue"), (dict(epi=2, n=48), "multiple of 32"), (dict(ldc=63), "ldc"),
+    (dict(epi=3, resid=A, ldr=63), "ldr"), (dict(w=None), "null"), (dict(sw=None), "null"), (dict(c=None), "null"), (dict(epi=3), "resid"), (dict(w=A + 8), "aligned"),
+    (dict(c=A + 1), "aligned"), (dict(epi=4, c=A + 2), "aligned"), (dict(m=1 << 31), "2^31"),
+])
+def test_product_refusals(kw, text):
+    for call, name in ((_gemm, "gemm_i8"), (_linear, "linear_i8")):
+        assert call(**kw) == -1
+        msg = _hip.lib().oasr_last_error().decode()
+        assert name in msg and text in msg, msg
+
+
+def test_operand_refusals():
+    L = _hip.lib()
+    assert _gemm(lda=48) == -1 and b"lda" in L.oasr_last_error()
+    assert _gemm(lda=72) == -1 and _gemm(k=65) == -1 and _gemm(a=None) == -1 and _gemm(a=A + 8) == -1 and _gemm(sa=None) == -1
+    assert _linear(ldx=63) == -1 and b"ldx" in L.oasr_last_error()
+    assert _linear(x=None) == -1 and _linear(ws=None) == -1 and _linear(ws=A + 16) == -1 and _linear(x=A + 1) == -1
+    need = L.oasr_linear_i8_workspace_bytes(4, 64)
+    assert need == 512 and _linear(bytes=need - 1) == -2 and b"workspace" in L.oasr_last_error()
+    assert _gemm(m=0, a=None, w=None, c=None) == 0 and _linear(m=0, x=None, ws=None) == 0     # nothing to do
+    q = lambda x=A, ldx=64, rows=4, k=64, y=A, ldy=64, s=A: L.oasr_quant_i8_rows(x, ldx, rows, k, y, ldy, s, None)
+    assert q(ldx=63) == -1 and q(ldy=56) == -1 and q(k=65, ldx=65) == -1 and q(k=0) == -1 and q(rows=-1) == -1
+    assert q(x=None) == -1 and q(y=A + 8) == -1 and q(s=A + 2) == -1 and q(rows=0, x=None) == 0
+    ln = lambda x=A, d=512, rows=4, y=A: L.oasr_layernorm_i8(x, A, A, y, A, rows, d, 1e-5, 0, None)
+    assert ln(d=160) == -1 and b"unsupported width" in L.oasr_last_error()
+    assert ln(x=None) == -1 and ln(x=A + 4) == -1 and ln(y=A + 4) == -1 and ln(rows=-1) == -1 and ln(rows=0) == 0
+    assert L.oasr_layernorm2_i8(A, A, A, None, A, A, A, 4, 512, 1e-5, None) == -1
+    pack = lambda w=A, ldw=64, n=16, k=64, out=2 * A: L.oasr_gemm_pack_w_i8(w, ldw, n, k, out, None)
+    assert pack(w=None) == -1 and pack(out=A) == -1 and pack(ldw=63) == -1 and pack(n=0) == -1 and pack(out=2 * A + 8) == -1
+    assert pack(k=131073, ldw=131073) == -1
+
+
+def test_packed_bytes():
+    f = _hip.lib().oasr_gemm_i8_packed_bytes
+    assert f(1, 1) == 1024 and f(16, 64) == 1024 and f(17, 64) == 2048 and f(16, 65) == 2048 and f(0, 4) == 0 and f(4, -1) == 0
+
+
+def test_tensor_refusals_without_a_device():
+    w, x = torch.zeros((32, 64)), torch.zeros((3, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="HIP device"):
+        ops.LinearI8(w)
+    with pytest.raises(ValueError, match="float tensor"):
+        ops.LinearI8(w.to(torch.int8))
+    with pytest.raises(ValueError, match=r"\[out, in\]"):
+        ops.LinearI8.from_codes(torch.zeros((4,), dtype=torch.int8), torch.ones((4,)))
+    with pytest.raises(ValueError, match="int8"):
+        ops.LinearI8.from_codes(w, torch.ones((32,)))
+    layer = ops.LinearI8.__new__(ops.LinearI8)
+    layer.device, layer.in_features, layer.out_features = torch.device("cpu"), 64, 32
+    with pytest.raises(ValueError, match="HIP device"):
+        layer(x)
+    with pytest.raises(ValueError, match="bfloat16"):
+        layer(x.float())
+
+
+def test_host_quantiser_is_the_definition():
+    g = torch.Generator().manual_seed(3)
+    w = torch.randn((37, 129), generator=g)
+    w[5] = 0
+    codes, scale = quantize_rows_i8(w)
+    want, s = quantize64(w)
+    assert codes.dtype == torch.int8 and torch.equal(codes.double(), want) and torch.equal(scale, s.float())
+    assert scale[5] == 1.0 and int(codes.abs().max()) == 127
