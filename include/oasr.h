@@ -509,6 +509,34 @@ int oasr_pcm_to_mono_f32(const void* pcm, int64_t frames, int32_t channels, int3
 int oasr_gather_chunks(const float* pcm, int64_t pcm_len, const int64_t* start, const int32_t* len, int32_t batch,
                        int64_t width, float* out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Token scores: how sure an answer is.  No counterpart in the reference (its remote model returns text only,
+ * ref:src/omnilingual_asr/models/inference/gemini_pipeline.py:512-530).
+ *
+ * For every row of logits z[0 .. vocab-1] (rows `ld` elements apart, OASR_F32 or OASR_BF16, any alignment):
+ *   logprobs[r][i] = log softmax(z)[tokens[r][i]]; a token below 0 means none (0), one at or past vocab gives NaN
+ *   entropy[r]     = -sum p log p, natural units; may be NULL
+ *   ids, best [r][0 .. top-1] = the likeliest tokens and their log probabilities, best first, ties to the lower index
+ * float32 results, sums in float32.  A logit of -inf is a token ruled out: probability 0, never among the likeliest (id -1,
+ * log probability -inf where fewer than `top` remain).  A row that allows nothing: log probabilities -inf, entropy 0, no
+ * likeliest.  A NaN or +inf in a row: NaN results, ids -1.  top 0 .. 32, given (tokens per row) and rows may be 0.
+ * workspace: device, oasr_token_scores_workspace_bytes(rows, vocab, top) bytes (0 for most sizes), 256-byte aligned,
+ * contents on entry do not matter; calls that may overlap need one each. */
+typedef enum oasr_dtype { OASR_F32 = 0, OASR_BF16 = 1 } oasr_dtype;
+
+int64_t oasr_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
+int oasr_token_scores(const void* logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab, const int32_t* tokens,
+                      int32_t given, float* logprobs, float* entropy, int32_t top, int32_t* ids, float* best,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same for the tokens a CTC decode emitted: tokens, frames int32 [batch][width] as oasr_ctc_greedy writes them (-1 past
+ * an utterance's count), logits [batch * t_pad][ld].  Result (b, i) is tokens[b][i] under logits row b * t_pad +
+ * frames[b][i]; where the token or the frame is negative: log probability 0, entropy 0, no likeliest; a frame at or past
+ * t_pad gives NaN.  workspace: as above for rows = batch * width. */
+int oasr_ctc_token_scores(const void* logits, int32_t dtype, int64_t ld, int32_t vocab, int32_t batch, int64_t t_pad,
+                          const int32_t* tokens, const int32_t* frames, int64_t width, float* logprobs, float* entropy,
+                          int32_t top, int32_t* ids, float* best, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

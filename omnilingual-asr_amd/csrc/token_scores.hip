@@ -1,0 +1,569 @@
+// Log probabilities of given tokens under rows of logits, the rows' entropies and their k likeliest tokens, one pass over
+// the logits.  For a row z with reference m (its maximum when the pass ends):
+//   S = sum exp(z - m),  T = sum exp(z - m) (m - z):   log p(t) = (z_t - m) - log S,   entropy = log S + T / S
+// (every term of T is >= 0, so the entropy loses nothing by cancellation; natural units).  S, T and m are float32.
+// Partial results over different references join by f = exp(m' - m): S = S + f S', T = T + f (T' + (m - m') S').
+//
+// What is masked: -inf has probability 0 and is never among the likeliest (id -1, log p -inf where fewer than k tokens
+// remain); a row that allows nothing gives log p = -inf, entropy 0; the lowest finite value is a value like any other.
+// A NaN or +inf anywhere makes S NaN, and the row's results NaN with ids -1.
+// Ties go to the lower index: candidates are ranked by (value, index), never by the order in which they were found.
+//
+// Bandwidth-bound for rows that number in the hundreds (2 or 4 bytes per logit against about ten issue slots), bound by
+// latency below.  Rows up to 1024 tokens stay in the registers of a group of lanes; longer ones are streamed by a
+// work-group each, or by several where rows are few, whose results a second launch joins.
+#include "oasr_common.h"
+
+namespace oasr {
+namespace scores {
+
+constexpr float kLowest = -3.402823466e38f;       // the lowest finite float32
+constexpr float kLargest = 3.402823466e38f;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMaxTop = 32;
+constexpr int kMaxSplits = 64;
+constexpr int kCandidates = 512;                  // kept in LDS per row before ranking
+
+struct Args {
+    const void* logits;
+    int64_t ld, rows;           // rows of results
+    int vocab, given, top;
+    const int32_t* tokens;      // [rows][given]
+    const int32_t* frames;      // null: result row r reads logits row r; else row (r / width) * frames_per + frames[r]
+    int64_t width, frames_per;
+    float* logprobs;            // [rows][given]
+    float* entropy;             // [rows]
+    int32_t* ids;               // [rows][top]
+    float* best;                // [rows][top]
+    int splits;                 // work-groups per row
+    float* part;                // [rows][splits][4]: m, S, T
+    uint2* cand;                // [rows][splits][top]: (ordered value, index), best first
+};
+
+// The order of float values as the order of unsigned integers; -0 equals 0.
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t b = __float_as_uint(f + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+    return __uint_as_float(u ^ ((u >> 31) ? 0x80000000u : 0xffffffffu));
+}
+constexpr uint32_t kOrderedLowest = 0x00800000u;  // ordered(kLowest): -inf lies below
+
+__device__ __forceinline__ bool before(uint32_t va, uint32_t ia, uint32_t vb, uint32_t ib) { return va > vb || (va == vb && ia < ib); }
+
+// 16 bytes of logits from any element's address.
+template <typename E>
+struct Chunk;
+template <>
+struct Chunk<float> {
+    static constexpr int N = 4;
+    struct __attribute__((packed, aligned(4))) Raw {
+        float v[4];
+    };
+    static __device__ __forceinline__ void load(const float* p, float (&z)[4]) {
+        const Raw r = *reinterpret_cast<const Raw*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = r.v[e];
+    }
+    static __device__ __forceinline__ float one(const float* p) { return *p; }
+};
+template <>
+struct Chunk<uint16_t> {
+    static constexpr int N = 8;
+    struct __attribute__((packed, aligned(2))) Raw {
+        uint32_t v[4];
+    };
+    static __device__ __forceinline__ void load(const uint16_t* p, float (&z)[8]) {
+        const Raw r = *reinterpret_cast<const Raw*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            z[2 * e] = __uint_as_float(r.v[e] << 16);
+            z[2 * e + 1] = __uint_as_float(r.v[e] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ float one(const uint16_t* p) { return bf2f(*p); }
+};
+
+// Where result row r reads its logits: >= 0 the logits row, -1 absent (no token here), -2 a frame that does not exist.
+__device__ __forceinline__ int64_t source_row(const Args& p, int64_t r) {
+    if (!p.frames) return r;
+    const int32_t f = p.frames[r];
+    if (p.tokens[r] < 0 || f < 0) return -1;
+    return f < p.frames_per ? r / p.width * p.frames_per + f : -2;
+}
+
+__device__ __forceinline__ float nan32() { return __uint_as_float(0x7fc00000u); }
+
+// One given token's log probability.
+template <typename E>
+__device__ __forceinline__ float token_logprob(const E* row, int vocab, int32_t token, float m, float s, float log_s) {
+    if (token < 0) return 0.f;                        // no token given here
+    if (token >= vocab || s != s) return nan32();
+    if (s == 0.f) return -INFINITY;
+    return (Chunk<E>::one(row + token) - m) - log_s;
+}
+
+__device__ __forceinline__ float row_entropy(float s, float t, float log_s) { return s == 0.f ? 0.f : log_s + t / s; }
+
+// One of the likeliest: rank `at` of row r.
+__device__ __forceinline__ void write_best(const Args& p, int64_t r, int at, uint32_t value, uint32_t index, float m, float log_s) {
+    p.ids[r * p.top + at] = (int32_t)index;
+    p.best[r * p.top + at] = (unordered(value) - m) - log_s;
+}
+__device__ __forceinline__ void write_none(const Args& p, int64_t r, int at, float value) {
+    p.ids[r * p.top + at] = -1;
+    p.best[r * p.top + at] = value;
+}
+
+// ---- short rows: a group of 2^g lanes holds a row in registers, C chunks of four per lane -----------------------------
+template <typename E, int C>
+__global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, int lanes_log2) {
+    const int lane = threadIdx.x & 63, group = 1 << lanes_log2, sub = lane & (group - 1);
+    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t r = (wave << (6 - lanes_log2)) + (lane >> lanes_log2);
+    const bool live = r < p.rows;
+    const int64_t src = live ? source_row(p, r) : -1;
+    const E* row = reinterpret_cast<const E*>(p.logits) + (src < 0 ? 0 : src) * p.ld;
+    float z[4 * C];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int at = 4 * (sub + c * group) + e;
+            z[4 * c + e] = src >= 0 && at < p.vocab ? Chunk<E>::one(row + at) : -INFINITY;
+        }
+    float m = kLowest;
+#pragma unroll
+    for (int j = 0; j < 4 * C; ++j) m = fmaxf(m, z[j]);
+    for (int o = group >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4 * C; ++j) {
+        const float d = fminf(m - z[j], kLargest), e = __builtin_amdgcn_exp2f(d * -kLog2e);
+        // a NaN must survive the minimum
+        s += z[j] == z[j] && m < INFINITY ? e : nan32();
+        t = fmaf(e, d, t);
+    }
+    for (int o = group >> 1; o > 0; o >>= 1) {
+        s += __shfl_xor(s, o, 64);
+        t += __shfl_xor(t, o, 64);
+    }
+    const float log_s = logf(s);
+    if (live && p.given > 0)
+        for (int i = sub; i < p.given; i += group) {
+            float v = 0.f;
+            if (src >= 0) v = token_logprob(row, p.vocab, p.tokens[r * p.given + i], m, s, log_s);
+            if (src == -2) v = nan32();
+            p.logprobs[r * p.given + i] = v;
+        }
+    if (live && p.entropy && sub == 0) p.entropy[r] = src >= 0 ? row_entropy(s, t, log_s) : (src == -2 ? nan32() : 0.f);
+    const bool usable = src >= 0 && s == s;
+    uint32_t taken = 0;                               // this lane's values that are out already
+    for (int k = 0; k < p.top; ++k) {
+        uint32_t v = 0, idx = 0xffffffffu;
+#pragma unroll
+        for (int j = 0; j < 4 * C; ++j) {
+            const uint32_t u = ordered(z[j]), at = 4 * (sub + (j >> 2) * group) + (j & 3);
+            if (!(taken >> j & 1) && u >= kOrderedLowest && before(u, at, v, idx)) {
+                v = u;
+                idx = at;
+            }
+        }
+        for (int o = group >> 1; o > 0; o >>= 1) {
+            const uint32_t ov = __shfl_xor(v, o, 64), oi = __shfl_xor(idx, o, 64);
+            if (before(ov, oi, v, idx)) {
+                v = ov;
+                idx = oi;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4 * C; ++j)
+            if (idx == 4 * (sub + (j >> 2) * group) + (j & 3)) taken |= 1u << j;
+        if (live && sub == 0) {
+            if (usable && v) write_best(p, r, k, v, idx, m, log_s);
+            else write_none(p, r, k, src == -1 || usable ? -INFINITY : nan32());
+        }
+    }
+}
+
+// ---- long rows --------------------------------------------------------------------------------------------------------
+// A wave's running sums: the reference m is shared by the wave, so that it rises rarely and rescaling costs little.
+struct Sums {
+    float m, s, t;
+};
+
+template <int N>
+__device__ __forceinline__ void add_values(Sums& a, float& top, const float (&z)[N]) {
+    float b = z[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) b = fmaxf(b, z[j]);
+    top = fmaxf(top, b);
+    if (__any(b > a.m)) {
+        const float m = fmaxf(a.m, wave_max(b));
+        const float d = fminf(m - a.m, kLargest), f = __builtin_amdgcn_exp2f(d * -kLog2e);
+        a.t = f > 0.f ? f * fmaf(d, a.s, a.t) : 0.f * a.s;     // NaN stays NaN
+        a.s *= f;
+        a.m = m;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float x = a.m - z[j], e = __builtin_amdgcn_exp2f(x * -kLog2e);
+        a.s += e;
+        a.t = fmaf(e, fminf(x, kLargest), a.t);
+    }
+}
+
+// Joins sums over another reference.
+__device__ __forceinline__ void join(Sums& a, const Sums& b) {
+    const float m = fmaxf(a.m, b.m);
+    auto onto = [&](const Sums& x, float& s, float& t) {
+        const float d = fminf(m - x.m, kLargest), f = __builtin_amdgcn_exp2f(d * -kLog2e);
+        s = f * x.s;
+        t = f > 0.f ? f * fmaf(d, x.s, x.t) : 0.f * x.s;
+    };
+    float s0, t0, s1, t1;
+    onto(a, s0, t0);
+    onto(b, s1, t1);
+    a = {m, s0 + s1, t0 + t1};
+}
+
+// The largest value that at least `count` lanes of the wave reach.
+__device__ __forceinline__ uint32_t wave_nth_largest(uint32_t v, int count) {
+    uint32_t at = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = at | 1u << bit;
+        if (__popcll(__ballot(v >= trial)) >= count) at = trial;
+    }
+    return at;
+}
+
+template <typename E, int T, bool SPLIT>
+__global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
+    constexpr int N = Chunk<E>::N, W = T / 64, U = 16 / N;      // U chunks = 16 values per lane and step
+    __shared__ Sums wave_sums[W];
+    __shared__ uint32_t wave_bound[W], found;
+    __shared__ uint2 cand[kCandidates];
+    __shared__ uint2 wave_pick[W];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t r = SPLIT ? blockIdx.x / p.splits : blockIdx.x;
+    const int split = SPLIT ? blockIdx.x % p.splits : 0;
+    const int64_t src = source_row(p, r);
+    if (src < 0) {                                              // uniform: nothing to read
+        if (split == 0) {
+            const float nothing = src == -2 ? nan32() : 0.f;
+            for (int i = tid; i < p.given; i += T) p.logprobs[r * p.given + i] = nothing;
+            if (tid == 0 && p.entropy) p.entropy[r] = nothing;
+            if (tid < p.top) write_none(p, r, tid, src == -2 ? nan32() : -INFINITY);
+        }
+        return;
+    }
+    const E* row = reinterpret_cast<const E*>(p.logits) + src * p.ld;
+    // this work-group's chunks, and for the last split the values behind the last whole chunk
+    const int chunks = p.vocab / N;
+    const int lo = SPLIT ? (int)((int64_t)chunks * split / p.splits) : 0;
+    const int hi = SPLIT ? (int)((int64_t)chunks * (split + 1) / p.splits) : chunks;
+    const int tail = !SPLIT || split == p.splits - 1 ? p.vocab - chunks * N : 0;
+
+    Sums a = {kLowest, 0.f, 0.f};
+    float top = -INFINITY;
+    int base = lo;
+    for (; base + U * T <= hi; base += U * T) {
+        float z[16];
+#pragma unroll
+        for (int u = 0; u < U; ++u) Chunk<E>::load(row + (int64_t)(base + u * T + tid) * N, *reinterpret_cast<float(*)[N]>(&z[u * N]));
+        add_values(a, top, z);
+    }
+    for (; base < hi; base += T) {
+        float z[N];
+        if (base + tid < hi) {
+            Chunk<E>::load(row + (int64_t)(base + tid) * N, z);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) z[e] = -INFINITY;
+        }
+        add_values(a, top, z);
+    }
+    {
+        const float z[1] = {tid < tail ? Chunk<E>::one(row + (int64_t)chunks * N + tid) : -INFINITY};
+        add_values(a, top, z);
+    }
+    a.s = wave_sum(a.s);
+    a.t = wave_sum(a.t);
+    // A bound that at least `top` values reach: the least over the waves of each wave's ceil(top / W)-th largest lane.
+    const uint32_t mine = ordered(top);
+    const uint32_t reach = p.top > 0 ? wave_nth_largest(mine, (p.top + W - 1) / W) : 0;
+    if (lane == 0) {
+        wave_sums[wave] = a;
+        wave_bound[wave] = reach;
+    }
+    if (tid == 0) found = 0;
+    __syncthreads();
+    a = wave_sums[0];
+    uint32_t bound = wave_bound[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+        join(a, wave_sums[w]);
+        bound = bound < wave_bound[w] ? bound : wave_bound[w];
+    }
+    bound = bound > kOrderedLowest ? bound : kOrderedLowest;
+    const float log_s = logf(a.s);
+    if (SPLIT) {
+        if (tid == 0) {
+            float* o = p.part + (r * p.splits + split) * 4;
+            o[0] = a.m;
+            o[1] = a.s;
+            o[2] = a.t;
+        }
+    } else {
+        for (int i = tid; i < p.given; i += T)
+            p.logprobs[r * p.given + i] = token_logprob(row, p.vocab, p.tokens[r * p.given + i], a.m, a.s, log_s);
+        if (tid == 0 && p.entropy) p.entropy[r] = row_entropy(a.s, a.t, log_s);
+    }
+    if (p.top == 0) return;
+    uint2* const list = SPLIT ? p.cand + (r * p.splits + split) * p.top : nullptr;
+    auto emit = [&](int at, uint32_t v, uint32_t i) {
+        if (SPLIT) list[at] = make_uint2(v, i);
+        else write_best(p, r, at, v, i, a.m, log_s);
+    };
+    auto emit_none = [&](int at) {
+        if (SPLIT) list[at] = make_uint2(0, 0xffffffffu);
+        else write_none(p, r, at, a.s != a.s ? nan32() : -INFINITY);
+    };
+    if (a.s != a.s) {                                           // uniform
+        if (tid < p.top) emit_none(tid);
+        return;
+    }
+    // Every value at or above the bound becomes a candidate; only lanes whose own largest reaches it read again.
+    auto offer = [&](float z, uint32_t index) {
+        const uint32_t u = ordered(z);
+        if (u >= bound) {
+            const uint32_t at = atomicAdd(&found, 1u);
+            if (at < kCandidates) cand[at] = make_uint2(u, index);
+        }
+    };
+    if (mine >= bound) {
+        for (int c = lo + tid; c < hi; c += T) {
+            float z[N];
+            Chunk<E>::load(row + (int64_t)c * N, z);
+#pragma unroll
+            for (int e = 0; e < N; ++e) offer(z[e], (uint32_t)c * N + e);
+        }
+        if (tid < tail) offer(Chunk<E>::one(row + (int64_t)chunks * N + tid), (uint32_t)chunks * N + tid);
+    }
+    __syncthreads();
+    const int n = (int)found;
+    if (n <= kCandidates) {
+        for (int c = tid; c < n; c += T) {
+            const uint2 me = cand[c];
+            int rank = 0;
+            for (int o = 0; o < n; ++o) rank += before(cand[o].x, cand[o].y, me.x, me.y);
+            if (rank < p.top) emit(rank, me.x, me.y);
+        }
+        for (int k = n + tid; k < p.top; k += T) emit_none(k);
+        return;
+    }
+    // Too many values reach the bound (long runs of equal ones): the next in order, one after the other.
+    uint2 last = make_uint2(0xffffffffu, 0u);
+    for (int k = 0; k < p.top; ++k) {
+        uint32_t v = 0, idx = 0xffffffffu;
+        auto look = [&](float z, uint32_t index) {
+            const uint32_t u = ordered(z);
+            if (u >= kOrderedLowest && before(last.x, last.y, u, index) && before(u, index, v, idx)) {
+                v = u;
+                idx = index;
+            }
+        };
+        for (int c = lo + tid; c < hi; c += T) {
+            float z[N];
+            Chunk<E>::load(row + (int64_t)c * N, z);
+#pragma unroll
+            for (int e = 0; e < N; ++e) look(z[e], (uint32_t)c * N + e);
+        }
+        if (tid < tail) look(Chunk<E>::one(row + (int64_t)chunks * N + tid), (uint32_t)chunks * N + tid);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint32_t ov = __shfl_xor(v, o, 64), oi = __shfl_xor(idx, o, 64);
+            if (before(ov, oi, v, idx)) {
+                v = ov;
+                idx = oi;
+            }
+        }
+        if (lane == 0) wave_pick[wave] = make_uint2(v, idx);
+        __syncthreads();
+        last = wave_pick[0];
+        for (int w = 1; w < W; ++w)
+            if (before(wave_pick[w].x, wave_pick[w].y, last.x, last.y)) last = wave_pick[w];
+        __syncthreads();                                        // picked before the next round writes
+        if (tid == 0) {
+            if (last.x) emit(k, last.x, last.y);
+            else emit_none(k);
+        }
+        if (!last.x) last = make_uint2(0, 0xffffffffu);
+    }
+}
+
+// Joins the splits of a row: one wave per row, lane s holds split s and the head of its list.
+template <typename E>
+__global__ __launch_bounds__(64) void token_scores_join_kernel(const Args p) {
+    const int lane = threadIdx.x;
+    const int64_t r = blockIdx.x, src = source_row(p, r);
+    if (src < 0) return;                                        // written by the first split
+    const E* row = reinterpret_cast<const E*>(p.logits) + src * p.ld;
+    Sums a = {kLowest, 0.f, 0.f};
+    if (lane < p.splits) {
+        const float* o = p.part + (r * p.splits + lane) * 4;
+        a = {o[0], o[1], o[2]};
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const Sums b = {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)};
+        join(a, b);
+    }
+    const float log_s = logf(a.s);
+    for (int i = lane; i < p.given; i += 64)
+        p.logprobs[r * p.given + i] = token_logprob(row, p.vocab, p.tokens[r * p.given + i], a.m, a.s, log_s);
+    if (lane == 0 && p.entropy) p.entropy[r] = row_entropy(a.s, a.t, log_s);
+    if (p.top == 0) return;
+    if (a.s != a.s) {
+        if (lane < p.top) write_none(p, r, lane, nan32());
+        return;
+    }
+    const uint2* list = p.cand + (r * p.splits + (lane < p.splits ? lane : 0)) * p.top;
+    int at = 0;
+    uint2 head = lane < p.splits ? list[0] : make_uint2(0, 0xffffffffu);
+    for (int k = 0; k < p.top; ++k) {
+        uint32_t v = head.x, idx = head.y;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint32_t ov = __shfl_xor(v, o, 64), oi = __shfl_xor(idx, o, 64);
+            if (before(ov, oi, v, idx)) {
+                v = ov;
+                idx = oi;
+            }
+        }
+        if (lane == 0) {
+            if (v) write_best(p, r, k, v, idx, a.m, log_s);
+            else write_none(p, r, k, -INFINITY);
+        }
+        if (v && head.x == v && head.y == idx) {                // the winner's next
+            ++at;
+            head = at < p.top ? list[at] : make_uint2(0, 0xffffffffu);
+        }
+    }
+}
+
+// Work-groups per row: rows that fill the chip by themselves are not cut; a part has at least 4096 tokens.
+static int splits_for(int64_t rows, int64_t vocab) {
+    if (vocab <= 1024 || rows >= 256) return 1;
+    int64_t s = 512 / rows;
+    if (s > vocab / 4096) s = vocab / 4096;
+    if (s > kMaxSplits) s = kMaxSplits;
+    return s < 1 ? 1 : (int)s;
+}
+
+static int64_t workspace_bytes(int64_t rows, int64_t vocab, int64_t top) {
+    if (rows <= 0 || vocab <= 0 || top < 0) return 0;
+    const int64_t s = splits_for(rows, vocab);
+    return s == 1 ? 0 : round_up(rows * s * 16, 256) + rows * s * top * 8;
+}
+
+template <typename E>
+static void launch(const Args& p, hipStream_t st) {
+    if (p.vocab <= 1024) {
+        int g = 0;
+        while (g < 6 && (4 << g) < p.vocab) ++g;
+        const int64_t per_wg = (int64_t)4 << (6 - g);
+        const dim3 grid((unsigned)((p.rows + per_wg - 1) / per_wg)), blk(256);
+        if (p.vocab <= 256) hipLaunchKernelGGL((token_scores_short_kernel<E, 1>), grid, blk, 0, st, p, g);
+        else if (p.vocab <= 512) hipLaunchKernelGGL((token_scores_short_kernel<E, 2>), grid, blk, 0, st, p, g);
+        else hipLaunchKernelGGL((token_scores_short_kernel<E, 4>), grid, blk, 0, st, p, g);
+    } else if (p.splits > 1) {
+        hipLaunchKernelGGL((token_scores_long_kernel<E, 256, true>), dim3((unsigned)(p.rows * p.splits)), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((token_scores_join_kernel<E>), dim3((unsigned)p.rows), dim3(64), 0, st, p);
+    } else {
+        hipLaunchKernelGGL((token_scores_long_kernel<E, 256, false>), dim3((unsigned)p.rows), dim3(256), 0, st, p);
+    }
+}
+
+static int run(const char* what, Args& p, int32_t dtype, void* workspace, int64_t bytes, hipStream_t st) {
+    OASR_REQUIRE(dtype == OASR_F32 || dtype == OASR_BF16, "%s: dtype must be OASR_F32 or OASR_BF16", what);
+    OASR_REQUIRE(p.rows >= 0 && p.rows < ((int64_t)1 << 31) / kMaxSplits, "%s: rows must lie in [0, 2^25)", what);
+    OASR_REQUIRE(p.vocab > 0 && p.vocab < (1 << 30), "%s: vocab must lie in [1, 2^30)", what);
+    OASR_REQUIRE(p.ld >= p.vocab, "%s: ld=%lld does not cover the vocabulary", what, (long long)p.ld);
+    OASR_REQUIRE(p.given >= 0, "%s: the count of given tokens is negative", what);
+    OASR_REQUIRE(p.top >= 0 && p.top <= kMaxTop, "%s: top must lie in [0, %d]", what, kMaxTop);
+    if (p.rows == 0) return OASR_OK;
+    OASR_REQUIRE(p.logits && (p.given == 0 || (p.tokens && p.logprobs)) && (p.top == 0 || (p.ids && p.best)), "%s: null pointer", what);
+    const uintptr_t words = (uintptr_t)p.tokens | (uintptr_t)p.frames | (uintptr_t)p.logprobs | (uintptr_t)p.entropy | (uintptr_t)p.ids |
+                            (uintptr_t)p.best;
+    OASR_REQUIRE(((uintptr_t)p.logits & (dtype == OASR_F32 ? 3 : 1)) == 0 && (words & 3) == 0, "%s: misaligned pointer", what);
+    p.splits = splits_for(p.rows, p.vocab);
+    const int64_t need = workspace_bytes(p.rows, p.vocab, p.top);
+    if (need > 0) {
+        if (bytes < need) {
+            set_error("%s: workspace needs %lld bytes, got %lld", what, (long long)need, (long long)bytes);
+            return OASR_ECAPACITY;
+        }
+        OASR_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0, "%s: workspace missing or not 256-byte aligned", what);
+        p.part = static_cast<float*>(workspace);
+        p.cand = reinterpret_cast<uint2*>(static_cast<char*>(workspace) + round_up(p.rows * p.splits * 16, 256));
+    }
+    if (dtype == OASR_F32) launch<float>(p, st);
+    else launch<uint16_t>(p, st);
+    OASR_CHECK_LAUNCH(what);
+    return OASR_OK;
+}
+
+}  // namespace scores
+}  // namespace oasr
+
+using namespace oasr;
+
+extern "C" {
+
+int64_t oasr_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int32_t top) { return scores::workspace_bytes(rows, vocab, top); }
+
+int oasr_token_scores(const void* logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab, const int32_t* tokens,
+                      int32_t given, float* logprobs, float* entropy, int32_t top, int32_t* ids, float* best, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+    scores::Args p = {};
+    p.logits = logits;
+    p.ld = ld;
+    p.rows = rows;
+    p.vocab = vocab;
+    p.given = given;
+    p.top = top;
+    p.tokens = tokens;
+    p.logprobs = logprobs;
+    p.entropy = entropy;
+    p.ids = ids;
+    p.best = best;
+    return scores::run("token_scores", p, dtype, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int oasr_ctc_token_scores(const void* logits, int32_t dtype, int64_t ld, int32_t vocab, int32_t batch, int64_t t_pad,
+                          const int32_t* tokens, const int32_t* frames, int64_t width, float* logprobs, float* entropy,
+                          int32_t top, int32_t* ids, float* best, void* workspace, int64_t workspace_bytes, void* stream) {
+    OASR_REQUIRE(batch >= 0 && t_pad > 0 && width >= 0 && width < ((int64_t)1 << 31), "ctc_token_scores: bad batch, t_pad or width");
+    if (batch == 0 || width == 0) return OASR_OK;
+    OASR_REQUIRE(frames && tokens && logprobs, "ctc_token_scores: null pointer");
+    scores::Args p = {};
+    p.logits = logits;
+    p.ld = ld;
+    p.rows = batch * width;
+    p.vocab = vocab;
+    p.given = 1;
+    p.top = top;
+    p.tokens = tokens;
+    p.frames = frames;
+    p.width = width;
+    p.frames_per = t_pad;
+    p.logprobs = logprobs;
+    p.entropy = entropy;
+    p.ids = ids;
+    p.best = best;
+    return scores::run("ctc_token_scores", p, dtype, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@ _lib = None
 c_i32, c_i64, c_f32, c_f64, c_vp = C.c_int32, C.c_int64, C.c_float, C.c_double, C.c_void_p
 
 EPI_BIAS_BF16, EPI_BIAS_SWISH_BF16, EPI_GLU_BF16, EPI_RESIDUAL_F32, EPI_BIAS_F32 = range(5)
+F32, BF16 = 0, 1                                         # oasr_dtype
 GEMM_W_PACKED, GEMM_A_PACKED, GEMM_C_PACKED = 1, 2, 4    # layout flags of oasr_gemm_bf16_ex
 
 
@@ -137,6 +138,10 @@ _SIGNATURES = {
     "oasr_ctc_static_max_frames": (c_i64, []),
     "oasr_ctc_greedy_static": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_i32, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp]),
     "oasr_ctc_greedy": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_i32, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "oasr_token_scores_workspace_bytes": (c_i64, [c_i64, c_i64, c_i32]),
+    "oasr_token_scores": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "oasr_ctc_token_scores": (c_i32, [c_vp, c_i32, c_i64, c_i32, c_i32, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp,
+                                      c_vp, c_i64, c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -9,6 +9,8 @@ No counterpart in the reference, whose projections and answers are made by a rem
 from __future__ import annotations
 
 import contextlib
+import math
+from typing import NamedTuple
 
 import torch
 
@@ -32,10 +34,10 @@ def _rows(t, what: str, dtype):
         raise ValueError(f"{what} must be a {dtype} tensor")
     if not t.is_cuda:
         raise ValueError(f"{what} must be on a HIP device; there is no CPU fallback")
-    if t.dim() < 1:
-        raise ValueError(f"{what} must have at least one dimension")
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{what} must have at least one column")
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1]) if t.dim() > 2 else t[None, :]
+        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
     rows, cols = t.shape
     pitch = t.stride(0) if rows > 1 else cols
     if cols > 1 and t.stride(1) != 1 or pitch < cols:
@@ -176,3 +178,89 @@ class LinearI8:
                                       None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m,
                                       self.out_features, k, alpha, epi, st), "oasr_gemm_i8")
         return out
+
+
+MAX_ALTERNATIVES = 32
+
+
+class TokenScores(NamedTuple):
+    """What `token_scores` returns; float32 (ids int32) on the logits' device, natural logarithms."""
+    logprobs: torch.Tensor      # of the given tokens
+    entropy: torch.Tensor       # of each row's distribution
+    ids: torch.Tensor           # [..., alternatives]: the likeliest tokens, best first, -1 where there are fewer
+    best: torch.Tensor          # [..., alternatives]: their log probabilities
+
+
+def _int32(t, shape, what: str, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != shape or t.device != device:
+        raise ValueError(f"{what} must be an int32 tensor of shape {tuple(shape)} on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _score_outputs(lead, given, alternatives, device):
+    if not 0 <= alternatives <= MAX_ALTERNATIVES:
+        raise ValueError(f"alternatives must lie in [0, {MAX_ALTERNATIVES}]")
+    f32 = lambda shape: torch.empty(shape, dtype=torch.float32, device=device)  # noqa: E731
+    return TokenScores(f32(given), f32(lead), torch.empty((*lead, alternatives), dtype=torch.int32, device=device),
+                       f32((*lead, alternatives)))
+
+
+def _score_workspace(rows, vocab, alternatives, device):
+    n = int(_hip.lib().oasr_token_scores_workspace_bytes(rows, vocab, alternatives))
+    return n, torch.empty((n,), dtype=torch.uint8, device=device) if n else None
+
+
+def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, alternatives: int = 0) -> TokenScores:
+    """Log probabilities of given tokens under rows of logits [..., vocab] (float32 or bfloat16; rows evenly spaced), with
+    every row's entropy and its `alternatives` likeliest tokens.  `tokens`: int32 [...] or [..., n]; a negative one means
+    none (0).  Masked logits (-inf) have probability 0 and are no alternatives; include/oasr.h says what else rows hold."""
+    z, rows, vocab, ld = _rows(logits, "logits", (torch.float32, torch.bfloat16))
+    lead, device = logits.shape[:-1], logits.device
+    given, n = (*lead, 0), 0
+    if tokens is not None:
+        given = tokens.shape if isinstance(tokens, torch.Tensor) else ()
+        if given != lead and given[:-1] != lead:
+            raise ValueError(f"tokens must be of shape {tuple(lead)} or {tuple(lead)} and one more dimension")
+        tokens, n = _int32(tokens, given, "tokens", device), 1 if given == lead else given[-1]
+    out = _score_outputs(lead, given, alternatives, device)
+    if rows == 0:
+        return out
+    with _on(device):
+        ws_bytes, ws = _score_workspace(rows, vocab, alternatives, device)
+        _hip.check(_hip.lib().oasr_token_scores(
+            z.data_ptr(), _hip.F32 if z.dtype == torch.float32 else _hip.BF16, ld, rows, vocab,
+            None if tokens is None else tokens.data_ptr(), n, out.logprobs.data_ptr(), out.entropy.data_ptr(), alternatives,
+            out.ids.data_ptr(), out.best.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes,
+            _hip.current_stream_ptr()), "oasr_token_scores")
+    return out
+
+
+def ctc_token_scores(logits: torch.Tensor, tokens: torch.Tensor, frames: torch.Tensor, *, vocab: int | None = None,
+                     alternatives: int = 0) -> TokenScores:
+    """The same for the tokens a CTC decode emitted: logits [batch, frames, pitch] of which the first `vocab` columns count
+    (all by default), tokens and frames int32 [batch, n] as `HipEngine.decode` returns them (-1 past an utterance's
+    count: log probability 0, entropy 0, no alternatives)."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 3 or not logits.is_contiguous():
+        raise ValueError("logits must be a contiguous tensor [batch, frames, pitch]")
+    batch, t_pad, ld = logits.shape
+    _rows(logits, "logits", (torch.float32, torch.bfloat16))
+    vocab = ld if vocab is None else int(vocab)
+    if not 1 <= vocab <= ld:
+        raise ValueError(f"vocab must lie in [1, {ld}]")
+    if not isinstance(tokens, torch.Tensor) or tokens.dim() != 2 or tokens.shape[0] != batch:
+        raise ValueError("tokens must be [batch, n]")
+    device, shape = logits.device, tokens.shape
+    tokens, frames = _int32(tokens, shape, "tokens", device), _int32(frames, shape, "frames", device)
+    if t_pad == 0 and tokens.numel():
+        raise ValueError("logits have no frames")
+    out = _score_outputs(shape, shape, alternatives, device)
+    if tokens.numel() == 0:
+        return out
+    with _on(device):
+        ws_bytes, ws = _score_workspace(tokens.numel(), vocab, alternatives, device)
+        _hip.check(_hip.lib().oasr_ctc_token_scores(
+            logits.data_ptr(), _hip.F32 if logits.dtype == torch.float32 else _hip.BF16, ld, vocab, batch, t_pad,
+            tokens.data_ptr(), frames.data_ptr(), shape[1], out.logprobs.data_ptr(), out.entropy.data_ptr(), alternatives,
+            out.ids.data_ptr(), out.best.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes,
+            _hip.current_stream_ptr()), "oasr_ctc_token_scores")
+    return out
