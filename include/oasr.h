@@ -188,6 +188,23 @@ typedef struct oasr_layer_fp8_weights {
     const uint8_t* ffn2_w2_q; const float* ffn2_w2_s;
 } oasr_layer_fp8_weights;
 int oasr_encoder_set_fp8(oasr_encoder* enc, const oasr_layer_fp8_weights* layers);
+/* The same for 8-bit integers: q = int8 codes packed by oasr_gemm_pack_w_i8 (rows as above; codes = weight / s), s = float32
+ * scale per output row (max|row| / 127).  After this call the LayerNorms that feed a projection write int8 rows and their
+ * scales (oasr_layernorm_i8), the other projection inputs are quantised per row (oasr_quant_i8_rows), and every large
+ * projection is oasr_gemm_i8.  Call before oasr_encoder_workspace_bytes.  Passing NULL returns to bf16.  An encoder has
+ * e4m3 weights or int8 weights, not both: the second call of the two kinds is refused. */
+typedef struct oasr_layer_int8_weights {
+    const int8_t* ffn1_w1_q; const float* ffn1_w1_s;
+    const int8_t* ffn1_w2_q; const float* ffn1_w2_s;
+    const int8_t* wqkv_q;    const float* wqkv_s;
+    const int8_t* wo_q;      const float* wo_s;
+    const int8_t* pw1_q;     const float* pw1_s;
+    const int8_t* pw2_q;     const float* pw2_s;
+    const int8_t* ffn2_w1_q; const float* ffn2_w1_s;
+    const int8_t* ffn2_w2_q; const float* ffn2_w2_s;
+} oasr_layer_int8_weights;
+int oasr_encoder_set_int8(oasr_encoder* enc, const oasr_layer_int8_weights* layers);
+
 /* Declares that every bf16 projection matrix handed to oasr_encoder_create (fp_w and the eight per layer:
  * ffn1_w1, ffn1_w2, wqkv, wo, pw1, pw2, ffn2_w1, ffn2_w2) is in the packed layout of oasr_gemm_pack_w_bf16
  * (packed != 0) or row-major (0, the default); with fp8 weights set, the same holds for their e4m3 matrices

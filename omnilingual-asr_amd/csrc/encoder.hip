@@ -10,7 +10,8 @@ struct oasr_encoder {
     oasr_encoder_config cfg;
     oasr_top_weights top;
     std::vector<oasr_layer_weights> layers;
-    std::vector<oasr_layer_fp8_weights> fp8;   // empty: bf16 projections
+    std::vector<oasr_layer_fp8_weights> fp8;   // both empty: bf16 projections
+    std::vector<oasr_layer_int8_weights> int8;
     bool packed_w = false;                      // bf16 projection matrices in the layout of oasr_gemm_pack_w_bf16
 };
 
@@ -23,12 +24,24 @@ struct Workspace {
     uint16_t* big;  // [rows][max(ffn, 3d)]  FFN hidden / fused qkv / padded features
     uint16_t* ctx;  // [rows][d]      attention context / GLU output
     float* tmp;     // [rows][d]      depthwise-conv output
-    uint8_t* a8;    // [rows][max(ffn, d)]  e4m3 copy of the projection input (fp8 mode only)
+    uint8_t* a8;    // [rows][max(ffn, d)]  e4m3 or int8 copy of the projection input (8-bit modes only)
     float* sa;      // [rows]               its row scales
     int64_t bytes;
 };
 
-static Workspace carve(const oasr_encoder_config& c, int64_t rows, char* base, bool fp8) {
+// A layer's 8-bit matrices and scales, whichever of the two kinds they are.
+struct EightBit {
+    const void *ffn1_w1_q, *ffn1_w2_q, *wqkv_q, *wo_q, *pw1_q, *pw2_q, *ffn2_w1_q, *ffn2_w2_q;
+    const float *ffn1_w1_s, *ffn1_w2_s, *wqkv_s, *wo_s, *pw1_s, *pw2_s, *ffn2_w1_s, *ffn2_w2_s;
+};
+
+template <typename T>
+static EightBit eight_bit(const T& w) {
+    return {w.ffn1_w1_q, w.ffn1_w2_q, w.wqkv_q, w.wo_q, w.pw1_q, w.pw2_q, w.ffn2_w1_q, w.ffn2_w2_q,
+            w.ffn1_w1_s, w.ffn1_w2_s, w.wqkv_s, w.wo_s, w.pw1_s, w.pw2_s, w.ffn2_w1_s, w.ffn2_w2_s};
+}
+
+static Workspace carve(const oasr_encoder_config& c, int64_t rows, char* base, bool eight) {
     Workspace w;
     const int64_t wide = c.ffn_dim > 3 * c.d_model ? c.ffn_dim : 3 * c.d_model;
     int64_t off = 0;
@@ -43,7 +56,7 @@ static Workspace carve(const oasr_encoder_config& c, int64_t rows, char* base, b
     w.tmp = reinterpret_cast<float*>(take(rows * c.d_model * 4));
     w.a8 = nullptr;
     w.sa = nullptr;
-    if (fp8) {
+    if (eight) {
         w.a8 = reinterpret_cast<uint8_t*>(take(rows * (c.ffn_dim > c.d_model ? c.ffn_dim : c.d_model)));
         w.sa = reinterpret_cast<float*>(take(rows * 4));
     }
@@ -95,6 +108,7 @@ int oasr_encoder_set_fp8(oasr_encoder* enc, const oasr_layer_fp8_weights* layers
         enc->fp8.clear();
         return OASR_OK;
     }
+    OASR_REQUIRE(enc->int8.empty(), "encoder_set_fp8: the encoder has int8 weights");
     OASR_REQUIRE(enc->cfg.d_model % 64 == 0 && enc->cfg.ffn_dim % 64 == 0, "encoder_set_fp8: dimensions must be multiples of 64");
     for (int l = 0; l < enc->cfg.n_layers; ++l) {
         const oasr_layer_fp8_weights& w = layers[l];
@@ -104,6 +118,24 @@ int oasr_encoder_set_fp8(oasr_encoder* enc, const oasr_layer_fp8_weights* layers
                      "encoder_set_fp8: layer %d has a null pointer", l);
     }
     enc->fp8.assign(layers, layers + enc->cfg.n_layers);
+    return OASR_OK;
+}
+
+int oasr_encoder_set_int8(oasr_encoder* enc, const oasr_layer_int8_weights* layers) {
+    OASR_REQUIRE(enc, "encoder_set_int8: null handle");
+    if (!layers) {
+        enc->int8.clear();
+        return OASR_OK;
+    }
+    OASR_REQUIRE(enc->fp8.empty(), "encoder_set_int8: the encoder has e4m3 weights");
+    for (int l = 0; l < enc->cfg.n_layers; ++l) {
+        const oasr_layer_int8_weights& w = layers[l];
+        OASR_REQUIRE(w.ffn1_w1_q && w.ffn1_w1_s && w.ffn1_w2_q && w.ffn1_w2_s && w.wqkv_q && w.wqkv_s && w.wo_q &&
+                         w.wo_s && w.pw1_q && w.pw1_s && w.pw2_q && w.pw2_s && w.ffn2_w1_q && w.ffn2_w1_s &&
+                         w.ffn2_w2_q && w.ffn2_w2_s,
+                     "encoder_set_int8: layer %d has a null pointer", l);
+    }
+    enc->int8.assign(layers, layers + enc->cfg.n_layers);
     return OASR_OK;
 }
 
@@ -119,7 +151,7 @@ int64_t oasr_encoder_rows(int32_t batch, int64_t t_pad) { return round_up((int64
 
 int64_t oasr_encoder_workspace_bytes(const oasr_encoder* enc, int32_t batch, int64_t t_pad) {
     if (!enc || batch <= 0 || t_pad <= 0) return 0;
-    return carve(enc->cfg, oasr_encoder_rows(batch, t_pad), nullptr, !enc->fp8.empty()).bytes;
+    return carve(enc->cfg, oasr_encoder_rows(batch, t_pad), nullptr, !enc->fp8.empty() || !enc->int8.empty()).bytes;
 }
 
 int oasr_encoder_forward(const oasr_encoder* enc, const float* feats, const int32_t* lengths,
@@ -131,8 +163,8 @@ int oasr_encoder_forward(const oasr_encoder* enc, const float* feats, const int3
     const oasr_encoder_config& c = enc->cfg;
     const int64_t rows = oasr_encoder_rows(batch, t_pad);
     const int64_t live = (int64_t)batch * t_pad;
-    const bool fp8 = !enc->fp8.empty();
-    Workspace ws = carve(c, rows, reinterpret_cast<char*>(workspace), fp8);
+    const bool fp8 = !enc->fp8.empty(), int8 = !enc->int8.empty(), eight = fp8 || int8;
+    Workspace ws = carve(c, rows, reinterpret_cast<char*>(workspace), eight);
     if (ws.bytes > workspace_bytes) {
         set_error("encoder_forward: workspace needs %lld bytes, got %lld", (long long)ws.bytes,
                   (long long)workspace_bytes);
@@ -152,26 +184,32 @@ int oasr_encoder_forward(const oasr_encoder* enc, const float* feats, const int3
     // The FFN hidden activations go from the up-projection to the down-projection in the packed layout as
     // well (bf16 path): the down-projection has only d / 256 column tiles to share each copy of its A
     // operand, and a packed A makes those copies whole cache lines.
-    const int hid_out = fp8 ? 0 : OASR_GEMM_C_PACKED, hid_in = fp8 ? 0 : OASR_GEMM_A_PACKED;
-    // one large projection: bf16 GEMM, or row quantisation + fp8 GEMM when fp8 weights are set
-    // `a` = nullptr: the operand already sits in ws.a8 / ws.sa (written by a LayerNorm of the fp8 path)
-    auto project = [&](const uint16_t* a, int64_t k, const uint16_t* wb, const uint8_t* wq, const float* wscale,
+    const int hid_out = eight ? 0 : OASR_GEMM_C_PACKED, hid_in = eight ? 0 : OASR_GEMM_A_PACKED;
+    int8_t* const ai = reinterpret_cast<int8_t*>(ws.a8);
+    // one large projection: bf16 GEMM, or row quantisation + 8-bit GEMM when e4m3 or int8 weights are set
+    // `a` = nullptr: the operand already sits in ws.a8 / ws.sa (written by a LayerNorm of an 8-bit path)
+    auto project = [&](const uint16_t* a, int64_t k, const uint16_t* wb, const void* wq, const float* wscale,
                        const float* bias, const float* resid, void* dst, int64_t n, float alpha, int epi,
                        int layout = 0) -> int {
+        if (int8) {
+            if (a) OASR_TRY(oasr_quant_i8_rows(a, k, rows, k, ai, k, ws.sa, stream));
+            return oasr_gemm_i8(ai, k, static_cast<const int8_t*>(wq), ws.sa, wscale, bias, resid, n, dst,
+                                epi == OASR_EPI_GLU_BF16 ? n / 2 : n, rows, n, k, alpha, epi, stream);
+        }
         if (!fp8) return oasr_gemm_bf16_ex(a, wb, bias, resid, dst, rows, n, k, alpha, epi, wflag | layout, stream);
         if (a) OASR_TRY(oasr_quant_fp8_rows(a, rows, k, ws.a8, ws.sa, stream));
-        return (enc->packed_w ? oasr_gemm_fp8_pw : oasr_gemm_fp8)(ws.a8, wq, ws.sa, wscale, bias, resid, dst, rows, n, k, alpha, epi, stream);
+        return (enc->packed_w ? oasr_gemm_fp8_pw : oasr_gemm_fp8)(ws.a8, static_cast<const uint8_t*>(wq), ws.sa, wscale, bias, resid, dst, rows, n, k, alpha, epi, stream);
     };
-    // LayerNorm feeding a projection: bf16 rows in ws.xn, or (fp8 path) e4m3 rows + scales in ws.a8 / ws.sa
+    // LayerNorm feeding a projection: bf16 rows in ws.xn, or (8-bit paths) e4m3 / int8 rows + scales in ws.a8 / ws.sa
     auto norm = [&](const float* src, const float* lw, const float* lb, int64_t nrows, int swish) -> int {
+        if (int8) return oasr_layernorm_i8(src, lw, lb, ai, ws.sa, nrows, d, c.ln_eps, swish, stream);
         if (fp8) return oasr_layernorm_fp8(src, lw, lb, ws.a8, ws.sa, nrows, d, c.ln_eps, swish, stream);
         return oasr_layernorm(src, lw, lb, ws.xn, nrows, d, d, c.ln_eps, 1, swish, stream);
     };
-    const uint16_t* xn = fp8 ? nullptr : ws.xn;
-    static const oasr_layer_fp8_weights kNoFp8 = {};
+    const uint16_t* xn = eight ? nullptr : ws.xn;
     for (int l = 0; l < nl; ++l) {
         const oasr_layer_weights& w = enc->layers[l];
-        const oasr_layer_fp8_weights& q = fp8 ? enc->fp8[l] : kNoFp8;
+        const EightBit q = fp8 ? eight_bit(enc->fp8[l]) : int8 ? eight_bit(enc->int8[l]) : EightBit{};
         if (l == 0) OASR_TRY(norm(x, w.ffn1_ln_w, w.ffn1_ln_b, rows, 0));
         // half-step feed-forward 1
         OASR_TRY(project(xn, d, w.ffn1_w1, q.ffn1_w1_q, q.ffn1_w1_s, w.ffn1_b1, nullptr, ws.big, f, 1.0f,
@@ -209,7 +247,10 @@ int oasr_encoder_forward(const oasr_encoder* enc, const float* feats, const int3
         // block output LayerNorm, fused with the next block's first LayerNorm when there is one
         if (l + 1 < nl) {
             const oasr_layer_weights& nx = enc->layers[l + 1];
-            if (fp8)
+            if (int8)
+                OASR_TRY(oasr_layernorm2_i8(x, w.final_ln_w, w.final_ln_b, nx.ffn1_ln_w, nx.ffn1_ln_b, ai, ws.sa, rows, d,
+                                            c.ln_eps, stream));
+            else if (fp8)
                 OASR_TRY(oasr_layernorm2_fp8(x, w.final_ln_w, w.final_ln_b, nx.ffn1_ln_w, nx.ffn1_ln_b, ws.a8, ws.sa,
                                              rows, d, c.ln_eps, stream));
             else

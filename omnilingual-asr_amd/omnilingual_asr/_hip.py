@@ -51,6 +51,10 @@ class LayerFp8Weights(C.Structure):
     _fields_ = [(n, c_vp) for n in FP8_FIELDS]
 
 
+class LayerInt8Weights(C.Structure):
+    _fields_ = [(n, c_vp) for n in FP8_FIELDS]
+
+
 class TopWeights(C.Structure):
     _fields_ = [(n, c_vp) for n in TOP_FIELDS]
 
@@ -93,6 +97,7 @@ _SIGNATURES = {
     "oasr_gemm_bf16_ex": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_f32, c_i32, c_i32, c_vp]),
     "oasr_encoder_set_packed_weights": (c_i32, [c_vp, c_i32]),
     "oasr_encoder_set_fp8": (c_i32, [c_vp, c_vp]),
+    "oasr_encoder_set_int8": (c_i32, [c_vp, c_vp]),
     "oasr_layernorm_fp8": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_f32, c_i32, c_vp]),
     "oasr_layernorm2_fp8": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_f32, c_vp]),
     "oasr_quant_fp8_rows": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),

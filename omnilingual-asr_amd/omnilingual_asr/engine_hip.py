@@ -13,7 +13,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from . import _hip, tokenizer
+from . import _hip, ops, tokenizer
 from .weights import CTC_LOGIT_PITCH, Geometry, init_random_weights, pack_for_device, resolve_geometry
 
 SAMPLE_RATE = 16000
@@ -26,7 +26,10 @@ def pad_frames(t: int) -> int:
 
 class HipEngine:
     def __init__(self, model="G300", *, weights: dict | None = None, seed: int = 0,
-                 device: int | str | torch.device | None = None, use_graphs: bool = True, fp8: bool = False):
+                 device: int | str | torch.device | None = None, use_graphs: bool = True, fp8: bool = False,
+                 int8: bool = False):
+        if fp8 and int8:
+            raise ValueError("fp8 and int8 exclude each other: the large projections have one kind of 8-bit weights")
         _hip.lib()
         _hip.require_device()
         self.geometry: Geometry = resolve_geometry(model)
@@ -38,7 +41,8 @@ class HipEngine:
         if weights is None:
             weights = init_random_weights(g, seed)
         self.fp8 = bool(fp8)    # e4m3 weights + per-row quantised activations in the eight large projections
-        self._packed = pack_for_device(weights, g, self.device, fp8=self.fp8)   # keeps device buffers alive
+        self.int8 = bool(int8)  # 8-bit integer weights (a scale per output row) and activations (a scale per frame) there
+        self._packed = pack_for_device(weights, g, self.device, fp8=self.fp8, int8=self.int8)   # keeps device buffers alive
         self._pack_gemm_weights()
         self._tables = torch.from_numpy(_hip.logmel_table_blob().view(np.int32)).to(self.device)
         self._handle = self._create_handle()
@@ -76,12 +80,18 @@ class HipEngine:
                            "oasr_gemm_pack_w_fp8")
                 return out
 
+            def packed_i8(w):
+                n, k = w.shape
+                out = torch.empty((int(L.oasr_gemm_i8_packed_bytes(n, k)),), dtype=torch.int8, device=w.device)
+                _hip.check(L.oasr_gemm_pack_w_i8(w.data_ptr(), k, n, k, out.data_ptr(), st), "oasr_gemm_pack_w_i8")
+                return out
+
             self._packed["top"]["fp_w"] = packed(self._packed["top"]["fp_w"])
             for layer in self._packed["layers"]:
                 for name in self.GEMM_WEIGHTS:
                     layer[name] = packed(layer[name])
-                    if self.fp8:
-                        layer[name + "_q"] = packed8(layer[name + "_q"])
+                    if self.fp8 or self.int8:
+                        layer[name + "_q"] = (packed8 if self.fp8 else packed_i8)(layer[name + "_q"])
             if "ctc_w" in self._packed:
                 self._packed["ctc_w"] = packed(self._packed["ctc_w"])
             torch.cuda.synchronize()
@@ -101,12 +111,15 @@ class HipEngine:
                    "oasr_encoder_create")
         _hip.check(_hip.lib().oasr_encoder_set_packed_weights(handle, int(self._packed["gemm_weights_packed"])),
                    "oasr_encoder_set_packed_weights")
-        if self.fp8:
-            q = (_hip.LayerFp8Weights * max(1, g.n_layers))()
+        if self.fp8 or self.int8:
+            q = ((_hip.LayerFp8Weights if self.fp8 else _hip.LayerInt8Weights) * max(1, g.n_layers))()
             for i, L in enumerate(self._packed["layers"]):
                 for k in _hip.FP8_FIELDS:
                     setattr(q[i], k, L[k].data_ptr())
-            _hip.check(_hip.lib().oasr_encoder_set_fp8(handle, q), "oasr_encoder_set_fp8")
+            if self.fp8:
+                _hip.check(_hip.lib().oasr_encoder_set_fp8(handle, q), "oasr_encoder_set_fp8")
+            else:
+                _hip.check(_hip.lib().oasr_encoder_set_int8(handle, q), "oasr_encoder_set_int8")
         return handle
 
     def close(self):
@@ -314,6 +327,18 @@ class HipEngine:
                                      buf["counts"].data_ptr(), buf["ctc_ids"].data_ptr(), st), "oasr_ctc_greedy")
         return buf["tokens"], buf["tok_frames"], buf["counts"]
 
+    def score(self, tokens: torch.Tensor, frames: torch.Tensor, alternatives: int = 0) -> ops.TokenScores:
+        """How sure the last `decode` of this shape was of its tokens (tokens, frames [B, t_pad] as it returned them): per
+        token the log probability under its frame's logits, that frame's entropy and its `alternatives` likeliest symbols,
+        on the device (`ops.ctc_token_scores`).  Reads the logits `decode` left in the engine's buffers, so it belongs
+        behind it on the same stream, before the next batch of this shape."""
+        batch, t_pad = tokens.shape
+        buf = self._buffers.get((batch, t_pad))
+        if buf is None:
+            raise ValueError("score takes the tokens and frames of a decode: [batch, %s] tensors" % t_pad)
+        logits = buf["logits"][: batch * t_pad].view(batch, t_pad, CTC_LOGIT_PITCH)
+        return ops.ctc_token_scores(logits, tokens, frames, vocab=self.geometry.vocab_size, alternatives=alternatives)
+
     def step(self, pcm: torch.Tensor, n_valid: torch.Tensor):
         """One pass of the whole device path over one resident batch (eager launches)."""
         buf = self._get_buffers(pcm.shape[0], pcm.shape[1])
@@ -418,16 +443,21 @@ class HipEngine:
             hidden, lengths = self._run(pcm_d, nv)
             return hidden, lengths.cpu().numpy()
 
-    def transcribe_batch(self, pcm, n_valid):
+    def transcribe_batch(self, pcm, n_valid, alternatives: int | None = None):
         """`encode_batch` plus the CTC stage.  Returns (hidden, lengths, tokens) where tokens is a list
-        of (ids int32 array, frame-index int32 array) per utterance, on the host."""
+        of (ids int32 array, frame-index int32 array) per utterance, on the host.  With `alternatives` given (0 to 32)
+        a fourth item says how sure each token is: per utterance an `ops.TokenScores` of host arrays, one entry per token."""
         with torch.cuda.device(self.device):
             pcm_d, nv = self._upload(pcm, n_valid)
             hidden, lengths = self._run(pcm_d, nv)
             tok, frm, cnt = self.decode(hidden, lengths)
             tok_h, frm_h, cnt_h = tok.cpu().numpy(), frm.cpu().numpy(), cnt.cpu().numpy()
             out = [(tok_h[i, : cnt_h[i]].copy(), frm_h[i, : cnt_h[i]].copy()) for i in range(tok_h.shape[0])]
-            return hidden, lengths.cpu().numpy(), out
+            if alternatives is None:
+                return hidden, lengths.cpu().numpy(), out
+            host = [t.cpu().numpy() for t in self.score(tok, frm, alternatives)]
+            scores = [ops.TokenScores(*(t[i, : cnt_h[i]].copy() for t in host)) for i in range(tok_h.shape[0])]
+            return hidden, lengths.cpu().numpy(), out, scores
 
     # ---- two-deep asynchronous path -------------------------------------------------------------------
     # submit() queues one batch (upload on a copy stream, device path, CTC stage, results to page-locked

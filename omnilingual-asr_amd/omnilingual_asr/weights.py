@@ -151,9 +151,10 @@ def quantize_rows_i8(w: torch.Tensor):
     return codes, amax / 127.0
 
 
-def pack_for_device(weights: dict, g: Geometry, device, fp8: bool = False) -> dict:
+def pack_for_device(weights: dict, g: Geometry, device, fp8: bool = False, int8: bool = False) -> dict:
     """Device tensors in the layout of `oasr_layer_weights` / `oasr_top_weights` (include/oasr.h);
-    with `fp8`, also the e4m3 codes and row scales of `oasr_layer_fp8_weights`."""
+    with `fp8`, also the e4m3 codes and row scales of `oasr_layer_fp8_weights`, with `int8` the int8 codes (row-major
+    still) and row scales of `oasr_layer_int8_weights`."""
     bf = lambda t: t.to(device=device, dtype=torch.bfloat16).contiguous()
     f32 = lambda t: t.to(device=device, dtype=torch.float32).contiguous()
     fp_w = torch.zeros((g.d_model, 192), dtype=torch.float32)
@@ -180,12 +181,12 @@ def pack_for_device(weights: dict, g: Geometry, device, fp8: bool = False) -> di
             P[pfx + "_w2"], P[pfx + "_b2"] = bf(L[pfx + "_w2"]), f32(L[pfx + "_b2"])
         for n in ("ffn1_ln", "attn_ln", "conv_ln", "dw_ln", "ffn2_ln", "final_ln"):
             P[n + "_w"], P[n + "_b"] = f32(L[n + "_w"]), f32(L[n + "_b"])
-        if fp8:
+        if fp8 or int8:
             mats = {"ffn1_w1": L["ffn1_w1"], "ffn1_w2": L["ffn1_w2"], "ffn2_w1": L["ffn2_w1"], "ffn2_w2": L["ffn2_w2"],
                     "wqkv": torch.cat([L["wq"] * q_scale, L["wk"], L["wv"]], dim=0), "wo": L["wo"],
                     "pw1": glu_interleave(L["pw1"]), "pw2": L["pw2"]}
             for name, m in mats.items():
-                codes, scale = quantize_rows_e4m3(m)
+                codes, scale = (quantize_rows_e4m3 if fp8 else quantize_rows_i8)(m)
                 P[name + "_q"], P[name + "_s"] = codes.to(device).contiguous(), f32(scale)
         layers.append(P)
     packed = {"top": top, "layers": layers}

@@ -79,6 +79,8 @@ LAYER_KEYS = (
 # quantised per row and the weight per output row to OCP e4m3 (scale = max|row| / 448), the product
 # is taken on the de-quantised values.  Test infrastructure: set/reset by `forward(..., fp8=True)`.
 _FP8 = False
+# The same for 8-bit integers (scale = max|row| / 127), `forward(..., int8=True)`.
+_INT8 = False
 # When set, tensors are rounded where the device stores them in 16 bits (`forward(..., device_rounding=True)`).
 _DEV = False
 
@@ -106,7 +108,15 @@ def _fake_quant_rows(t):
     return (t / scale).to(torch.float32).to(torch.float8_e4m3fn).to(t.dtype) * scale
 
 
+def _fake_quant_rows_int8(t):
+    amax = t.abs().amax(dim=-1, keepdim=True)
+    top = torch.where(amax > 0, amax, torch.full_like(amax, 127.0))
+    return ((127.0 * t.double() / top).round() * (top / 127.0)).to(t.dtype)
+
+
 def _proj(x, w, b=None):
+    if _INT8:
+        return F.linear(_fake_quant_rows_int8(x), _fake_quant_rows_int8(w.to(x.dtype)), b)
     if _FP8:
         return F.linear(_fake_quant_rows(x), _fake_quant_rows(w.to(x.dtype)), b)
     return F.linear(x, _r(w), b)
@@ -121,7 +131,9 @@ def _ffn(x, w, pfx):
 
 
 def _ln(x, w, b, g):
-    """LayerNorm whose output feeds a projection (bfloat16 rows on the device)."""
+    """LayerNorm whose output feeds a projection (bfloat16 rows on the device; its int8 form quantises the float32 rows)."""
+    if _INT8:
+        return F.layer_norm(x, (x.shape[-1],), w, b, g.ln_eps)
     return _r(F.layer_norm(x, (x.shape[-1],), w, b, g.ln_eps))
 
 
@@ -192,6 +204,8 @@ def conv_module(x, w, g: Geometry):
     yt = F.pad(y.transpose(1, 2), (g.conv_kernel - 1, 0))
     yt = F.conv1d(yt, w["dw"][:, None, :], groups=d)
     y = F.layer_norm(yt.transpose(1, 2), (d,), w["dw_ln_w"], w["dw_ln_b"], g.ln_eps)
+    if _INT8 and d not in (512, 1024, 2048):     # the unfused convolution branch: LayerNorm + Swish straight to int8 rows
+        return _proj(_swish(y), w["pw2"])
     return _proj(_r(_swish(y)), w["pw2"])
 
 
@@ -217,25 +231,26 @@ def input_projection(feats, w, g: Geometry):
 
 @torch.no_grad()
 def forward(feats, lengths, weights: dict, g: Geometry = G300, dtype=torch.float32, per_layer=False, fp8=False,
-            device_rounding=False):
+            device_rounding=False, int8=False):
     """weights: {'fp_ln_w','fp_ln_b','fp_w','fp_b','layers': [ {LAYER_KEYS...} ]}.
     Returns hidden [B, T, d] (and the list of per-layer outputs when per_layer).  `fp8`: the eight large
-    projections of a block on e4m3 operands; `device_rounding`: 16-bit storage roundings as on the device."""
+    projections of a block on e4m3 operands (`int8`: on 8-bit integers); `device_rounding`: 16-bit storage roundings as on the device."""
     cast = lambda t: t.to(dtype)
     if feats.shape[1] == 0:     # audio shorter than two frames: no encoder rows at all
         x = torch.zeros((feats.shape[0], 0, g.d_model), dtype=dtype)
         return (x, [x] * (len(weights["layers"]) + 1)) if per_layer else x
     top = {k: cast(v) for k, v in weights.items() if k != "layers"}
-    global _FP8, _DEV
+    global _FP8, _DEV, _INT8
     _DEV = bool(device_rounding)
     try:
         x = input_projection(cast(feats), top, g)
         outs = [x]
         _FP8 = bool(fp8)
+        _INT8 = bool(int8)
         for lw in weights["layers"]:
             x = block(x, lengths, {k: cast(v) for k, v in lw.items()}, g)
             outs.append(x)
     finally:
-        _FP8 = False
+        _FP8 = _INT8 = False
         _DEV = False
     return (x, outs) if per_layer else x

@@ -304,3 +304,95 @@ def test_streams_and_repeated_graph_replays():
             for graph, out in graphs:
                 assert all(torch.equal(a, b) for a, b in zip(out, want))
             assert all(torch.equal(a, b) for a, b in zip(eager, want_other))
+
+
+def test_encoder_int8_against_the_quantising_oracle():
+    """GTINY (2 blocks), ragged batch, every large projection in 8-bit integers.  What to expect, by arithmetic: rounding to a
+    step max / 127 leaves an rms error of max / (127 sqrt 12); activations reach about 3.7 of their rms (max over 512), the
+    uniform weights sqrt 3: relative errors 0.0084 and 0.0039 per operand, 0.0093 per product, against e4m3's 0.026 per
+    operand and 0.037 per product, whose two blocks end 3.6e-2 from the float32 oracle: int8 should end near 0.9e-2 (bound
+    2e-2).  Two correct implementations end at up to about two thirds of that from one another after two blocks, since values next
+    to a rounding step fall on either side (bound 1.3e-2)."""
+    from omnilingual_asr.engine_hip import HipEngine
+    from omnilingual_asr.weights import GEOMETRIES, init_random_weights
+    from oracle import conformer as OC
+    from oracle import logmel as OL
+    from tests.test_gpu_ops import synth_pcm
+
+    g = GEOMETRIES["GTINY"]
+    og = OC.Geometry(name=g.name, d_model=g.d_model, ffn_dim=g.ffn_dim, n_heads=g.n_heads, n_layers=g.n_layers)
+    w = init_random_weights(g, 21)
+    pcm = synth_pcm(2, 64000, seed=5)
+    n_valid = [64000, 41000]
+    feats, lens = OL.features_batch(pcm.numpy(), n_valid)
+    enc_w = {k: v for k, v in w.items() if not k.startswith("ctc_")}
+    ft, lt = torch.from_numpy(feats), torch.from_numpy(lens)
+    emulated = OC.forward(ft, lt, enc_w, og, int8=True, device_rounding=True)
+    plain = OC.forward(ft, lt, enc_w, og)
+    h8, l8 = HipEngine("GTINY", weights=w, int8=True).encode_batch(pcm, n_valid)
+    h16 = HipEngine("GTINY", weights=w).encode_batch(pcm, n_valid)[0].cpu()
+    h8 = h8.cpu()
+    rel = lambda a, b: float((a - b).norm() / b.norm())  # noqa: E731
+    for i, n in enumerate(lens):
+        assert int(l8[i]) == int(n)
+        print("int8 against emulation %.2e, float32 %.2e" % (rel(h8[i, :n], emulated[i, :n]), rel(h8[i, :n], plain[i, :n])))
+        assert rel(h8[i, :n], emulated[i, :n]) <= 1.3e-2
+        assert rel(h8[i, :n], plain[i, :n]) <= 2e-2
+        assert rel(h8[i, :n], h16[i, :n]) > 2e-3              # and not the bf16 path
+    assert torch.isfinite(h8).all()
+    with pytest.raises(ValueError, match="exclude"):
+        HipEngine("GTINY", weights=w, int8=True, fp8=True)
+
+
+def test_encoder_int8_unfused_convolution_width():
+    """One block at d = 4096 (LayerNorm + Swish of the convolution branch goes straight to int8 rows there)."""
+    import dataclasses
+    from omnilingual_asr.engine_hip import HipEngine
+    from omnilingual_asr.weights import GEOMETRIES, init_random_weights
+    from oracle import conformer as OC
+    from oracle import logmel as OL
+    from tests.test_gpu_ops import synth_pcm
+
+    g = dataclasses.replace(GEOMETRIES["G7B"], n_layers=1, ffn_dim=2048)
+    og = OC.Geometry(name=g.name, d_model=g.d_model, ffn_dim=g.ffn_dim, n_heads=g.n_heads, n_layers=1)
+    w = init_random_weights(g, 31)
+    pcm = synth_pcm(1, 32000, seed=6)
+    feats, lens = OL.features_batch(pcm.numpy(), [32000])
+    enc_w = {k: v for k, v in w.items() if not k.startswith("ctc_")}
+    ft, lt = torch.from_numpy(feats), torch.from_numpy(lens)
+    n = int(lens[0])
+    want = OC.forward(ft, lt, enc_w, og, int8=True, device_rounding=True)[0, :n]
+    got = HipEngine(g, weights=w, int8=True).encode_batch(pcm, [32000])[0][0, :n].cpu()
+    assert float((got - want).norm() / want.norm()) <= 1.3e-2
+
+
+def test_int8_transcription_with_scores():
+    """The whole run as a user makes it: int8 encoder, greedy decode, scores of what was decoded, against 64-bit scores of the
+    engine's own logits; a second batch of the same shape gets its own."""
+    from omnilingual_asr.engine_hip import HipEngine
+    from omnilingual_asr.weights import CTC_LOGIT_PITCH
+    from tests.test_gpu_ops import synth_pcm
+    from tests.test_gpu_token_scores import close, reference
+
+    eng = HipEngine("GTINY", seed=4, int8=True)
+    for seed in (1, 2):
+        pcm = synth_pcm(3, 48000, seed=seed)
+        hidden, lengths, toks = eng.transcribe_batch(pcm, [48000, 20000, 0])
+        hidden2, lengths2, toks2, scores = eng.transcribe_batch(pcm, [48000, 20000, 0], alternatives=3)
+        assert len(scores) == 3 and sum(len(t[0]) for t in toks) > 0
+        t_pad = hidden.shape[1]
+        logits = eng._buffers[(3, t_pad)]["logits"][: 3 * t_pad].view(3, t_pad, CTC_LOGIT_PITCH)[:, :, : eng.geometry.vocab_size].cpu()
+        for b in range(3):
+            ids, frames = toks2[b]
+            assert (ids == toks[b][0]).all() and (frames == toks[b][1]).all()
+            s = scores[b]
+            assert s.logprobs.shape == s.entropy.shape == (len(ids),) and s.ids.shape == s.best.shape == (len(ids), 3)
+            if not len(ids):
+                continue
+            lp, ent, top, best = reference(logits[b, frames], torch.from_numpy(ids)[:, None], 3)
+            close(torch.from_numpy(s.logprobs)[:, None], lp, lambda w: 2.0 ** -17 + 2.0 ** -22 * w.abs())
+            close(torch.from_numpy(s.entropy), ent, lambda w: 2.0 ** -16 * (1 + w))
+            close(torch.from_numpy(s.best), best, lambda w: 2.0 ** -17 + 2.0 ** -22 * w.abs())
+            assert (s.ids == top.numpy()).all() and (s.ids[:, 0] == ids).all()
+    with pytest.raises(ValueError, match="decode"):
+        eng.score(torch.zeros((5, 7), dtype=torch.int32, device="cuda"), torch.zeros((5, 7), dtype=torch.int32, device="cuda"))

@@ -89,3 +89,33 @@ def test_host_quantiser_is_the_definition():
     want, s = quantize64(w)
     assert codes.dtype == torch.int8 and torch.equal(codes.double(), want) and torch.equal(scale, s.float())
     assert scale[5] == 1.0 and int(codes.abs().max()) == 127
+
+
+def test_pipeline_takes_one_kind_of_8_bit_weights():
+    from omnilingual_asr import Pipeline
+    with pytest.raises(ValueError, match="exclude"):
+        Pipeline(fp8=True, int8=True)
+    assert Pipeline(int8=True).gemini._int8
+
+
+def test_encoder_takes_one_kind_of_8_bit_weights():
+    """Handles are host memory: the refusals need no device."""
+    import ctypes as C
+    L = _hip.lib()
+    cfg = _hip.EncoderConfig(160, 512, 1024, 8, 1, 31, 64, 8, 1e-5)
+    handle = C.c_void_p()
+    assert L.oasr_encoder_create(C.byref(cfg), C.byref(_hip.TopWeights()), (_hip.LayerWeights * 1)(), C.byref(handle)) == 0
+    try:
+        full = {k: A for k in _hip.FP8_FIELDS}
+        before = L.oasr_encoder_workspace_bytes(handle, 1, 32)
+        assert L.oasr_encoder_set_int8(None, None) == -1
+        assert L.oasr_encoder_set_int8(handle, (_hip.LayerInt8Weights * 1)()) == -1 and b"layer 0" in L.oasr_last_error()
+        assert L.oasr_encoder_set_int8(handle, (_hip.LayerInt8Weights * 1)(_hip.LayerInt8Weights(**full))) == 0
+        assert L.oasr_encoder_workspace_bytes(handle, 1, 32) > before
+        assert L.oasr_encoder_set_fp8(handle, (_hip.LayerFp8Weights * 1)(_hip.LayerFp8Weights(**full))) == -1
+        assert b"int8" in L.oasr_last_error()
+        assert L.oasr_encoder_set_int8(handle, None) == 0 and L.oasr_encoder_workspace_bytes(handle, 1, 32) == before
+        assert L.oasr_encoder_set_fp8(handle, (_hip.LayerFp8Weights * 1)(_hip.LayerFp8Weights(**full))) == 0
+        assert L.oasr_encoder_set_int8(handle, (_hip.LayerInt8Weights * 1)(_hip.LayerInt8Weights(**full))) == -1
+    finally:
+        L.oasr_encoder_destroy(handle)
