@@ -247,6 +247,131 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmAr
     epilogue<EPI, MT, NT>(p, acc, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
 }
 
+// Large problems: 256 x 256 tiles, eight waves as two groups (the upper and the lower 128 rows) one barrier apart, so that
+// one group reads fragments and issues copies while the other multiplies (32 MFMAs per slice); a wave owns 128 x 64.  The
+// grid is one work-group per CU; each walks its tiles in one continuous pipeline, the next tile's first slices being in
+// flight during the epilogue.  A ring of four slices of 64 k (16 KiB per operand), copied two slices ahead.
+// Work-groups with equal blockIdx % 8 share an XCD (used for locality only): an XCD owns a contiguous range of row tiles and
+// walks it in bands of four column tiles, so that a band's weights stay in that XCD's L2.
+constexpr int kWide = 256, kWideRing = 4, kWideSlice = kWide * kSlice;
+
+template <int EPI>
+__global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int tiles_m, int tiles_n) {
+    __shared__ __attribute__((aligned(1024))) char ring[2 * kWideRing * kWideSlice];      // A slots, then W slots
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 2, wn = wave & 3;
+
+    const int xcd = blockIdx.x & 7, first = blockIdx.x >> 3, stride = gridDim.x >> 3;
+    const int n_tiles = tiles_m * tiles_n;
+    const bool banded = tiles_m >= 16;
+    const int m_lo = (int)((int64_t)tiles_m * xcd / 8), m_cnt = (int)((int64_t)tiles_m * (xcd + 1) / 8) - m_lo;
+    const int flat_lo = (int)((int64_t)n_tiles * xcd / 8);
+    const int local = banded ? m_cnt * tiles_n : (int)((int64_t)n_tiles * (xcd + 1) / 8) - flat_lo;
+    if (first >= local) return;
+    const int mine = (local - first + stride - 1) / stride;
+    auto tile_at = [&](int i, int& tm, int& tn) {
+        const int l = first + i * stride;
+        if (!banded) {
+            tm = (flat_lo + l) / tiles_n;
+            tn = (flat_lo + l) % tiles_n;
+            return;
+        }
+        const int band = l / (m_cnt * 4), width = min(4, tiles_n - 4 * band), in = l - band * m_cnt * 4;
+        tm = m_lo + in / width;
+        tn = 4 * band + in % width;
+    };
+
+    i32x4 acc[8][4];
+    const int nph = p.ks, total = mine * nph;
+    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ ((fr >> 2) & 3)) << 4);
+    // Copies: wave w brings rows 32 w .. 32 w + 31 of both operands' slices, two pieces each.  Rows past the last repeat it.
+    const uint32_t chunk = (uint32_t)(((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+    const char *src_a, *src_w0, *src_w1;
+    uint32_t off0, off1;
+    int st_i = 0, st_t = 0;
+    auto seek = [&](int i) {
+        int tm, tn;
+        tile_at(i, tm, tn);
+        int64_t row = (int64_t)tm * kWide + wave * 32;
+        row = row < p.m ? row : p.m - 1;
+        const int left = (int)min(p.m - 1 - row, (int64_t)31);
+        src_a = reinterpret_cast<const char*>(p.a) + row * p.lda;
+        off0 = (uint32_t)min(lane >> 2, left) * (uint32_t)p.lda + chunk;
+        off1 = (uint32_t)min(16 + (lane >> 2), left) * (uint32_t)p.lda + chunk;
+        const int grp = tn * (kWide / 16) + wave * 2;
+        src_w0 = reinterpret_cast<const char*>(p.w) + (int64_t)min(grp, p.ng - 1) * p.ks * kPiece;
+        src_w1 = reinterpret_cast<const char*>(p.w) + (int64_t)min(grp + 1, p.ng - 1) * p.ks * kPiece;
+    };
+    auto copy_next = [&](int ph) {
+        char* da = ring + (ph & 3) * kWideSlice + wave * 2 * kPiece;
+        char* dw = da + kWideRing * kWideSlice;
+        __builtin_amdgcn_global_load_lds((gbl_void*)(src_a + off0), (lds_void*)da, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gbl_void*)(src_a + off1), (lds_void*)(da + kPiece), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gbl_void*)(src_w0 + (uint32_t)lane * 16), (lds_void*)dw, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gbl_void*)(src_w1 + (uint32_t)lane * 16), (lds_void*)(dw + kPiece), 16, 0, 0);
+        src_a += kSlice;
+        src_w0 += kPiece;
+        src_w1 += kPiece;
+        if (++st_t == nph) {
+            st_t = 0;
+            if (++st_i < mine) seek(st_i);
+        }
+    };
+    seek(0);
+    copy_next(0);
+    if (total > 1) {
+        copy_next(1);
+        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    OASR_I8_BARRIER();
+    if (wm == 1) OASR_I8_BARRIER();          // the second group runs one barrier behind
+
+    int ph = 0;
+    const i32x4 zero = {0, 0, 0, 0};
+    for (int i = 0; i < mine; ++i) {
+        int tm, tn;
+        tile_at(i, tm, tn);
+        for (int t = 0; t < nph; ++t, ++ph) {
+            const char* sa = ring + (ph & 3) * kWideSlice + wm * 8 * kPiece + frag;
+            const char* sw = ring + (kWideRing + (ph & 3)) * kWideSlice + wn * 4 * kPiece + frag;
+            i32x4 wf[4], xf[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wf[j] = *reinterpret_cast<const i32x4*>(sw + j * kPiece);
+#pragma unroll
+            for (int ii = 0; ii < 8; ++ii) xf[ii] = *reinterpret_cast<const i32x4*>(sa + ii * kPiece);
+            if (ph + 2 < total) {
+                copy_next(ph + 2);
+                asm volatile("s_waitcnt vmcnt(4)" ::: "memory");     // own pieces of slice ph + 1 have landed
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            OASR_I8_BARRIER();
+            __builtin_amdgcn_s_setprio(1);
+            if (t == 0) {                    // a tile's first slice accumulates onto zero: no clearing pass
+#pragma unroll
+                for (int ii = 0; ii < 8; ++ii)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[ii][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[ii], zero, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int ii = 0; ii < 8; ++ii)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[ii][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[ii], acc[ii][j], 0, 0, 0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            // the second group holds the barrier that ends a tile's last slice until its epilogue is done, so that the two
+            // groups' epilogues overlap
+            if (!(wm == 1 && t == nph - 1)) OASR_I8_BARRIER();
+        }
+        epilogue<EPI, 8, 4>(p, acc, (int64_t)tm * kWide + wm * 128, (int64_t)tn * kWide + wn * 64, lane);
+        if (wm == 1) OASR_I8_BARRIER();
+    }
+    if (wm == 0) OASR_I8_BARRIER();          // the same number of barriers in both groups
+}
+
 // Per-row quantisation of bf16 rows.  One wavefront per row with the row in registers (k <= 512 NV: NV loads of 16
 // bytes per lane, all issued before the first use), or, for longer rows, in two sweeps of which the second reads from
 // cache.  HBM-bound: 2 bytes in, 1 byte out per element.  Row starts need no alignment; the codes' rows are whole
@@ -359,6 +484,13 @@ static int check_gemm(const char* what, const int8_t* w, const float* scale_w, c
 
 template <int EPI>
 static void launch_tiles(const GemmArgs& p, hipStream_t st) {
+    const int64_t wide_m = (p.m + kWide - 1) / kWide, wide_n = (p.n + kWide - 1) / kWide;
+    // 32 row pitches have to fit the wide kernel's 32-bit offsets
+    if (wide_m * wide_n >= 128 && p.lda < (1 << 26)) {
+        const int grid = (int)(wide_m * wide_n < 256 ? (wide_m * wide_n + 7) / 8 * 8 : 256);
+        hipLaunchKernelGGL((gemm_i8_wide_kernel<EPI>), dim3(grid), dim3(512), 0, st, p, (int)wide_m, (int)wide_n);
+        return;
+    }
     const int64_t tiles_n = (p.n + 127) / 128, tiles = (p.m + 127) / 128 * tiles_n;
     hipLaunchKernelGGL((gemm_i8_tile_kernel<EPI, 2, 2, 4, 4, 4>), dim3((unsigned)tiles), dim3(256), 0, st, p, (int)tiles_n);
 }

@@ -68,7 +68,7 @@ def test_quant_rows_at_the_ends_of_the_range():
 SHAPES = [(1, 1, 1), (1, 33, 64), (1, 1024, 512), (2, 1000, 1000), (3, 64, 65), (15, 96, 63), (16, 128, 128), (17, 130, 640),
           (33, 4096, 256), (64, 512, 4096), (99, 2048, 1024), (127, 257, 191), (128, 128, 64), (129, 384, 320), (200, 777, 1000),
           (256, 256, 64), (300, 96, 16448), (513, 1024, 512), (1000, 4096, 64), (1504, 1024, 1024), (2100, 640, 192),
-          (4096, 512, 512), (8200, 1056, 320)]
+          (4096, 512, 512), (8200, 1056, 320), (2100, 4128, 128), (4500, 2080, 64), (2049, 4097, 65)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
