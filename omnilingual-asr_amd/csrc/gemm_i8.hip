@@ -58,18 +58,38 @@ __device__ __forceinline__ uint32_t cvt_pk_bf16(float a, float b) {
         asm volatile("" ::: "memory");        \
     } while (0)
 
-// Four consecutive entries of a per-column vector, guarded at n.
-__device__ __forceinline__ f32x4 load_cols(const float* __restrict__ p, int64_t col, int64_t n, float missing) {
-    f32x4 v = {missing, missing, missing, missing};
+// Four consecutive entries of a per-column vector, guarded at n unless the tile lies inside the matrix.
+struct __attribute__((packed, aligned(4))) f32x4_any {
+    float v[4];
+};
+
+template <bool FULL>
+__device__ __forceinline__ f32x4 load_cols(const float* __restrict__ p, int64_t col, int64_t n) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (FULL) {
+        const f32x4_any t = *reinterpret_cast<const f32x4_any*>(p + col);
+        v = (f32x4){t.v[0], t.v[1], t.v[2], t.v[3]};
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (p && col + e < n) v[e] = p[col + e];
+        for (int e = 0; e < 4; ++e)
+            if (col + e < n) v[e] = p[col + e];
+    }
     return v;
 }
 
-// Four consecutive outputs, of which the first `count` exist.
-__device__ __forceinline__ void store_f32(float* p, f32x4 v, int64_t count, bool vec) {
-    if (vec && count >= 4) {
+// Four consecutive float32 values of a row, of which the first `count` exist.
+template <bool FULL>
+__device__ __forceinline__ f32x4 load_f32(const float* p, int64_t count) {
+    if (FULL) return *reinterpret_cast<const f32x4*>(p);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < count) v[e] = p[e];
+    return v;
+}
+template <bool FULL>
+__device__ __forceinline__ void store_f32(float* p, f32x4 v, int64_t count) {
+    if (FULL) {
         *reinterpret_cast<f32x4*>(p) = v;
     } else {
 #pragma unroll
@@ -85,8 +105,9 @@ __device__ __forceinline__ void store_bf16(uint16_t* p, u32x2 v, int64_t count) 
 
 // Two neighbouring 16-column tiles of bf16 results, four columns of each per lane: lanes 16 apart trade halves, so
 // that a lane holds eight consecutive columns and a row leaves as 64 consecutive bytes.
-__device__ __forceinline__ void store_bf16_pair(uint16_t* row, int64_t col, u32x2 t0, u32x2 t1, int64_t n, bool vec, int g) {
-    if (vec && col + 32 <= n) {
+template <bool FULL>
+__device__ __forceinline__ void store_bf16_pair(uint16_t* row, int64_t col, u32x2 t0, u32x2 t1, int64_t n, int g) {
+    if (FULL) {
         const auto p = __builtin_amdgcn_permlane16_swap(t0[0], t1[0], false, false);
         const auto q = __builtin_amdgcn_permlane16_swap(t0[1], t1[1], false, false);
         // even lane rows hold tile 0, odd ones tile 1; lane rows 0, 1 its columns 0..7, lane rows 2, 3 columns 8..15
@@ -98,45 +119,49 @@ __device__ __forceinline__ void store_bf16_pair(uint16_t* row, int64_t col, u32x
     }
 }
 
-// A wave's MT x NT tiles of 16 x 16, the first at (m0, n0): scales, bias, epilogue, guarded stores.
-template <int EPI, int MT, int NT>
-__device__ __forceinline__ void epilogue(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane) {
+// A wave's MT x NT tiles of 16 x 16, the first at (m0, n0): scales, bias, epilogue, stores.  FULL: the whole of it lies
+// inside the matrix and rows start on 16-byte boundaries, so nothing is guarded.
+template <int EPI, int MT, int NT, bool FULL>
+__device__ __forceinline__ void epilogue_form(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane) {
     static_assert(NT % 2 == 0, "columns are stored in pairs of tiles");
     const int r = lane & 15, g = lane >> 4;
     f32x4 sw[NT], bv[NT];
+    float sa[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sa[i] = FULL || m0 + 16 * i + r < p.m ? p.scale_a[m0 + 16 * i + r] : 0.f;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        sw[j] = load_cols(p.scale_w, n0 + 16 * j + 4 * g, p.n, 0.f);
-        bv[j] = load_cols(p.bias, n0 + 16 * j + 4 * g, p.n, 0.f);
+        sw[j] = load_cols<FULL>(p.scale_w, n0 + 16 * j + 4 * g, p.n);
+        bv[j] = p.bias ? load_cols<FULL>(p.bias, n0 + 16 * j + 4 * g, p.n) : (f32x4){0.f, 0.f, 0.f, 0.f};
     }
+    constexpr bool kResidual = EPI == OASR_EPI_RESIDUAL_F32;
+    f32x4 now[NT], next[NT];
+    auto load_resid = [&](int i, f32x4 (&x)[NT]) {
+        const int64_t row = m0 + 16 * i + r;
+        if (!FULL && row >= p.m) return;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) x[j] = load_f32<FULL>(p.resid + row * p.ldr + n0 + 16 * j + 4 * g, p.n - (n0 + 16 * j + 4 * g));
+    };
+    if (kResidual) load_resid(0, now);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int64_t row = m0 + 16 * i + r;
-        if (row >= p.m) continue;
-        const float s = p.scale_a[row];
+        if (kResidual && i + 1 < MT) load_resid(i + 1, next);       // requested before this row group's stores
+        if (!FULL && row >= p.m) continue;
         f32x4 o[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] = fmaf((float)acc[i][j][e] * sw[j][e], s, bv[j][e]);   // the weight's scale first: a token's may be as large as float32 goes
-        if (EPI == OASR_EPI_BIAS_F32 || EPI == OASR_EPI_RESIDUAL_F32) {
+            for (int e = 0; e < 4; ++e)      // the weight's scale first: a token's may be as large as float32 goes
+                o[j][e] = fmaf((float)acc[i][j][e] * sw[j][e], sa[i], bv[j][e]);
+        if (EPI == OASR_EPI_BIAS_F32 || kResidual) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int64_t col = n0 + 16 * j + 4 * g, count = p.n - col;
-                if (EPI == OASR_EPI_RESIDUAL_F32) {
-                    const float* from = p.resid + row * p.ldr + col;
-                    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                    if (p.vec && count >= 4) {
-                        x = *reinterpret_cast<const f32x4*>(from);
-                    } else {
+                const int64_t col = n0 + 16 * j + 4 * g;
+                if (kResidual)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < count) x[e] = from[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] = fmaf(p.alpha, o[j][e], x[e]);
-                }
-                store_f32(reinterpret_cast<float*>(p.c) + row * p.ldc + col, o[j], count, p.vec);
+                    for (int e = 0; e < 4; ++e) o[j][e] = fmaf(p.alpha, o[j][e], now[j][e]);
+                store_f32<FULL>(reinterpret_cast<float*>(p.c) + row * p.ldc + col, o[j], p.n - col);
             }
         } else {
             uint16_t* crow = reinterpret_cast<uint16_t*>(p.c) + row * p.ldc;
@@ -154,7 +179,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& p, const i32x4 (&acc)[M
                 } else {
 #pragma unroll
                     for (int q = 0; q + 1 < NT / 2; q += 2)
-                        store_bf16_pair(crow, n0 / 2 + 16 * q, t[q], t[q + 1], p.n / 2, p.vec, g);
+                        store_bf16_pair<FULL>(crow, n0 / 2 + 16 * q, t[q], t[q + 1], p.n / 2, g);
                 }
             } else {
                 u32x2 t[NT];
@@ -166,10 +191,19 @@ __device__ __forceinline__ void epilogue(const GemmArgs& p, const i32x4 (&acc)[M
                     t[j] = (u32x2){cvt_pk_bf16(o[j][0], o[j][1]), cvt_pk_bf16(o[j][2], o[j][3])};
                 }
 #pragma unroll
-                for (int j = 0; j < NT; j += 2) store_bf16_pair(crow, n0 + 16 * j, t[j], t[j + 1], p.n, p.vec, g);
+                for (int j = 0; j < NT; j += 2) store_bf16_pair<FULL>(crow, n0 + 16 * j, t[j], t[j + 1], p.n, g);
             }
         }
+        if (kResidual && i + 1 < MT)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) now[j] = next[j];
     }
+}
+
+template <int EPI, int MT, int NT>
+__device__ __forceinline__ void epilogue(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane) {
+    if (p.vec && m0 + 16 * MT <= p.m && n0 + 16 * NT <= p.n) epilogue_form<EPI, MT, NT, true>(p, acc, m0, n0, lane);
+    else epilogue_form<EPI, MT, NT, false>(p, acc, m0, n0, lane);
 }
 
 // One work-group of WM x WN waves computes a tile of (16 MT WM) x (16 NT WN).  K runs through a ring of RING slices in
