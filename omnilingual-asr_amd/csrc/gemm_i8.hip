@@ -97,34 +97,49 @@ __device__ __forceinline__ void store_f32(float* p, f32x4 v, int64_t count) {
             if (e < count) p[e] = v[e];
     }
 }
-__device__ __forceinline__ void store_bf16(uint16_t* p, u32x2 v, int64_t count) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (e < count) p[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-}
-
-// Two neighbouring 16-column tiles of bf16 results, four columns of each per lane: lanes 16 apart trade halves, so
-// that a lane holds eight consecutive columns and a row leaves as 64 consecutive bytes.
+// Eight bf16 values of a row, of which the first `count` exist.
 template <bool FULL>
-__device__ __forceinline__ void store_bf16_pair(uint16_t* row, int64_t col, u32x2 t0, u32x2 t1, int64_t n, int g) {
+__device__ __forceinline__ void store_bf16x8(uint16_t* p, u32x4 v, int64_t count) {
     if (FULL) {
-        const auto p = __builtin_amdgcn_permlane16_swap(t0[0], t1[0], false, false);
-        const auto q = __builtin_amdgcn_permlane16_swap(t0[1], t1[1], false, false);
-        // even lane rows hold tile 0, odd ones tile 1; lane rows 0, 1 its columns 0..7, lane rows 2, 3 columns 8..15
-        const u32x4 v = {p[0], q[0], p[1], q[1]};
-        *reinterpret_cast<u32x4*>(row + col + 16 * (g & 1) + 8 * (g >> 1)) = v;
+        *reinterpret_cast<u32x4*>(p) = v;
     } else {
-        store_bf16(row + col + 4 * g, t0, n - (col + 4 * g));
-        store_bf16(row + col + 16 + 4 * g, t1, n - (col + 16 + 4 * g));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < count) p[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
     }
 }
 
+// Orders a wave's own LDS writes before its reads of them (LDS operations of a wave execute in order).
+#define OASR_I8_WAVE_LDS()                                              \
+    do {                                                                \
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local"); \
+        __builtin_amdgcn_wave_barrier();                                \
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local"); \
+    } while (0)
+
+constexpr int kSlab = 4096;     // LDS per wave of the epilogue: 16 rows x 64 columns of float32
+
 // A wave's MT x NT tiles of 16 x 16, the first at (m0, n0): scales, bias, epilogue, stores.  FULL: the whole of it lies
 // inside the matrix and rows start on 16-byte boundaries, so nothing is guarded.
+// The matrix instruction leaves four columns of one row in a lane and the 16 rows of a tile in neighbouring lanes, which
+// stored as it is costs a memory request per lane (measured: 16 bytes per clock and CU).  Each group of 16 rows therefore
+// crosses a wave-private slab, and leaves with the columns of a row in neighbouring lanes: whole 128-byte lines.  The slab's
+// 16-byte chunks are permuted by the row so that neither side has bank conflicts.
 template <int EPI, int MT, int NT, bool FULL>
-__device__ __forceinline__ void epilogue_form(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane) {
-    static_assert(NT % 2 == 0, "columns are stored in pairs of tiles");
+__device__ __forceinline__ void epilogue_form(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane,
+                                              char* slab) {
+    static_assert(NT == 4 || NT == 2, "a wave owns 64 or 32 columns");
+    constexpr bool kResidual = EPI == OASR_EPI_RESIDUAL_F32, kFloat = kResidual || EPI == OASR_EPI_BIAS_F32,
+                   kGlu = EPI == OASR_EPI_GLU_BF16;
+    constexpr int kOut = kGlu ? 8 * NT : 16 * NT;                     // output columns of the wave
+    constexpr int kChunks = kFloat ? kOut / 4 : kOut / 8;             // 16-byte chunks per row: 16, 8, 4 or 2
+    constexpr int kRows = 64 / kChunks < 16 ? 64 / kChunks : 16;      // rows per store instruction
+    constexpr int kShift = kChunks == 16 ? 0 : kChunks == 8 ? 1 : kChunks == 4 ? 2 : 3;   // rows per 256 bytes, log2
     const int r = lane & 15, g = lane >> 4;
+    const int out_row = lane / kChunks, out_chunk = lane % kChunks;   // in the storing role (lanes past 16 rows idle)
+    const bool storing = kRows * kChunks == 64 || out_row < kRows;
+    const int64_t out0 = kGlu ? n0 / 2 : n0, out_n = kGlu ? p.n / 2 : p.n;
+    const int64_t out_col = out0 + out_chunk * (kFloat ? 4 : 8);
     f32x4 sw[NT], bv[NT];
     float sa[MT];
 #pragma unroll
@@ -134,76 +149,77 @@ __device__ __forceinline__ void epilogue_form(const GemmArgs& p, const i32x4 (&a
         sw[j] = load_cols<FULL>(p.scale_w, n0 + 16 * j + 4 * g, p.n);
         bv[j] = p.bias ? load_cols<FULL>(p.bias, n0 + 16 * j + 4 * g, p.n) : (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    constexpr bool kResidual = EPI == OASR_EPI_RESIDUAL_F32;
-    f32x4 now[NT], next[NT];
-    auto load_resid = [&](int i, f32x4 (&x)[NT]) {
-        const int64_t row = m0 + 16 * i + r;
-        if (!FULL && row >= p.m) return;
+    f32x4 now[16 / kRows], next[16 / kRows];
+    auto load_resid = [&](int i, f32x4 (&x)[16 / kRows]) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) x[j] = load_f32<FULL>(p.resid + row * p.ldr + n0 + 16 * j + 4 * g, p.n - (n0 + 16 * j + 4 * g));
+        for (int q = 0; q < 16 / kRows; ++q) {
+            const int64_t row = m0 + 16 * i + kRows * q + out_row;
+            if (FULL || row < p.m) x[q] = load_f32<FULL>(p.resid + row * p.ldr + out_col, out_n - out_col);
+        }
     };
     if (kResidual) load_resid(0, now);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const int64_t row = m0 + 16 * i + r;
-        if (kResidual && i + 1 < MT) load_resid(i + 1, next);       // requested before this row group's stores
-        if (!FULL && row >= p.m) continue;
+        if (kResidual && i + 1 < MT) load_resid(i + 1, next);         // requested before this row group's stores
         f32x4 o[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e)      // the weight's scale first: a token's may be as large as float32 goes
                 o[j][e] = fmaf((float)acc[i][j][e] * sw[j][e], sa[i], bv[j][e]);
-        if (EPI == OASR_EPI_BIAS_F32 || kResidual) {
+        const int turn = r >> kShift;
+        if (kFloat) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int64_t col = n0 + 16 * j + 4 * g;
-                if (kResidual)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] = fmaf(p.alpha, o[j][e], now[j][e]);
-                store_f32<FULL>(reinterpret_cast<float*>(p.c) + row * p.ldc + col, o[j], p.n - col);
-            }
+            for (int j = 0; j < NT; ++j)
+                *reinterpret_cast<f32x4*>(slab + r * (16 * kChunks) + (((4 * j + g) ^ (turn & (kChunks - 1))) << 4)) = o[j];
         } else {
-            uint16_t* crow = reinterpret_cast<uint16_t*>(p.c) + row * p.ldc;
-            if (EPI == OASR_EPI_GLU_BF16) {      // tile 2 q = 16 value columns, tile 2 q + 1 = their gates (n % 32 == 0)
-                u32x2 t[NT / 2];
 #pragma unroll
-                for (int q = 0; q < NT / 2; ++q) {
-                    f32x4 v;
+            for (int j = 0; j < NT; j += kGlu ? 2 : 1) {
+                f32x4 v = o[j];
+                if (kGlu) {                  // tile 2 q = 16 value columns, tile 2 q + 1 = their gates (n % 32 == 0)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = o[2 * q][e] * sigmoidf(o[2 * q + 1][e]);
-                    t[q] = (u32x2){cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
+                    for (int e = 0; e < 4; ++e) v[e] *= sigmoidf(o[j + 1][e]);
                 }
-                if (NT == 2) {
-                    store_bf16(crow + n0 / 2 + 4 * g, t[0], p.n / 2 - (n0 / 2 + 4 * g));
-                } else {
+                if (EPI == OASR_EPI_BIAS_SWISH_BF16) {
 #pragma unroll
-                    for (int q = 0; q + 1 < NT / 2; q += 2)
-                        store_bf16_pair<FULL>(crow, n0 / 2 + 16 * q, t[q], t[q + 1], p.n / 2, g);
+                    for (int e = 0; e < 4; ++e) v[e] = swishf(v[e]);
                 }
-            } else {
-                u32x2 t[NT];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if (EPI == OASR_EPI_BIAS_SWISH_BF16)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][e] = swishf(o[j][e]);
-                    t[j] = (u32x2){cvt_pk_bf16(o[j][0], o[j][1]), cvt_pk_bf16(o[j][2], o[j][3])};
-                }
-#pragma unroll
-                for (int j = 0; j < NT; j += 2) store_bf16_pair<FULL>(crow, n0 + 16 * j, t[j], t[j + 1], p.n, g);
+                const int half = 4 * (kGlu ? j / 2 : j) + g;          // 8-byte half of a chunk
+                *reinterpret_cast<u32x2*>(slab + r * (16 * kChunks) + (((half >> 1) ^ (turn & (kChunks - 1))) << 4) + (half & 1) * 8) =
+                    (u32x2){cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
             }
         }
+        OASR_I8_WAVE_LDS();
+#pragma unroll
+        for (int q = 0; q < 16 / kRows; ++q) {
+            const int sr = kRows * q + out_row;
+            const int64_t row = m0 + 16 * i + sr;
+            u32x4 v = {0, 0, 0, 0};
+            if (storing)
+                v = *reinterpret_cast<const u32x4*>(slab + sr * (16 * kChunks) + ((out_chunk ^ ((sr >> kShift) & (kChunks - 1))) << 4));
+            if (!storing || !(FULL || row < p.m)) continue;
+            if (kFloat) {
+                f32x4 f = __builtin_bit_cast(f32x4, v);
+                if (kResidual) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[e] = fmaf(p.alpha, f[e], now[q][e]);
+                }
+                store_f32<FULL>(reinterpret_cast<float*>(p.c) + row * p.ldc + out_col, f, out_n - out_col);
+            } else {
+                store_bf16x8<FULL>(reinterpret_cast<uint16_t*>(p.c) + row * p.ldc + out_col, v, out_n - out_col);
+            }
+        }
+        OASR_I8_WAVE_LDS();
         if (kResidual && i + 1 < MT)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) now[j] = next[j];
+            for (int q = 0; q < 16 / kRows; ++q) now[q] = next[q];
     }
 }
 
 template <int EPI, int MT, int NT>
-__device__ __forceinline__ void epilogue(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane) {
-    if (p.vec && m0 + 16 * MT <= p.m && n0 + 16 * NT <= p.n) epilogue_form<EPI, MT, NT, true>(p, acc, m0, n0, lane);
-    else epilogue_form<EPI, MT, NT, false>(p, acc, m0, n0, lane);
+__device__ __forceinline__ void epilogue(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane, char* slab) {
+    if (p.vec && m0 + 16 * MT <= p.m && n0 + 16 * NT <= p.n) epilogue_form<EPI, MT, NT, true>(p, acc, m0, n0, lane, slab);
+    else epilogue_form<EPI, MT, NT, false>(p, acc, m0, n0, lane, slab);
 }
 
 // One work-group of WM x WN waves computes a tile of (16 MT WM) x (16 NT WN).  K runs through a ring of RING slices in
@@ -278,7 +294,9 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmAr
             for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[i][j], 0, 0, 0);
         slot = slot + 1 == RING ? 0 : slot + 1;
     }
-    epilogue<EPI, MT, NT>(p, acc, m0 + wm * MT * 16, n0 + wn * NT * 16, lane);
+    static_assert(RING * kSlot >= kWaves * kSlab, "the slabs take the ring's place");
+    __syncthreads();                         // every wave has read its last slice
+    epilogue<EPI, MT, NT>(p, acc, m0 + wm * MT * 16, n0 + wn * NT * 16, lane, ring + wave * kSlab);
 }
 
 // Large problems: 256 x 256 tiles, eight waves as two groups (the upper and the lower 128 rows) one barrier apart, so that
@@ -291,7 +309,7 @@ constexpr int kWide = 256, kWideRing = 4, kWideSlice = kWide * kSlice;
 
 template <int EPI>
 __global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int tiles_m, int tiles_n) {
-    __shared__ __attribute__((aligned(1024))) char ring[2 * kWideRing * kWideSlice];      // A slots, then W slots
+    __shared__ __attribute__((aligned(1024))) char ring[2 * kWideRing * kWideSlice + 8 * kSlab];      // A slots, W slots, slabs
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 2, wn = wave & 3;
@@ -400,7 +418,8 @@ __global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int
             // groups' epilogues overlap
             if (!(wm == 1 && t == nph - 1)) OASR_I8_BARRIER();
         }
-        epilogue<EPI, 8, 4>(p, acc, (int64_t)tm * kWide + wm * 128, (int64_t)tn * kWide + wn * 64, lane);
+        epilogue<EPI, 8, 4>(p, acc, (int64_t)tm * kWide + wm * 128, (int64_t)tn * kWide + wn * 64, lane,
+                            ring + 2 * kWideRing * kWideSlice + wave * kSlab);
         if (wm == 1) OASR_I8_BARRIER();
     }
     if (wm == 0) OASR_I8_BARRIER();          // the same number of barriers in both groups
