@@ -5,9 +5,11 @@
 // the epilogue and the output type.
 //
 // Weights are packed once (oasr_gemm_pack_w_i8): pieces of 16 rows x 64 k, 1 KiB each, ordered [row group][K slice],
-// rows and k padded with zeros; chunk c (16 bytes) of row r of a piece sits at chunk c ^ ((r >> 2) & 3).  That is the
-// LDS image of a piece, and it makes the fragment reads (lane = (row r = lane & 15, chunk lane >> 4)) free of bank
-// conflicts; A's rows are brought into the same image by the copies' source addresses.
+// rows and k padded with zeros; a piece holds its 16-byte chunks in the order in which the lanes of a fragment take them
+// (lane = (row lane & 15, chunk lane >> 4)), so a fragment is one contiguous KiB, in memory as in LDS.  A's rows stay
+// row-major: a copy brings 16 rows x 64 k with four neighbouring lanes per row (whole 64-byte segments) and its source
+// addresses put chunk c of row r at place c ^ ((r >> 2) & 3) of the row, which keeps the fragment reads free of bank
+// conflicts.
 // The weight fragment is the matrix instruction's A operand (v_mfma_i32_16x16x64_i8), so a lane ends up with four
 // consecutive n of one row m: C[m = lane & 15][n = 4 (lane >> 4) + e].
 #include "oasr_common.h"
@@ -126,112 +128,141 @@ __device__ __forceinline__ float sigmoid_of(float z) { return __builtin_amdgcn_r
 
 constexpr int kSlab = 4096;     // LDS per wave of the epilogue: 16 rows x 64 columns of float32
 
-// A wave's MT x NT tiles of 16 x 16, the first at (m0, n0): scales, bias, epilogue, stores.  FULL: the whole of it lies
-// inside the matrix and rows start on 16-byte boundaries, so nothing is guarded.
+// The epilogue of a wave's MT x NT tiles of 16 x 16, the first at (m0, n0): scales, bias, activation or residual, stores.
+// FULL: the whole of it lies inside the matrix and rows start on 16-byte boundaries, so nothing is guarded.
 // The matrix instruction leaves four columns of one row in a lane and the 16 rows of a tile in neighbouring lanes, which
 // stored as it is costs a memory request per lane (measured: 16 bytes per clock and CU).  Each group of 16 rows therefore
 // crosses a wave-private slab, and leaves with the columns of a row in neighbouring lanes: whole 128-byte lines.  The slab's
 // 16-byte chunks are permuted by the row so that neither side has bank conflicts.
-template <int EPI, int MT, int NT, bool FULL>
-__device__ __forceinline__ void epilogue_form(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane,
-                                              char* slab) {
+template <int EPI, int MT, int NT>
+struct Epilogue {
     static_assert(NT == 4 || NT == 2, "a wave owns 64 or 32 columns");
-    constexpr bool kResidual = EPI == OASR_EPI_RESIDUAL_F32, kFloat = kResidual || EPI == OASR_EPI_BIAS_F32,
-                   kGlu = EPI == OASR_EPI_GLU_BF16;
-    constexpr int kOut = kGlu ? 8 * NT : 16 * NT;                     // output columns of the wave
-    constexpr int kChunks = kFloat ? kOut / 4 : kOut / 8;             // 16-byte chunks per row: 16, 8, 4 or 2
-    constexpr int kRows = 64 / kChunks < 16 ? 64 / kChunks : 16;      // rows per store instruction
-    constexpr int kShift = kChunks == 16 ? 0 : kChunks == 8 ? 1 : kChunks == 4 ? 2 : 3;   // rows per 256 bytes, log2
-    const int r = lane & 15, g = lane >> 4;
-    const int out_row = lane / kChunks, out_chunk = lane % kChunks;   // in the storing role (lanes past 16 rows idle)
-    const bool storing = kRows * kChunks == 64 || out_row < kRows;
-    const int64_t out0 = kGlu ? n0 / 2 : n0, out_n = kGlu ? p.n / 2 : p.n;
-    const int64_t out_col = out0 + out_chunk * (kFloat ? 4 : 8);
-    f32x4 sw[NT], bv[NT];
+    static constexpr bool kResidual = EPI == OASR_EPI_RESIDUAL_F32, kFloat = kResidual || EPI == OASR_EPI_BIAS_F32,
+                          kGlu = EPI == OASR_EPI_GLU_BF16;
+    static constexpr int kOut = kGlu ? 8 * NT : 16 * NT;                     // output columns of the wave
+    static constexpr int kChunks = kFloat ? kOut / 4 : kOut / 8;             // 16-byte chunks per row: 16, 8, 4 or 2
+    static constexpr int kRows = 64 / kChunks < 16 ? 64 / kChunks : 16;      // rows per store instruction
+    static constexpr int kStores = 16 / kRows;
+    static constexpr int kShift = kChunks == 16 ? 0 : kChunks == 8 ? 1 : kChunks == 4 ? 2 : 3;   // rows per 256 bytes, log2
+
+    f32x4 sw[NT], bv[NT], resid[kStores];     // resid: of the row group whose turn is next
     float sa[MT];
+
+    static __device__ __forceinline__ bool full(const GemmArgs& p, int64_t m0, int64_t n0) {
+        return p.vec && m0 + 16 * MT <= p.m && n0 + 16 * NT <= p.n;
+    }
+    static __device__ __forceinline__ int64_t out_col(int64_t n0, int lane) { return (kGlu ? n0 / 2 : n0) + lane % kChunks * (kFloat ? 4 : 8); }
+
+    template <bool FULL>
+    __device__ __forceinline__ void load_resid(const GemmArgs& p, int64_t m0, int64_t n0, int lane, int i) {
+        const int64_t col = out_col(n0, lane);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sa[i] = FULL || m0 + 16 * i + r < p.m ? p.scale_a[m0 + 16 * i + r] : 0.f;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        sw[j] = load_cols<FULL>(p.scale_w, n0 + 16 * j + 4 * g, p.n);
-        bv[j] = p.bias ? load_cols<FULL>(p.bias, n0 + 16 * j + 4 * g, p.n) : (f32x4){0.f, 0.f, 0.f, 0.f};
-        if (EPI == OASR_EPI_BIAS_SWISH_BF16 || (kGlu && (j & 1))) {
-            sw[j] *= -kLog2e;
-            bv[j] *= -kLog2e;
+        for (int q = 0; q < kStores; ++q) {
+            const int64_t row = m0 + 16 * i + kRows * q + lane / kChunks;
+            if (FULL || row < p.m) resid[q] = load_f32<FULL>(p.resid + row * p.ldr + col, p.n - col);
         }
     }
-    f32x4 now[16 / kRows], next[16 / kRows];
-    auto load_resid = [&](int i, f32x4 (&x)[16 / kRows]) {
+
+    template <bool FULL>
+    __device__ __forceinline__ void load_form(const GemmArgs& p, int64_t m0, int64_t n0, int lane) {
+        const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-        for (int q = 0; q < 16 / kRows; ++q) {
-            const int64_t row = m0 + 16 * i + kRows * q + out_row;
-            if (FULL || row < p.m) x[q] = load_f32<FULL>(p.resid + row * p.ldr + out_col, out_n - out_col);
+        for (int i = 0; i < MT; ++i) sa[i] = FULL || m0 + 16 * i + r < p.m ? p.scale_a[m0 + 16 * i + r] : 0.f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            sw[j] = load_cols<FULL>(p.scale_w, n0 + 16 * j + 4 * g, p.n);
+            bv[j] = p.bias ? load_cols<FULL>(p.bias, n0 + 16 * j + 4 * g, p.n) : (f32x4){0.f, 0.f, 0.f, 0.f};
         }
-    };
-    if (kResidual) load_resid(0, now);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        if (kResidual && i + 1 < MT) load_resid(i + 1, next);         // requested before this row group's stores
-        f32x4 o[NT];
+        if (kResidual) load_resid<FULL>(p, m0, n0, lane, 0);
+    }
+    __device__ __forceinline__ void load(const GemmArgs& p, int64_t m0, int64_t n0, int lane) {
+        if (full(p, m0, n0)) load_form<true>(p, m0, n0, lane);
+        else load_form<false>(p, m0, n0, lane);
+    }
+
+    template <bool FULL>
+    __device__ __forceinline__ void finish_form(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane, char* slab) {
+        const int r = lane & 15, g = lane >> 4;
+        const int out_row = lane / kChunks, out_chunk = lane % kChunks;   // in the storing role (lanes past 16 rows idle)
+        const bool storing = kRows * kChunks == 64 || out_row < kRows;
+        const int64_t col = out_col(n0, lane), left = (kGlu ? p.n / 2 : p.n) - col;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
+            if (EPI == OASR_EPI_BIAS_SWISH_BF16 || (kGlu && (j & 1))) {
+                sw[j] *= -kLog2e;
+                bv[j] *= -kLog2e;
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)      // the weight's scale first: a token's may be as large as float32 goes
-                o[j][e] = fmaf((float)acc[i][j][e] * sw[j][e], sa[i], bv[j][e]);
-        const int turn = r >> kShift;
-        if (kFloat) {
+        for (int i = 0; i < MT; ++i) {
+            f32x4 o[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-                *reinterpret_cast<f32x4*>(slab + r * (16 * kChunks) + (((4 * j + g) ^ (turn & (kChunks - 1))) << 4)) = o[j];
-        } else {
 #pragma unroll
-            for (int j = 0; j < NT; j += kGlu ? 2 : 1) {
-                f32x4 v = o[j];
-                if (kGlu) {                  // tile 2 q = 16 value columns, tile 2 q + 1 = their gates (n % 32 == 0)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] *= sigmoid_of(o[j + 1][e]);
-                }
-                if (EPI == OASR_EPI_BIAS_SWISH_BF16) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = swish_of(v[e]);
-                }
-                const int half = 4 * (kGlu ? j / 2 : j) + g;          // 8-byte half of a chunk
-                *reinterpret_cast<u32x2*>(slab + r * (16 * kChunks) + (((half >> 1) ^ (turn & (kChunks - 1))) << 4) + (half & 1) * 8) =
-                    (u32x2){cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
-            }
-        }
-        OASR_I8_WAVE_LDS();
-#pragma unroll
-        for (int q = 0; q < 16 / kRows; ++q) {
-            const int sr = kRows * q + out_row;
-            const int64_t row = m0 + 16 * i + sr;
-            u32x4 v = {0, 0, 0, 0};
-            if (storing)
-                v = *reinterpret_cast<const u32x4*>(slab + sr * (16 * kChunks) + ((out_chunk ^ ((sr >> kShift) & (kChunks - 1))) << 4));
-            if (!storing || !(FULL || row < p.m)) continue;
+                for (int e = 0; e < 4; ++e)      // the weight's scale first: a token's may be as large as float32 goes
+                    o[j][e] = fmaf((float)acc[i][j][e] * sw[j][e], sa[i], bv[j][e]);
+            const int turn = (r >> kShift) & (kChunks - 1);
             if (kFloat) {
-                f32x4 f = __builtin_bit_cast(f32x4, v);
-                if (kResidual) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[e] = fmaf(p.alpha, f[e], now[q][e]);
-                }
-                store_f32<FULL>(reinterpret_cast<float*>(p.c) + row * p.ldc + out_col, f, out_n - out_col);
+                for (int j = 0; j < NT; ++j)
+                    *reinterpret_cast<f32x4*>(slab + r * (16 * kChunks) + (((4 * j + g) ^ turn) << 4)) = o[j];
             } else {
-                store_bf16x8<FULL>(reinterpret_cast<uint16_t*>(p.c) + row * p.ldc + out_col, v, out_n - out_col);
+#pragma unroll
+                for (int j = 0; j < NT; j += kGlu ? 2 : 1) {
+                    f32x4 v = o[j];
+                    if (kGlu) {                  // tile 2 q = 16 value columns, tile 2 q + 1 = their gates (n % 32 == 0)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] *= sigmoid_of(o[j + 1][e]);
+                    }
+                    if (EPI == OASR_EPI_BIAS_SWISH_BF16) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = swish_of(v[e]);
+                    }
+                    const int half = 4 * (kGlu ? j / 2 : j) + g;          // 8-byte half of a chunk
+                    *reinterpret_cast<u32x2*>(slab + r * (16 * kChunks) + (((half >> 1) ^ turn) << 4) + (half & 1) * 8) =
+                        (u32x2){cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
+                }
+            }
+            OASR_I8_WAVE_LDS();
+            u32x4 v[kStores];
+#pragma unroll
+            for (int q = 0; q < kStores; ++q) {
+                const int sr = kRows * q + out_row;
+                v[q] = (u32x4){0, 0, 0, 0};
+                if (storing) v[q] = *reinterpret_cast<const u32x4*>(slab + sr * (16 * kChunks) + ((out_chunk ^ ((sr >> kShift) & (kChunks - 1))) << 4));
+                if (kResidual) {
+                    f32x4 f = __builtin_bit_cast(f32x4, v[q]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[e] = fmaf(p.alpha, f[e], resid[q][e]);
+                    v[q] = __builtin_bit_cast(u32x4, f);
+                }
+            }
+            OASR_I8_WAVE_LDS();
+            if (kResidual && i + 1 < MT) load_resid<FULL>(p, m0, n0, lane, i + 1);      // requested before this row group's stores
+#pragma unroll
+            for (int q = 0; q < kStores; ++q) {
+                const int64_t row = m0 + 16 * i + kRows * q + out_row;
+                if (!storing || !(FULL || row < p.m)) continue;
+                if (kFloat) store_f32<FULL>(reinterpret_cast<float*>(p.c) + row * p.ldc + col, __builtin_bit_cast(f32x4, v[q]), left);
+                else store_bf16x8<FULL>(reinterpret_cast<uint16_t*>(p.c) + row * p.ldc + col, v[q], left);
             }
         }
-        OASR_I8_WAVE_LDS();
-        if (kResidual && i + 1 < MT)
-#pragma unroll
-            for (int q = 0; q < 16 / kRows; ++q) now[q] = next[q];
     }
-}
-
-template <int EPI, int MT, int NT>
-__device__ __forceinline__ void epilogue(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane, char* slab) {
-    if (p.vec && m0 + 16 * MT <= p.m && n0 + 16 * NT <= p.n) epilogue_form<EPI, MT, NT, true>(p, acc, m0, n0, lane, slab);
-    else epilogue_form<EPI, MT, NT, false>(p, acc, m0, n0, lane, slab);
-}
+    __device__ __forceinline__ void finish(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane, char* slab) {
+        if (full(p, m0, n0)) finish_form<true>(p, acc, m0, n0, lane, slab);
+        else finish_form<false>(p, acc, m0, n0, lane, slab);
+    }
+    // both at once
+    static __device__ __forceinline__ void run(const GemmArgs& p, const i32x4 (&acc)[MT][NT], int64_t m0, int64_t n0, int lane, char* slab) {
+        Epilogue e;
+        if (full(p, m0, n0)) {
+            e.template load_form<true>(p, m0, n0, lane);
+            e.template finish_form<true>(p, acc, m0, n0, lane, slab);
+        } else {
+            e.template load_form<false>(p, m0, n0, lane);
+            e.template finish_form<false>(p, acc, m0, n0, lane, slab);
+        }
+    }
+};
 
 // One work-group of WM x WN waves computes a tile of (16 MT WM) x (16 NT WN).  K runs through a ring of RING slices in
 // LDS, filled by direct copies RING - 1 slices ahead, one barrier per slice: behind the barrier of slice p every wave
@@ -296,7 +327,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmAr
         const char* sw = ring + slot * kSlot + (BM / 16 + wn * NT) * kPiece;
         i32x4 wf[NT], xf[MT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) wf[j] = *reinterpret_cast<const i32x4*>(sw + j * kPiece + frag);
+        for (int j = 0; j < NT; ++j) wf[j] = *reinterpret_cast<const i32x4*>(sw + j * kPiece + lane * 16);
 #pragma unroll
         for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(sa + i * kPiece + frag);
 #pragma unroll
@@ -307,7 +338,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmAr
     }
     static_assert(RING * kSlot >= kWaves * kSlab, "the slabs take the ring's place");
     __syncthreads();                         // every wave has read its last slice
-    epilogue<EPI, MT, NT>(p, acc, m0 + wm * MT * 16, n0 + wn * NT * 16, lane, ring + wave * kSlab);
+    Epilogue<EPI, MT, NT>::run(p, acc, m0 + wm * MT * 16, n0 + wn * NT * 16, lane, ring + wave * kSlab);
 }
 
 // Large problems: 256 x 256 tiles, eight waves as two groups (the upper and the lower 128 rows) one barrier apart, so that
@@ -399,7 +430,7 @@ __global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int
         tile_at(i, tm, tn);
         for (int t = 0; t < nph; ++t, ++ph) {
             const char* sa = ring + (ph & 3) * kWideSlice + wm * 8 * kPiece + frag;
-            const char* sw = ring + (kWideRing + (ph & 3)) * kWideSlice + wn * 4 * kPiece + frag;
+            const char* sw = ring + (kWideRing + (ph & 3)) * kWideSlice + wn * 4 * kPiece + lane * 16;
             i32x4 wf[4], xf[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) wf[j] = *reinterpret_cast<const i32x4*>(sw + j * kPiece);
@@ -429,11 +460,124 @@ __global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int
             // groups' epilogues overlap
             if (!(wm == 1 && t == nph - 1)) OASR_I8_BARRIER();
         }
-        epilogue<EPI, 8, 4>(p, acc, (int64_t)tm * kWide + wm * 128, (int64_t)tn * kWide + wn * 64, lane,
-                            ring + 2 * kWideRing * kWideSlice + wave * kSlab);
+        // (loading the scales during the last slice instead costs more in the loop than it saves here)
+        Epilogue<EPI, 8, 4>::run(p, acc, (int64_t)tm * kWide + wm * 128, (int64_t)tn * kWide + wn * 64, lane,
+                                 ring + 2 * kWideRing * kWideSlice + wave * kSlab);
         if (wm == 1) OASR_I8_BARRIER();
     }
     if (wm == 0) OASR_I8_BARRIER();          // the same number of barriers in both groups
+}
+
+// Problems with few tiles (single tokens, one utterance): a work-group of eight waves owns 16 MT x 64 outputs, and the
+// waves split K among them, slice by slice in turn.  Exact sums make the split free of consequences, and it is what keeps
+// enough bytes in flight: no wave waits for another before the end.  A wave brings its A rows through an LDS ring of its own
+// (DEPTH slices, no barriers) and its weight fragments straight to registers, both DEPTH - 1 slices ahead: about 200 KiB per
+// CU on their way, where the ring shared by the waves of a tile holds 48 (1504 x 1024 x 4096: 33 us).  At the end the partial
+// sums cross LDS, and every wave finishes its share of the 16 x 32 outputs.
+template <int MT>
+struct SplitShape {
+    static constexpr int kDepth = MT >= 8 ? 2 : 3;
+    static constexpr int kRingBytes = kDepth * MT * kPiece;                // per wave
+    static constexpr int kPasses = MT > 4 ? 2 : 1;                         // partial sums of 64 or, twice, of 32 columns
+    static constexpr int kCols = 4 / kPasses;                              // column tiles per pass
+    static constexpr int kUnits = MT * kCols / 2;                          // 16 x 32 outputs per pass, one per wave
+    static constexpr int kSumBytes = 8 * MT * kCols * 1024;
+    static constexpr int kLds = 8 * kRingBytes > kSumBytes + 8 * 2048 ? 8 * kRingBytes : kSumBytes + 8 * 2048;
+};
+
+template <int EPI, int MT>
+__global__ __launch_bounds__(512) void gemm_i8_split_kernel(const GemmArgs p, int tiles_m) {
+    typedef SplitShape<MT> Shape;
+    constexpr int D = Shape::kDepth;
+    __shared__ __attribute__((aligned(1024))) char lds[Shape::kLds];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t m0 = (int64_t)(blockIdx.x % tiles_m) * (16 * MT), n0 = (int64_t)(blockIdx.x / tiles_m) * 64;
+
+    char* const ring = lds + wave * Shape::kRingBytes;
+    const char* src_a[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        int64_t row = m0 + 16 * i + (lane >> 2);
+        row = row < p.m ? row : p.m - 1;
+        src_a[i] = reinterpret_cast<const char*>(p.a) + row * p.lda + (((lane & 3) ^ ((lane >> 4) & 3)) << 4) + wave * kSlice;
+    }
+    const char* src_w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        int64_t grp = n0 / 16 + j;
+        grp = grp < p.ng ? grp : p.ng - 1;
+        src_w[j] = reinterpret_cast<const char*>(p.w) + (grp * p.ks + wave) * kPiece + lane * 16;
+    }
+    i32x4 acc[MT][4], wf[D][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
+    const int count = p.ks > wave ? (p.ks - wave + 7) / 8 : 0;            // this wave's slices
+    auto request = [&](int slot, i32x4 (&w)[4]) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            __builtin_amdgcn_global_load_lds((gbl_void*)src_a[i], (lds_void*)(ring + (slot * MT + i) * kPiece), 16, 0, 0);
+            src_a[i] += 8 * kSlice;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w[j] = *reinterpret_cast<const i32x4*>(src_w[j]);
+            src_w[j] += 8 * kPiece;
+        }
+    };
+    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ ((fr >> 2) & 3)) << 4);
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+        if (d < count) request(d, wf[d]);
+    // the scales (and residual rows) of the 16 x 32 outputs that this wave will finish come along with the first slices
+    const int unit_row = Shape::kCols == 4 ? (wave >> 1) % MT : wave % MT, unit_col = Shape::kCols == 4 ? 2 * (wave & 1) : 0;
+    const int64_t mu = m0 + 16 * unit_row, nu = n0 + 16 * unit_col;
+    Epilogue<EPI, 1, 2> out;
+    out.load(p, mu, nu, lane);
+    for (int t = 0; t < count; t += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (t + d >= count) break;
+            // the slot of slice t + d - 1 is free: its fragments went into the products above
+            if (t + d + D - 1 < count) {
+                request((d + D - 1) % D, wf[(d + D - 1) % D]);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * (MT + 4)) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            i32x4 xf[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(ring + (d * MT + i) * kPiece + frag);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[d][j], xf[i], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // partial sums: [wave][row tile][column tile of the pass][lane]
+#pragma unroll
+    for (int pass = 0; pass < Shape::kPasses; ++pass) {
+        __syncthreads();                     // the rings, or the pass before, have been read
+        if (pass) out.load(p, mu, nu + 32 * pass, lane);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < Shape::kCols; ++j)
+                *reinterpret_cast<i32x4*>(lds + ((wave * MT + i) * Shape::kCols + j) * 1024 + lane * 16) = acc[i][pass * Shape::kCols + j];
+        __syncthreads();
+        if (wave < Shape::kUnits) {
+            i32x4 sum[1][2] = {};
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    sum[0][j] += *reinterpret_cast<const i32x4*>(lds + ((w * MT + unit_row) * Shape::kCols + unit_col + j) * 1024 + lane * 16);
+            out.finish(p, sum, mu, nu + 32 * pass, lane, lds + Shape::kSumBytes + wave * 2048);
+        }
+    }
 }
 
 // Per-row quantisation of bf16 rows.  One wavefront per row with the row in registers (k <= 512 NV: NV loads of 16
@@ -517,7 +661,7 @@ __global__ __launch_bounds__(256) void gemm_pack_w_i8_kernel(const int8_t* __res
     if (idx >= chunks) return;
     const int lane = (int)(idx & 63);
     const int64_t piece = idx >> 6, grp = piece / ks, t = piece - grp * ks;
-    const int64_t row = grp * 16 + (lane >> 2), col = t * kSlice + (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+    const int64_t row = grp * 16 + (lane & 15), col = t * kSlice + (lane >> 4) * 16;
     uint32_t v[4] = {0, 0, 0, 0};
     if (row < n)
         for (int e = 0; e < 16; ++e)
@@ -546,27 +690,68 @@ static int check_gemm(const char* what, const int8_t* w, const float* scale_w, c
     return OASR_OK;
 }
 
-template <int EPI>
-static void launch_tiles(const GemmArgs& p, hipStream_t st) {
-    const int64_t wide_m = (p.m + kWide - 1) / kWide, wide_n = (p.n + kWide - 1) / kWide;
-    // 32 row pitches have to fit the wide kernel's 32-bit offsets
-    if (wide_m * wide_n >= 128 && p.lda < (1 << 26)) {
-        const int grid = (int)(wide_m * wide_n < 256 ? (wide_m * wide_n + 7) / 8 * 8 : 256);
-        hipLaunchKernelGGL((gemm_i8_wide_kernel<EPI>), dim3(grid), dim3(512), 0, st, p, (int)wide_m, (int)wide_n);
-        return;
+// Which kernel runs a product: the one with the least estimated time, rounds * (begin + steps * step) microseconds.  A round is
+// 256 work-groups (one per CU; where several share a CU a further round costs `share` of one), a step one slice (64 k), or
+// for the splitting kernel eight.  The figures are fitted to times of all forms over 364 sizes (m 17 .. 4096, n 512 .. 16384,
+// k 512 .. 16384) and pick within 1.4 % of the fastest form on average: e.g. 1504 x 1024 x 4096: 96 rows split 14.8 us, 128 x 128
+// tiles 25.8, 256 x 256 43.4; 1504 x 4096 x 1024: 23.2 (32 rows split), 14.4, 20.1; 512 x 1024 x 512: 4.5, 6.2, 10.0.
+// 16 rows split re-read the weights once per row tile: with more than 128 work-groups of them 32 rows are faster
+// (99 x 2048 x 4096: 8.9 against 11.6 us).
+struct Form {
+    int bm, bn, slices;         // tile, slices per step
+    double begin, step, share;
+};
+enum { kSplit16, kSplit32, kSplit64, kSplit96, kSplit128, kTile128, kTile256, kForms };
+static const Form kFormTable[kForms] = {
+    {16, 64, 8, 1.50, 0.57, 0.7}, {32, 64, 8, 1.64, 0.68, 0.8},  {64, 64, 8, 2.40, 0.84, 1.0},  {96, 64, 8, 4.05, 1.10, 1.0},
+    {128, 64, 8, 4.35, 1.38, 1.0}, {128, 128, 1, 4.10, 0.33, 0.68}, {256, 256, 1, 11.3, 0.51, 1.0}};
+
+static int choose_form(const GemmArgs& p) {
+    int best = kTile128;
+    double least = 1e300;
+    for (int f = 0; f < kForms; ++f) {
+        const Form& t = kFormTable[f];
+        const int64_t groups = ((p.m + t.bm - 1) / t.bm) * ((p.n + t.bn - 1) / t.bn);
+        if (f == kSplit16 && p.m > 16 && groups > 128) continue;
+        if (f == kTile256 && p.lda >= (1 << 26)) continue;       // 32 row pitches have to fit its 32-bit offsets
+        const double rounds = (double)((groups + 255) / 256) * t.share;
+        const double us = (rounds < 1.0 ? 1.0 : rounds) * (t.begin + (p.ks + t.slices - 1) / t.slices * t.step);
+        if (us < least) {
+            least = us;
+            best = f;
+        }
     }
-    const int64_t tiles_n = (p.n + 127) / 128, tiles = (p.m + 127) / 128 * tiles_n;
-    hipLaunchKernelGGL((gemm_i8_tile_kernel<EPI, 2, 2, 4, 4, 4>), dim3((unsigned)tiles), dim3(256), 0, st, p, (int)tiles_n);
+    return best;
+}
+
+template <int EPI>
+static void launch_form(int form, const GemmArgs& p, hipStream_t st) {
+    const Form& t = kFormTable[form];
+    const int tm = (int)((p.m + t.bm - 1) / t.bm), tn = (int)((p.n + t.bn - 1) / t.bn);
+    const int64_t tiles = (int64_t)tm * tn;
+    const dim3 grid((unsigned)tiles), split(512);
+    switch (form) {
+        case kSplit16: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 1>), grid, split, 0, st, p, tm); break;
+        case kSplit32: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 2>), grid, split, 0, st, p, tm); break;
+        case kSplit64: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 4>), grid, split, 0, st, p, tm); break;
+        case kSplit96: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 6>), grid, split, 0, st, p, tm); break;
+        case kSplit128: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 8>), grid, split, 0, st, p, tm); break;
+        case kTile128: hipLaunchKernelGGL((gemm_i8_tile_kernel<EPI, 2, 2, 4, 4, 4>), grid, dim3(256), 0, st, p, tn); break;
+        default:
+            hipLaunchKernelGGL((gemm_i8_wide_kernel<EPI>), dim3((unsigned)(tiles < 256 ? (tiles + 7) / 8 * 8 : 256)), dim3(512), 0, st, p, tm, tn);
+    }
 }
 
 static int launch_gemm(const GemmArgs& p, int32_t epilogue, hipStream_t st) {
-    OASR_REQUIRE((p.m + 127) / 128 * ((p.n + 127) / 128) < ((int64_t)1 << 31), "gemm_i8: too many tiles");
+    const int form = choose_form(p);
+    const Form& t = kFormTable[form];
+    OASR_REQUIRE((p.m + t.bm - 1) / t.bm * ((p.n + t.bn - 1) / t.bn) < ((int64_t)1 << 30), "gemm_i8: too many tiles");
     switch (epilogue) {
-        case OASR_EPI_BIAS_BF16: launch_tiles<OASR_EPI_BIAS_BF16>(p, st); break;
-        case OASR_EPI_BIAS_SWISH_BF16: launch_tiles<OASR_EPI_BIAS_SWISH_BF16>(p, st); break;
-        case OASR_EPI_GLU_BF16: launch_tiles<OASR_EPI_GLU_BF16>(p, st); break;
-        case OASR_EPI_RESIDUAL_F32: launch_tiles<OASR_EPI_RESIDUAL_F32>(p, st); break;
-        default: launch_tiles<OASR_EPI_BIAS_F32>(p, st); break;
+        case OASR_EPI_BIAS_BF16: launch_form<OASR_EPI_BIAS_BF16>(form, p, st); break;
+        case OASR_EPI_BIAS_SWISH_BF16: launch_form<OASR_EPI_BIAS_SWISH_BF16>(form, p, st); break;
+        case OASR_EPI_GLU_BF16: launch_form<OASR_EPI_GLU_BF16>(form, p, st); break;
+        case OASR_EPI_RESIDUAL_F32: launch_form<OASR_EPI_RESIDUAL_F32>(form, p, st); break;
+        default: launch_form<OASR_EPI_BIAS_F32>(form, p, st); break;
     }
     OASR_CHECK_LAUNCH("gemm_i8");
     return OASR_OK;

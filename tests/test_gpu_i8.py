@@ -68,7 +68,8 @@ def test_quant_rows_at_the_ends_of_the_range():
 SHAPES = [(1, 1, 1), (1, 33, 64), (1, 1024, 512), (2, 1000, 1000), (3, 64, 65), (15, 96, 63), (16, 128, 128), (17, 130, 640),
           (33, 4096, 256), (64, 512, 4096), (99, 2048, 1024), (127, 257, 191), (128, 128, 64), (129, 384, 320), (200, 777, 1000),
           (256, 256, 64), (300, 96, 16448), (513, 1024, 512), (1000, 4096, 64), (1504, 1024, 1024), (2100, 640, 192),
-          (4096, 512, 512), (8200, 1056, 320), (2100, 4128, 128), (4500, 2080, 64), (2049, 4097, 65)]
+          (4096, 512, 512), (8200, 1056, 320), (2100, 4128, 128), (4500, 2080, 64), (2049, 4097, 65),
+          (48, 1000, 8192), (300, 2048, 4096), (400, 700, 4096), (1504, 1024, 4096), (1500, 1000, 4100), (2000, 2100, 4096), (64, 16400, 100)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -98,6 +99,22 @@ def _norm64(x, w, b, swish=0):
     hat = (x - x.mean(1, keepdim=True)) / torch.sqrt(x.var(1, unbiased=False, keepdim=True) + 1e-5)
     v, off = hat * w + b, 2.0 ** -19 * (w.abs() + (hat * w).abs() + b.abs())
     return (v * torch.sigmoid(v), 1.1 * off + 2.0 ** -16 * v.abs()) if swish else (v, off)
+
+
+@pytest.mark.parametrize("m,n,k", [(8200, 4128, 2112), (3000, 16416, 1050), (20000, 2080, 1024), (6016, 4096, 4096)])
+@pytest.mark.parametrize("epilogue", ["bias", "swish", "glu", "residual", "float"])
+def test_linear_i8_large(m, n, k, epilogue):
+    """Sizes that take the 256 x 256 form (by row bands and by flat tile ranges), ragged on every side; compared on the device."""
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    x = torch.randn((m, k), generator=g, device="cuda").to(torch.bfloat16)
+    codes = (torch.randn((n, k), generator=g, device="cuda") * 40).round().clamp(-127, 127).to(torch.int8)
+    scale = (0.5 + torch.rand((n,), generator=g, device="cuda")) / (40 * math.sqrt(k))
+    bias = torch.randn((n,), generator=g, device="cuda")
+    resid = torch.randn((m, n), generator=g, device="cuda") if epilogue == "residual" else None
+    got = ops.LinearI8.from_codes(codes, scale, bias)(x, epilogue=epilogue, resid=resid, alpha=0.5)
+    qa, _ = quantize64(x)
+    want, bound = finish64(product64(qa, x.float().abs().amax(1) / 127.0, codes, scale), bias, epilogue, resid, 0.5)
+    assert float(((got.double() - want).abs() - bound).max()) <= 0
 
 
 @pytest.mark.parametrize("rows,d,swish", [(9, 512, 0), (130, 1024, 0), (6, 4096, 1), (5, 2048, 1), (3, 256, 0), (1, 1024, 0)])
