@@ -433,8 +433,8 @@ int oasr_gemm_i8(const int8_t* a, int64_t lda, const int8_t* w_packed, const flo
                  float alpha, int32_t epilogue, void* stream);
 
 /* Both steps: the bf16 rows x (ldx apart) are quantised and multiplied.  The same bits as oasr_quant_i8_rows followed by
- * oasr_gemm_i8.  workspace: device, oasr_linear_i8_workspace_bytes(m, k), 256-byte aligned, contents on entry do not
- * matter; calls that may overlap need one each. */
+ * oasr_gemm_i8.  workspace: device, oasr_linear_i8_workspace_bytes(m, k) (0 for a few rows, which are quantised
+ * inside the product), 256-byte aligned, contents on entry do not matter; calls that may overlap need one each. */
 int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t k);
 int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const float* scale_w, const float* bias,
                    const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, float alpha,

@@ -167,7 +167,7 @@ struct Epilogue {
     __device__ __forceinline__ void load_form(const GemmArgs& p, int64_t m0, int64_t n0, int lane) {
         const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) sa[i] = FULL || m0 + 16 * i + r < p.m ? p.scale_a[m0 + 16 * i + r] : 0.f;
+        for (int i = 0; i < MT; ++i) sa[i] = p.scale_a && (FULL || m0 + 16 * i + r < p.m) ? p.scale_a[m0 + 16 * i + r] : 0.f;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             sw[j] = load_cols<FULL>(p.scale_w, n0 + 16 * j + 4 * g, p.n);
@@ -654,6 +654,103 @@ __global__ __launch_bounds__(256) void quant_i8_rows_kernel(const uint16_t* __re
     }
 }
 
+// A few tokens: quantisation and product in one launch.  Every work-group (32 columns, eight waves that split K) quantises the
+// rows itself - they are a few KiB that all of them read from L2 - into LDS, while its first weight slices are on their way;
+// the codes and scales are bit for bit those of the quantiser.  Bound by the weights' way from HBM: 16384 x 4096 at one row
+// 64 MiB; small ones by latency (a second launch would cost more than the work).
+constexpr int kFewBytes = 16384;             // rows * k at most: beyond, quantising once is cheaper
+constexpr int kFewColumns = 32;              // 64 at a time are 5 - 25 % slower at every size tried (1 x 4096 x 4096: 8.4 against 10.2 us)
+constexpr int kFewDepth = 6;                 // slices on their way (4: up to 4 % slower; 8: faster on short n, slower on long)
+constexpr int kFewItems = kFewBytes / 8 / 512;
+constexpr int kFewLds = kFewBytes + 16 * 16;
+
+template <int EPI>
+__global__ __launch_bounds__(512) void linear_i8_few_kernel(const GemmArgs p, const uint16_t* __restrict__ x, int64_t ldx, int k) {
+    constexpr int D = kFewDepth, CT = kFewColumns / 16, kSums = 8 * CT * 1024;
+    __shared__ __attribute__((aligned(1024))) char lds[kSums + 2048 > kFewLds ? kSums + 2048 : kFewLds];
+    __shared__ uint32_t row_amax[16];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (tid < 16) row_amax[tid] = 0;
+    const int64_t n0 = (int64_t)blockIdx.x * kFewColumns;
+    const int rows = (int)p.m, kp = p.ks * kSlice, pitch = kp + 16;        // 16 bytes apart: the rows' fragments in other banks
+
+    const char* src_w[CT];
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+        int64_t grp = n0 / 16 + j;
+        grp = grp < p.ng ? grp : p.ng - 1;
+        src_w[j] = reinterpret_cast<const char*>(p.w) + (grp * p.ks + wave) * kPiece + lane * 16;
+    }
+    const int count = p.ks > wave ? (p.ks - wave + 7) / 8 : 0;
+    i32x4 wf[D][CT];
+    auto request = [&](i32x4 (&w)[CT]) {
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            w[j] = *reinterpret_cast<const i32x4*>(src_w[j]);
+            src_w[j] += 8 * kPiece;
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+        if (d < count) request(wf[d]);
+    Epilogue<EPI, 1, 2> out;
+    if (wave == 0) out.load(p, 0, n0, lane);
+
+    // the rows, eight values to an item and up to four items to a thread, all requested at once; a row is a multiple of eight
+    // items, so eight neighbouring lanes always share one
+    const int per_row = kp / 8, items = rows * per_row;
+    u32x4 v[kFewItems];
+#pragma unroll
+    for (int i = 0; i < kFewItems; ++i) {
+        const int id = tid + 512 * i, r = id / per_row;
+        v[i] = id < items ? load_row8(x + r * ldx, 8 * (id - r * per_row), k) : (u32x4){0, 0, 0, 0};
+    }
+    __syncthreads();                         // row_amax is clear
+#pragma unroll
+    for (int i = 0; i < kFewItems; ++i) {
+        const int id = tid + 512 * i;
+        uint32_t amax = amax8(v[i], 0);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, o, 64));
+        if (id < items && (lane & 7) == 0) atomicMax(&row_amax[id / per_row], amax);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kFewItems; ++i) {
+        const int id = tid + 512 * i, r = id / per_row;
+        if (id >= items) break;
+        *reinterpret_cast<u32x2*>(lds + r * pitch + 8 * (id - r * per_row)) = codes8(v[i], row_scale(row_amax[r]));
+    }
+    __syncthreads();
+    const int row = min(lane & 15, rows - 1);
+    out.sa[0] = row_scale(row_amax[row]).scale;
+    const char* frag = lds + row * pitch + wave * kSlice + (lane >> 4) * 16;
+    i32x4 acc[CT] = {};
+    for (int t = 0; t < count; t += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (t + d >= count) break;
+            if (t + d + D - 1 < count) request(wf[(d + D - 1) % D]);
+            const i32x4 xf = *reinterpret_cast<const i32x4*>(frag + (t + d) * 8 * kSlice);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[d][j], xf, acc[j], 0, 0, 0);
+        }
+    }
+    __syncthreads();                         // the rows have been read
+#pragma unroll
+    for (int j = 0; j < CT; ++j) *reinterpret_cast<i32x4*>(lds + (wave * CT + j) * 1024 + lane * 16) = acc[j];
+    __syncthreads();
+    if (wave == 0) {
+        i32x4 sum[1][2] = {};
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) sum[0][j] += *reinterpret_cast<const i32x4*>(lds + (w * CT + j) * 1024 + lane * 16);
+        out.finish(p, sum, 0, n0, lane, lds + kSums);
+    }
+}
+
 // Row-major weight codes -> packed pieces, one 16-byte chunk per thread.
 __global__ __launch_bounds__(256) void gemm_pack_w_i8_kernel(const int8_t* __restrict__ w, int64_t ldw, int64_t n, int64_t k,
                                                              int64_t ks, int64_t chunks, int8_t* __restrict__ out) {
@@ -740,6 +837,24 @@ static void launch_form(int form, const GemmArgs& p, hipStream_t st) {
         default:
             hipLaunchKernelGGL((gemm_i8_wide_kernel<EPI>), dim3((unsigned)(tiles < 256 ? (tiles + 7) / 8 * 8 : 256)), dim3(512), 0, st, p, tm, tn);
     }
+}
+
+// Whether a call quantises inside the product (and needs no workspace).
+static bool few_rows(int64_t m, int64_t k) { return m <= 16 && m * round_up(k, kSlice) <= kFewBytes; }
+
+static int launch_few(const GemmArgs& p, const uint16_t* x, int64_t ldx, int64_t k, int32_t epilogue, hipStream_t st) {
+    const dim3 grid((unsigned)((p.n + kFewColumns - 1) / kFewColumns)), blk(512);
+#define OASR_FEW(E) hipLaunchKernelGGL((linear_i8_few_kernel<E>), grid, blk, 0, st, p, x, ldx, (int)k)
+    switch (epilogue) {
+        case OASR_EPI_BIAS_BF16: OASR_FEW(OASR_EPI_BIAS_BF16); break;
+        case OASR_EPI_BIAS_SWISH_BF16: OASR_FEW(OASR_EPI_BIAS_SWISH_BF16); break;
+        case OASR_EPI_GLU_BF16: OASR_FEW(OASR_EPI_GLU_BF16); break;
+        case OASR_EPI_RESIDUAL_F32: OASR_FEW(OASR_EPI_RESIDUAL_F32); break;
+        default: OASR_FEW(OASR_EPI_BIAS_F32); break;
+    }
+#undef OASR_FEW
+    OASR_CHECK_LAUNCH("linear_i8");
+    return OASR_OK;
 }
 
 static int launch_gemm(const GemmArgs& p, int32_t epilogue, hipStream_t st) {
@@ -851,7 +966,7 @@ int oasr_gemm_i8(const int8_t* a, int64_t lda, const int8_t* w_packed, const flo
 }
 
 int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t k) {
-    if (m <= 0 || k <= 0) return 0;
+    if (m <= 0 || k <= 0 || i8::few_rows(m, k)) return 0;
     return round_up(m * round_up(k, i8::kSlice), 256) + round_up(m * 4, 256);
 }
 
@@ -862,8 +977,12 @@ int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const
     if (rc != OASR_OK) return rc;
     OASR_REQUIRE(ldx >= k, "linear_i8: ldx must cover k");
     if (m == 0) return OASR_OK;
-    OASR_REQUIRE(x && workspace, "linear_i8: null pointer");
-    OASR_REQUIRE(((uintptr_t)x & 1) == 0 && ((uintptr_t)workspace & 255) == 0, "linear_i8: misaligned pointer (workspace: 256 bytes)");
+    OASR_REQUIRE(x, "linear_i8: null pointer");
+    OASR_REQUIRE(((uintptr_t)x & 1) == 0, "linear_i8: misaligned pointer");
+    if (i8::few_rows(m, k))
+        return i8::launch_few(i8::gemm_args(nullptr, 0, w_packed, nullptr, scale_w, bias, resid, ldr, c, ldc, m, n, k, alpha, epilogue), x,
+                              ldx, k, epilogue, (hipStream_t)stream);
+    OASR_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0, "linear_i8: workspace missing or not 256-byte aligned");
     if (workspace_bytes < oasr_linear_i8_workspace_bytes(m, k)) {
         set_error("linear_i8: workspace needs %lld bytes, got %lld", (long long)oasr_linear_i8_workspace_bytes(m, k),
                   (long long)workspace_bytes);

@@ -52,6 +52,59 @@ constexpr uint32_t kOrderedLowest = 0x00800000u;  // ordered(kLowest): -inf lies
 
 __device__ __forceinline__ bool before(uint32_t va, uint32_t ia, uint32_t vb, uint32_t ib) { return va > vb || (va == vb && ia < ib); }
 
+// Reductions over aligned groups of lanes without LDS: neighbours by data-parallel moves inside a row of 16 lanes (the mirrored
+// partner serves as well as the exclusive-or one, since its four or eight lanes agree by then), rows by lane swaps.  `op` takes
+// two values of any struct of 32-bit words and must be symmetric.  Every lane ends with the group's result.
+template <int CTRL, typename T>
+__device__ __forceinline__ T lane_move(const T& v) {
+    constexpr int N = sizeof(T) / 4;
+    int w[N];
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_update_dpp(0, w[i], CTRL, 0xf, 0xf, true);
+    T r;
+    __builtin_memcpy(&r, w, sizeof(T));
+    return r;
+}
+template <bool HALVES, typename T>
+__device__ __forceinline__ void lane_swap(const T& v, T& a, T& b) {     // rows 0 1 2 3 -> a: 0 0 2 2, b: 1 1 3 3 (halves alike)
+    constexpr int N = sizeof(T) / 4;
+    unsigned w[N], wa[N], wb[N];
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const auto p = HALVES ? __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false)
+                              : __builtin_amdgcn_permlane16_swap(w[i], w[i], false, false);
+        wa[i] = p[0];
+        wb[i] = p[1];
+    }
+    __builtin_memcpy(&a, wa, sizeof(T));
+    __builtin_memcpy(&b, wb, sizeof(T));
+}
+template <typename T, typename Op>
+__device__ __forceinline__ T group_reduce(T v, int lanes, Op op) {      // lanes: 1, 2, 4 .. 64, uniform
+    if (lanes > 1) v = op(v, lane_move<0xB1>(v));       // quad_perm [1 0 3 2]
+    if (lanes > 2) v = op(v, lane_move<0x4E>(v));       // quad_perm [2 3 0 1]
+    if (lanes > 4) v = op(v, lane_move<0x141>(v));      // row_half_mirror
+    if (lanes > 8) v = op(v, lane_move<0x140>(v));      // row_mirror
+    T a, b;
+    if (lanes > 16) {
+        lane_swap<false>(v, a, b);
+        v = op(a, b);
+    }
+    if (lanes > 32) {
+        lane_swap<true>(v, a, b);
+        v = op(a, b);
+    }
+    return v;
+}
+struct Pick {
+    uint32_t value, index;      // ordered value; the lower index wins a tie
+};
+__device__ __forceinline__ Pick better(const Pick& a, const Pick& b) { return before(b.value, b.index, a.value, a.index) ? b : a; }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
+
 // 16 bytes of logits from any element's address.
 template <typename E>
 struct Chunk;
@@ -136,7 +189,7 @@ __global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, i
     float m = kLowest;
 #pragma unroll
     for (int j = 0; j < 4 * C; ++j) m = fmaxf(m, z[j]);
-    for (int o = group >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    m = group_reduce(m, group, larger);
     float s = 0.f, t = 0.f;
 #pragma unroll
     for (int j = 0; j < 4 * C; ++j) {
@@ -145,10 +198,8 @@ __global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, i
         s += z[j] == z[j] && m < INFINITY ? e : nan32();
         t = fmaf(e, d, t);
     }
-    for (int o = group >> 1; o > 0; o >>= 1) {
-        s += __shfl_xor(s, o, 64);
-        t += __shfl_xor(t, o, 64);
-    }
+    s = group_reduce(s, group, sum_of);
+    t = group_reduce(t, group, sum_of);
     const float log_s = logf(s);
     if (live && p.given > 0)
         for (int i = sub; i < p.given; i += group) {
@@ -161,27 +212,18 @@ __global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, i
     const bool usable = src >= 0 && s == s;
     uint32_t taken = 0;                               // this lane's values that are out already
     for (int k = 0; k < p.top; ++k) {
-        uint32_t v = 0, idx = 0xffffffffu;
+        Pick best = {0, 0xffffffffu};
 #pragma unroll
         for (int j = 0; j < 4 * C; ++j) {
             const uint32_t u = ordered(z[j]), at = 4 * (sub + (j >> 2) * group) + (j & 3);
-            if (!(taken >> j & 1) && u >= kOrderedLowest && before(u, at, v, idx)) {
-                v = u;
-                idx = at;
-            }
+            if (!(taken >> j & 1) && u >= kOrderedLowest) best = better(best, {u, at});
         }
-        for (int o = group >> 1; o > 0; o >>= 1) {
-            const uint32_t ov = __shfl_xor(v, o, 64), oi = __shfl_xor(idx, o, 64);
-            if (before(ov, oi, v, idx)) {
-                v = ov;
-                idx = oi;
-            }
-        }
+        best = group_reduce(best, group, better);
 #pragma unroll
         for (int j = 0; j < 4 * C; ++j)
-            if (idx == 4 * (sub + (j >> 2) * group) + (j & 3)) taken |= 1u << j;
+            if (best.index == 4 * (sub + (j >> 2) * group) + (j & 3)) taken |= 1u << j;
         if (live && sub == 0) {
-            if (usable && v) write_best(p, r, k, v, idx, m, log_s);
+            if (usable && best.value) write_best(p, r, k, best.value, best.index, m, log_s);
             else write_none(p, r, k, src == -1 || usable ? -INFINITY : nan32());
         }
     }
@@ -200,7 +242,7 @@ __device__ __forceinline__ void add_values(Sums& a, float& top, const float (&z)
     for (int j = 1; j < N; ++j) b = fmaxf(b, z[j]);
     top = fmaxf(top, b);
     if (__any(b > a.m)) {
-        const float m = fmaxf(a.m, wave_max(b));
+        const float m = fmaxf(a.m, group_reduce(b, 64, larger));
         const float d = fminf(m - a.m, kLargest), f = __builtin_amdgcn_exp2f(d * -kLog2e);
         a.t = f > 0.f ? f * fmaf(d, a.s, a.t) : 0.f * a.s;     // NaN stays NaN
         a.s *= f;
@@ -228,12 +270,14 @@ __device__ __forceinline__ void join(Sums& a, const Sums& b) {
     a = {m, s0 + s1, t0 + t1};
 }
 
-// The largest value that at least `count` lanes of the wave reach.
+// A value that at least `count` lanes of the wave reach, and as few more as the ties of the count-th largest make.
 __device__ __forceinline__ uint32_t wave_nth_largest(uint32_t v, int count) {
     uint32_t at = 0;
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t trial = at | 1u << bit;
-        if (__popcll(__ballot(v >= trial)) >= count) at = trial;
+        const int reach = __popcll(__ballot(v >= trial));
+        if (reach >= count) at = trial;
+        if (reach == count) break;
     }
     return at;
 }
@@ -288,8 +332,8 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
         const float z[1] = {tid < tail ? Chunk<E>::one(row + (int64_t)chunks * N + tid) : -INFINITY};
         add_values(a, top, z);
     }
-    a.s = wave_sum(a.s);
-    a.t = wave_sum(a.t);
+    a.s = group_reduce(a.s, 64, sum_of);
+    a.t = group_reduce(a.t, 64, sum_of);
     // A bound that at least `top` values reach: the least over the waves of each wave's ceil(top / W)-th largest lane.
     const uint32_t mine = ordered(top);
     const uint32_t reach = p.top > 0 ? wave_nth_largest(mine, (p.top + W - 1) / W) : 0;
@@ -381,15 +425,8 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
             for (int e = 0; e < N; ++e) look(z[e], (uint32_t)c * N + e);
         }
         if (tid < tail) look(Chunk<E>::one(row + (int64_t)chunks * N + tid), (uint32_t)chunks * N + tid);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint32_t ov = __shfl_xor(v, o, 64), oi = __shfl_xor(idx, o, 64);
-            if (before(ov, oi, v, idx)) {
-                v = ov;
-                idx = oi;
-            }
-        }
-        if (lane == 0) wave_pick[wave] = make_uint2(v, idx);
+        const Pick best = group_reduce(Pick{v, idx}, 64, better);
+        if (lane == 0) wave_pick[wave] = make_uint2(best.value, best.index);
         __syncthreads();
         last = wave_pick[0];
         for (int w = 1; w < W; ++w)
@@ -403,23 +440,24 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
     }
 }
 
-// Joins the splits of a row: one wave per row, lane s holds split s and the head of its list.
+// Joins the splits of a row: one wave per row, lane s holds split s and, in LDS, its list.
 template <typename E>
 __global__ __launch_bounds__(64) void token_scores_join_kernel(const Args p) {
+    __shared__ uint2 lists[kMaxSplits * kMaxTop];
     const int lane = threadIdx.x;
     const int64_t r = blockIdx.x, src = source_row(p, r);
     if (src < 0) return;                                        // written by the first split
     const E* row = reinterpret_cast<const E*>(p.logits) + src * p.ld;
+    for (int i = lane; i < p.splits * p.top; i += 64) lists[i] = p.cand[r * p.splits * p.top + i];
     Sums a = {kLowest, 0.f, 0.f};
     if (lane < p.splits) {
         const float* o = p.part + (r * p.splits + lane) * 4;
         a = {o[0], o[1], o[2]};
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const Sums b = {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)};
-        join(a, b);
-    }
+    a = group_reduce(a, 64, [](Sums x, const Sums& y) {
+        join(x, y);
+        return x;
+    });
     const float log_s = logf(a.s);
     for (int i = lane; i < p.given; i += 64)
         p.logprobs[r * p.given + i] = token_logprob(row, p.vocab, p.tokens[r * p.given + i], a.m, a.s, log_s);
@@ -429,27 +467,18 @@ __global__ __launch_bounds__(64) void token_scores_join_kernel(const Args p) {
         if (lane < p.top) write_none(p, r, lane, nan32());
         return;
     }
-    const uint2* list = p.cand + (r * p.splits + (lane < p.splits ? lane : 0)) * p.top;
-    int at = 0;
-    uint2 head = lane < p.splits ? list[0] : make_uint2(0, 0xffffffffu);
+    __syncthreads();
+    const uint2 none = make_uint2(0, 0xffffffffu);
+    int at = lane * p.top;
+    const int end = lane < p.splits ? at + p.top : at;
+    uint2 head = at < end ? lists[at] : none;
     for (int k = 0; k < p.top; ++k) {
-        uint32_t v = head.x, idx = head.y;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint32_t ov = __shfl_xor(v, o, 64), oi = __shfl_xor(idx, o, 64);
-            if (before(ov, oi, v, idx)) {
-                v = ov;
-                idx = oi;
-            }
-        }
+        const Pick best = group_reduce(Pick{head.x, head.y}, 64, better);
         if (lane == 0) {
-            if (v) write_best(p, r, k, v, idx, a.m, log_s);
+            if (best.value) write_best(p, r, k, best.value, best.index, a.m, log_s);
             else write_none(p, r, k, -INFINITY);
         }
-        if (v && head.x == v && head.y == idx) {                // the winner's next
-            ++at;
-            head = at < p.top ? list[at] : make_uint2(0, 0xffffffffu);
-        }
+        if (best.value && head.x == best.value && head.y == best.index) head = ++at < end ? lists[at] : none;   // the winner's next
     }
 }
 

@@ -19,6 +19,7 @@ from .weights import quantize_rows_i8
 
 EPILOGUES = {"bias": _hip.EPI_BIAS_BF16, "swish": _hip.EPI_BIAS_SWISH_BF16, "glu": _hip.EPI_GLU_BF16,
              "residual": _hip.EPI_RESIDUAL_F32, "float": _hip.EPI_BIAS_F32}
+_INT8, _FLOAT32, _BFLOAT16, _LOGITS = (torch.int8,), (torch.float32,), (torch.bfloat16,), (torch.float32, torch.bfloat16)
 _NORM_WIDTHS = (256, 512, 1024, 2048, 4096)
 _NULL = contextlib.nullcontext()
 
@@ -28,17 +29,20 @@ def _on(device: torch.device):
     return _NULL if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def _rows(t, what: str, dtype):
+def _rows(t, what: str, dtypes: tuple):
     """(tensor, rows, columns, row pitch) of a [..., columns] tensor whose rows are contiguous and evenly spaced."""
-    if not isinstance(t, torch.Tensor) or t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
-        raise ValueError(f"{what} must be a {dtype} tensor")
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+        raise ValueError(f"{what} must be a tensor of {' or '.join(map(str, dtypes))}")
     if not t.is_cuda:
         raise ValueError(f"{what} must be on a HIP device; there is no CPU fallback")
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ValueError(f"{what} must have at least one column")
+    cols = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // cols, cols, cols
     if t.dim() != 2:
-        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
-    rows, cols = t.shape
+        t = t.reshape(math.prod(t.shape[:-1]), cols)
+    rows = t.shape[0]
     pitch = t.stride(0) if rows > 1 else cols
     if cols > 1 and t.stride(1) != 1 or pitch < cols:
         raise ValueError(f"{what} must have contiguous rows that do not overlap")
@@ -88,7 +92,7 @@ class LinearI8:
     def _lay_out(self, codes, scale, bias):
         if codes.dim() != 2:
             raise ValueError("codes must be [out, in]")
-        codes, n, k, ldw = _rows(codes, "codes", torch.int8)
+        codes, n, k, ldw = _rows(codes, "codes", _INT8)
         if n < 1 or not 1 <= k <= 131072:
             raise ValueError("a weight has at least one row and 1 to 131072 columns")
         self.device, self.out_features, self.in_features = codes.device, n, k
@@ -113,14 +117,16 @@ class LinearI8:
             if n % 32:
                 raise ValueError("the GLU epilogue needs a multiple of 32 output rows")
             n //= 2
-        dtype = torch.float32 if epi in (_hip.EPI_RESIDUAL_F32, _hip.EPI_BIAS_F32) else torch.bfloat16
+        dtype = torch.float32 if epi >= _hip.EPI_RESIDUAL_F32 else torch.bfloat16
         shape = (*x.shape[:-1], n)
         given = out is not None
         if not given:
-            out = torch.empty(shape, dtype=dtype, device=self.device)
+            out = x.new_empty(shape, dtype=dtype)
+            if epi != _hip.EPI_RESIDUAL_F32 and resid is None:
+                return epi, out, n, None, 0
         elif out.shape != shape or out.device != self.device:
             raise ValueError(f"out must be of shape {shape} on {self.device}")
-        flat, _, _, ldc = _rows(out, "out", dtype)
+        flat, _, _, ldc = _rows(out, "out", (dtype,))
         if given and flat.data_ptr() != out.data_ptr():
             raise ValueError("out must have evenly spaced rows")
         if given and _overlap(flat, x):
@@ -131,7 +137,7 @@ class LinearI8:
             return epi, out, ldc, None, 0
         if resid is None or resid.shape != shape or resid.device != self.device:
             raise ValueError(f"the residual epilogue needs resid of shape {shape} on {self.device}")
-        r, _, _, ldr = _rows(resid, "resid", torch.float32)
+        r, _, _, ldr = _rows(resid, "resid", _FLOAT32)
         if given and _overlap(flat, r) and (r.data_ptr() != flat.data_ptr() or ldr != ldc):
             raise ValueError("resid may be out itself, or must not overlap it")
         return epi, out, ldc, r, ldr
@@ -139,7 +145,7 @@ class LinearI8:
     def __call__(self, x: torch.Tensor, *, epilogue: str = "bias", resid: torch.Tensor | None = None, alpha: float = 1.0,
                  out: torch.Tensor | None = None) -> torch.Tensor:
         """x bf16 [..., in] -> [..., out].  `out` may be given (rows evenly spaced) and may be `resid`."""
-        x2, m, k, ldx = _rows(x, "x", torch.bfloat16)
+        x2, m, k, ldx = _rows(x, "x", _BFLOAT16)
         if k != self.in_features or x.device != self.device:
             raise ValueError(f"x must have {self.in_features} columns on {self.device}")
         epi, out, ldc, resid, ldr = self._output(x, epilogue, resid, out)
@@ -148,17 +154,18 @@ class LinearI8:
         L = _hip.lib()
         with _on(self.device):
             ws_bytes = int(L.oasr_linear_i8_workspace_bytes(m, k))
-            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=self.device)
+            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=self.device) if ws_bytes else None
             _hip.check(L.oasr_linear_i8(x2.data_ptr(), ldx, self._packed_ptr, self._scale_ptr, self._bias_ptr,
                                         None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m,
-                                        self.out_features, k, alpha, epi, ws.data_ptr(), ws_bytes, _hip.current_stream_ptr()), "oasr_linear_i8")
+                                        self.out_features, k, alpha, epi, None if ws is None else ws.data_ptr(),
+                                        ws_bytes, _hip.current_stream_ptr()), "oasr_linear_i8")
         return out
 
     def normed(self, x: torch.Tensor, gain: torch.Tensor, shift: torch.Tensor, *, eps: float = 1e-5, epilogue: str = "bias",
                resid: torch.Tensor | None = None, alpha: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
         """The layer on LayerNorm(x) * gain + shift: x float32 [..., in] contiguous, in 256, 512, 1024, 2048 or 4096.  The
         normalised rows go to 8-bit integers without being stored in between."""
-        x2, m, k, ldx = _rows(x, "x", torch.float32)
+        x2, m, k, ldx = _rows(x, "x", _FLOAT32)
         if k != self.in_features or x.device != self.device:
             raise ValueError(f"x must have {self.in_features} columns on {self.device}")
         if k not in _NORM_WIDTHS or ldx != k or x2.data_ptr() % 16:
@@ -197,12 +204,11 @@ def _int32(t, shape, what: str, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _score_outputs(lead, given, alternatives, device):
+def _score_outputs(lead, given, alternatives, like):
     if not 0 <= alternatives <= MAX_ALTERNATIVES:
         raise ValueError(f"alternatives must lie in [0, {MAX_ALTERNATIVES}]")
-    f32 = lambda shape: torch.empty(shape, dtype=torch.float32, device=device)  # noqa: E731
-    return TokenScores(f32(given), f32(lead), torch.empty((*lead, alternatives), dtype=torch.int32, device=device),
-                       f32((*lead, alternatives)))
+    new, f32, listed = like.new_empty, torch.float32, (*lead, alternatives)
+    return TokenScores(new(given, dtype=f32), new(lead, dtype=f32), new(listed, dtype=torch.int32), new(listed, dtype=f32))
 
 
 def _score_workspace(rows, vocab, alternatives, device):
@@ -214,7 +220,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, al
     """Log probabilities of given tokens under rows of logits [..., vocab] (float32 or bfloat16; rows evenly spaced), with
     every row's entropy and its `alternatives` likeliest tokens.  `tokens`: int32 [...] or [..., n]; a negative one means
     none (0).  Masked logits (-inf) have probability 0 and are no alternatives; include/oasr.h says what else rows hold."""
-    z, rows, vocab, ld = _rows(logits, "logits", (torch.float32, torch.bfloat16))
+    z, rows, vocab, ld = _rows(logits, "logits", _LOGITS)
     lead, device = logits.shape[:-1], logits.device
     given, n = (*lead, 0), 0
     if tokens is not None:
@@ -222,7 +228,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, al
         if given != lead and given[:-1] != lead:
             raise ValueError(f"tokens must be of shape {tuple(lead)} or {tuple(lead)} and one more dimension")
         tokens, n = _int32(tokens, given, "tokens", device), 1 if given == lead else given[-1]
-    out = _score_outputs(lead, given, alternatives, device)
+    out = _score_outputs(lead, given, alternatives, logits)
     if rows == 0:
         return out
     with _on(device):
@@ -243,7 +249,7 @@ def ctc_token_scores(logits: torch.Tensor, tokens: torch.Tensor, frames: torch.T
     if not isinstance(logits, torch.Tensor) or logits.dim() != 3 or not logits.is_contiguous():
         raise ValueError("logits must be a contiguous tensor [batch, frames, pitch]")
     batch, t_pad, ld = logits.shape
-    _rows(logits, "logits", (torch.float32, torch.bfloat16))
+    _rows(logits, "logits", _LOGITS)
     vocab = ld if vocab is None else int(vocab)
     if not 1 <= vocab <= ld:
         raise ValueError(f"vocab must lie in [1, {ld}]")
@@ -253,7 +259,7 @@ def ctc_token_scores(logits: torch.Tensor, tokens: torch.Tensor, frames: torch.T
     tokens, frames = _int32(tokens, shape, "tokens", device), _int32(frames, shape, "frames", device)
     if t_pad == 0 and tokens.numel():
         raise ValueError("logits have no frames")
-    out = _score_outputs(shape, shape, alternatives, device)
+    out = _score_outputs(shape, shape, alternatives, logits)
     if tokens.numel() == 0:
         return out
     with _on(device):
