@@ -10,7 +10,7 @@
 // Ties go to the lower index: candidates are ranked by (value, index), never by the order in which they were found.
 //
 // Bandwidth-bound for rows that number in the hundreds (2 or 4 bytes per logit against about ten issue slots), bound by
-// latency below.  Rows up to 1024 tokens stay in the registers of a group of lanes; longer ones are streamed by a
+// latency below.  Rows up to 2048 tokens stay in the registers of a group of lanes; longer ones are streamed by a
 // work-group each, or by several where rows are few, whose results a second launch joins.
 #include "oasr_common.h"
 
@@ -22,6 +22,7 @@ constexpr float kLargest = 3.402823466e38f;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxTop = 32;
 constexpr int kMaxSplits = 64;
+constexpr int kShort = 2048;                      // tokens that a wave holds in registers
 constexpr int kCandidates = 512;                  // kept in LDS per row before ranking
 
 struct Args {
@@ -169,34 +170,87 @@ __device__ __forceinline__ void write_none(const Args& p, int64_t r, int at, flo
     p.best[r * p.top + at] = value;
 }
 
+// A value that at least `count` lanes of the wave reach, and as few more as the ties of the count-th largest make.
+__device__ __forceinline__ uint32_t wave_nth_largest(uint32_t v, int count) {
+    uint32_t at = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = at | 1u << bit;
+        const int reach = __popcll(__ballot(v >= trial));
+        if (reach >= count) at = trial;
+        if (reach == count) break;
+    }
+    return at;
+}
+
+// Orders a wave's own LDS writes before its reads of them.
+#define OASR_SCORES_WAVE_LDS()                                          \
+    do {                                                                \
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local"); \
+        __builtin_amdgcn_wave_barrier();                                \
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local"); \
+    } while (0)
+
 // ---- short rows: a group of 2^g lanes holds a row in registers, C chunks of four per lane -----------------------------
+// Four consecutive values, of which the first `left` exist (the rest -inf).
+template <typename E>
+__device__ __forceinline__ void load_four(const E* p, int left, float (&z)[4]);
+template <>
+__device__ __forceinline__ void load_four<float>(const float* p, int left, float (&z)[4]) {
+    if (left >= 4) {
+        Chunk<float>::load(p, z);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = e < left ? p[e] : -INFINITY;
+    }
+}
+template <>
+__device__ __forceinline__ void load_four<uint16_t>(const uint16_t* p, int left, float (&z)[4]) {
+    struct __attribute__((packed, aligned(2))) Raw {
+        uint32_t v[2];
+    };
+    if (left >= 4) {
+        const Raw r = *reinterpret_cast<const Raw*>(p);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            z[2 * e] = __uint_as_float(r.v[e] << 16);
+            z[2 * e + 1] = __uint_as_float(r.v[e] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = e < left ? bf2f(p[e]) : -INFINITY;
+    }
+}
+
 template <typename E, int C>
 __global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, int lanes_log2) {
-    const int lane = threadIdx.x & 63, group = 1 << lanes_log2, sub = lane & (group - 1);
-    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t r = (wave << (6 - lanes_log2)) + (lane >> lanes_log2);
+    constexpr int kList = C > 1 ? 64 : 1;             // candidates of a wave's row, where a row takes the whole wave
+    __shared__ Pick lists[4][kList];
+    const int lane = threadIdx.x & 63, group = C > 1 ? 64 : 1 << lanes_log2, sub = lane & (group - 1);
+    const int wave_in = threadIdx.x >> 6;
+    const int64_t wave = (int64_t)blockIdx.x * 4 + wave_in;
+    const int64_t r = C > 1 ? wave : (wave << (6 - lanes_log2)) + (lane >> lanes_log2);
     const bool live = r < p.rows;
     const int64_t src = live ? source_row(p, r) : -1;
     const E* row = reinterpret_cast<const E*>(p.logits) + (src < 0 ? 0 : src) * p.ld;
     float z[4 * C];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+        const int at = 4 * (sub + c * group);
+        float four[4];
+        load_four<E>(row + at, src >= 0 ? p.vocab - at : 0, four);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int at = 4 * (sub + c * group) + e;
-            z[4 * c + e] = src >= 0 && at < p.vocab ? Chunk<E>::one(row + at) : -INFINITY;
-        }
-    float m = kLowest;
+        for (int e = 0; e < 4; ++e) z[4 * c + e] = four[e];
+    }
+    float own = z[0];
 #pragma unroll
-    for (int j = 0; j < 4 * C; ++j) m = fmaxf(m, z[j]);
-    m = group_reduce(m, group, larger);
+    for (int j = 1; j < 4 * C; ++j) own = fmaxf(own, z[j]);
+    const float m = group_reduce(fmaxf(own, kLowest), group, larger);
     float s = 0.f, t = 0.f;
 #pragma unroll
     for (int j = 0; j < 4 * C; ++j) {
-        const float d = fminf(m - z[j], kLargest), e = __builtin_amdgcn_exp2f(d * -kLog2e);
-        // a NaN must survive the minimum
-        s += z[j] == z[j] && m < INFINITY ? e : nan32();
-        t = fmaf(e, d, t);
+        const float x = m - z[j], e = __builtin_amdgcn_exp2f(x * -kLog2e);      // NaN for NaN, and for +inf against itself
+        s += e;
+        t = fmaf(e, fminf(x, kLargest), t);
     }
     s = group_reduce(s, group, sum_of);
     t = group_reduce(t, group, sum_of);
@@ -209,14 +263,44 @@ __global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, i
             p.logprobs[r * p.given + i] = v;
         }
     if (live && p.entropy && sub == 0) p.entropy[r] = src >= 0 ? row_entropy(s, t, log_s) : (src == -2 ? nan32() : 0.f);
+    if (p.top == 0) return;
     const bool usable = src >= 0 && s == s;
+    const float absent = src == -1 || usable ? -INFINITY : nan32();
+    uint32_t least = kOrderedLowest;
+    if (C > 1) {
+        // a whole wave per row: the values that reach the top-th largest of the lanes' own largest go to a list, and are
+        // ranked there; a list that overflows (ties) is left, and the rounds below take its place
+        const uint32_t bound = max(wave_nth_largest(ordered(own), p.top), kOrderedLowest);
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 4 * C; ++j) {
+            const uint32_t u = ordered(z[j]);
+            const uint64_t hits = __ballot(usable && u >= bound);
+            const int at = n + __popcll(hits & ((1ull << lane) - 1));
+            if ((hits >> lane & 1) && at < kList) lists[wave_in][at] = {u, (uint32_t)(4 * (sub + (j >> 2) * group) + (j & 3))};
+            n += __popcll(hits);
+        }
+        if (n <= kList) {
+            OASR_SCORES_WAVE_LDS();
+            if (!live) return;
+            if (lane < n) {
+                const Pick me = lists[wave_in][lane];
+                int rank = 0;
+                for (int o = 0; o < n; ++o) rank += before(lists[wave_in][o].value, lists[wave_in][o].index, me.value, me.index);
+                if (rank < p.top) write_best(p, r, rank, me.value, me.index, m, log_s);
+            }
+            if (lane >= n && lane < p.top) write_none(p, r, lane, absent);
+            return;
+        }
+        least = bound;
+    }
     uint32_t taken = 0;                               // this lane's values that are out already
     for (int k = 0; k < p.top; ++k) {
         Pick best = {0, 0xffffffffu};
 #pragma unroll
         for (int j = 0; j < 4 * C; ++j) {
             const uint32_t u = ordered(z[j]), at = 4 * (sub + (j >> 2) * group) + (j & 3);
-            if (!(taken >> j & 1) && u >= kOrderedLowest) best = better(best, {u, at});
+            if (!(taken >> j & 1) && u >= least) best = better(best, {u, at});
         }
         best = group_reduce(best, group, better);
 #pragma unroll
@@ -224,7 +308,7 @@ __global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, i
             if (best.index == 4 * (sub + (j >> 2) * group) + (j & 3)) taken |= 1u << j;
         if (live && sub == 0) {
             if (usable && best.value) write_best(p, r, k, best.value, best.index, m, log_s);
-            else write_none(p, r, k, src == -1 || usable ? -INFINITY : nan32());
+            else write_none(p, r, k, absent);
         }
     }
 }
@@ -270,23 +354,12 @@ __device__ __forceinline__ void join(Sums& a, const Sums& b) {
     a = {m, s0 + s1, t0 + t1};
 }
 
-// A value that at least `count` lanes of the wave reach, and as few more as the ties of the count-th largest make.
-__device__ __forceinline__ uint32_t wave_nth_largest(uint32_t v, int count) {
-    uint32_t at = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t trial = at | 1u << bit;
-        const int reach = __popcll(__ballot(v >= trial));
-        if (reach >= count) at = trial;
-        if (reach == count) break;
-    }
-    return at;
-}
-
 template <typename E, int T, bool SPLIT>
 __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
     constexpr int N = Chunk<E>::N, W = T / 64, U = 16 / N;      // U chunks = 16 values per lane and step
     __shared__ Sums wave_sums[W];
-    __shared__ uint32_t wave_bound[W], found;
+    __shared__ uint32_t wave_bound[W], found, holding;
+    __shared__ uint16_t holders[T];
     __shared__ uint2 cand[kCandidates];
     __shared__ uint2 wave_pick[W];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -315,22 +388,27 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
     for (; base + U * T <= hi; base += U * T) {
         float z[16];
 #pragma unroll
-        for (int u = 0; u < U; ++u) Chunk<E>::load(row + (int64_t)(base + u * T + tid) * N, *reinterpret_cast<float(*)[N]>(&z[u * N]));
-        add_values(a, top, z);
-    }
-    for (; base < hi; base += T) {
-        float z[N];
-        if (base + tid < hi) {
-            Chunk<E>::load(row + (int64_t)(base + tid) * N, z);
-        } else {
+        for (int u = 0; u < U; ++u) {
+            float some[N];
+            Chunk<E>::load(row + (int64_t)(base + u * T + tid) * N, some);
 #pragma unroll
-            for (int e = 0; e < N; ++e) z[e] = -INFINITY;
+            for (int e = 0; e < N; ++e) z[u * N + e] = some[e];
         }
         add_values(a, top, z);
     }
-    {
-        const float z[1] = {tid < tail ? Chunk<E>::one(row + (int64_t)chunks * N + tid) : -INFINITY};
-        add_values(a, top, z);
+    for (; base < hi; base += T) {
+        float some[N];
+        if (base + tid < hi) {
+            Chunk<E>::load(row + (int64_t)(base + tid) * N, some);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) some[e] = -INFINITY;
+        }
+        add_values(a, top, some);
+    }
+    if (tail) {                                                 // uniform
+        const float last[1] = {tid < tail ? Chunk<E>::one(row + (int64_t)chunks * N + tid) : -INFINITY};
+        add_values(a, top, last);
     }
     a.s = group_reduce(a.s, 64, sum_of);
     a.t = group_reduce(a.t, 64, sum_of);
@@ -341,7 +419,7 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
         wave_sums[wave] = a;
         wave_bound[wave] = reach;
     }
-    if (tid == 0) found = 0;
+    if (tid == 0) found = holding = 0;
     __syncthreads();
     a = wave_sums[0];
     uint32_t bound = wave_bound[0];
@@ -378,7 +456,8 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
         if (tid < p.top) emit_none(tid);
         return;
     }
-    // Every value at or above the bound becomes a candidate; only lanes whose own largest reaches it read again.
+    // Every value at or above the bound becomes a candidate.  Only lanes whose own largest reaches it hold any; their shares
+    // (`each` chunks, T apart) are read again by the whole work-group, a chunk per thread, so that it costs one latency.
     auto offer = [&](float z, uint32_t index) {
         const uint32_t u = ordered(z);
         if (u >= bound) {
@@ -386,15 +465,20 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
             if (at < kCandidates) cand[at] = make_uint2(u, index);
         }
     };
-    if (mine >= bound) {
-        for (int c = lo + tid; c < hi; c += T) {
-            float z[N];
-            Chunk<E>::load(row + (int64_t)c * N, z);
+    if (mine >= bound) holders[atomicAdd(&holding, 1u)] = (uint16_t)tid;
+    __syncthreads();
+    const uint32_t each = (uint32_t)(hi - lo + T - 1) / T, reads = holding * each;
+    for (uint32_t i = tid; i < reads; i += T) {
+        const uint32_t q = i / each;
+        const int c = lo + holders[q] + (int)(i - q * each) * T;
+        if (c < hi) {
+            float some[N];
+            Chunk<E>::load(row + (int64_t)c * N, some);
 #pragma unroll
-            for (int e = 0; e < N; ++e) offer(z[e], (uint32_t)c * N + e);
+            for (int e = 0; e < N; ++e) offer(some[e], (uint32_t)c * N + e);
         }
-        if (tid < tail) offer(Chunk<E>::one(row + (int64_t)chunks * N + tid), (uint32_t)chunks * N + tid);
     }
+    if (mine >= bound && tid < tail) offer(Chunk<E>::one(row + (int64_t)chunks * N + tid), (uint32_t)chunks * N + tid);
     __syncthreads();
     const int n = (int)found;
     if (n <= kCandidates) {
@@ -443,7 +527,9 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
 // Joins the splits of a row: one wave per row, lane s holds split s and, in LDS, its list.
 template <typename E>
 __global__ __launch_bounds__(64) void token_scores_join_kernel(const Args p) {
+    constexpr int kJoined = 128;
     __shared__ uint2 lists[kMaxSplits * kMaxTop];
+    __shared__ Pick joined[kJoined];
     const int lane = threadIdx.x;
     const int64_t r = blockIdx.x, src = source_row(p, r);
     if (src < 0) return;                                        // written by the first split
@@ -468,8 +554,33 @@ __global__ __launch_bounds__(64) void token_scores_join_kernel(const Args p) {
         return;
     }
     __syncthreads();
+    // A value that at least `top` entries reach: of each list the first `depth`, of enough lists.  What reaches it - few entries
+    // more than `top`, as a rule - is collected and ranked; ties may make it too many, and then the heads are picked in turn.
+    const int depth = (p.top + p.splits - 1) / p.splits, first = lane * p.top;
+    const uint32_t mark = lane < p.splits ? lists[first + depth - 1].x : 0;
+    const uint32_t bound = max(wave_nth_largest(mark, (p.top + depth - 1) / depth), 1u);       // 0: no entry
+    int n = 0;
+    for (int e = 0; e < p.top; ++e) {
+        const uint2 entry = lane < p.splits ? lists[first + e] : make_uint2(0, 0);
+        const uint64_t hits = __ballot(entry.x >= bound);
+        if (!hits) break;
+        const int at = n + __popcll(hits & ((1ull << lane) - 1));
+        if (entry.x >= bound && at < kJoined) joined[at] = {entry.x, entry.y};
+        n += __popcll(hits);
+    }
+    __syncthreads();
+    if (n <= kJoined) {
+        for (int c = lane; c < n; c += 64) {
+            const Pick me = joined[c];
+            int rank = 0;
+            for (int o = 0; o < n; ++o) rank += before(joined[o].value, joined[o].index, me.value, me.index);
+            if (rank < p.top) write_best(p, r, rank, me.value, me.index, a.m, log_s);
+        }
+        for (int k = n + lane; k < p.top; k += 64) write_none(p, r, k, -INFINITY);
+        return;
+    }
     const uint2 none = make_uint2(0, 0xffffffffu);
-    int at = lane * p.top;
+    int at = first;
     const int end = lane < p.splits ? at + p.top : at;
     uint2 head = at < end ? lists[at] : none;
     for (int k = 0; k < p.top; ++k) {
@@ -482,13 +593,14 @@ __global__ __launch_bounds__(64) void token_scores_join_kernel(const Args p) {
     }
 }
 
-// Work-groups per row: rows that fill the chip by themselves are not cut; a part has at least 4096 tokens.
+// Work-groups per row.  Cutting a row costs a second launch (some 4 us), which pays for few and very long rows only: parts of
+// 8192 tokens (one row of 131072: 9.7 against 14.7 us, 64 rows 14.3
+// against 18.0; one row of 32000: 9.1 against 7.6, 200 rows of 131072 bf16 21.9 against 20.9).
 static int splits_for(int64_t rows, int64_t vocab) {
-    if (vocab <= 1024 || rows >= 256) return 1;
-    int64_t s = 512 / rows;
-    if (s > vocab / 4096) s = vocab / 4096;
-    if (s > kMaxSplits) s = kMaxSplits;
-    return s < 1 ? 1 : (int)s;
+    if (vocab <= 65536 || rows > 128) return 1;
+    int64_t s = (vocab + 8191) / 8192;
+    if (s > 1024 / rows) s = 1024 / rows;
+    return (int)(s > kMaxSplits ? kMaxSplits : s);
 }
 
 static int64_t workspace_bytes(int64_t rows, int64_t vocab, int64_t top) {
@@ -499,19 +611,24 @@ static int64_t workspace_bytes(int64_t rows, int64_t vocab, int64_t top) {
 
 template <typename E>
 static void launch(const Args& p, hipStream_t st) {
-    if (p.vocab <= 1024) {
+    if (p.vocab <= kShort) {
         int g = 0;
         while (g < 6 && (4 << g) < p.vocab) ++g;
         const int64_t per_wg = (int64_t)4 << (6 - g);
         const dim3 grid((unsigned)((p.rows + per_wg - 1) / per_wg)), blk(256);
         if (p.vocab <= 256) hipLaunchKernelGGL((token_scores_short_kernel<E, 1>), grid, blk, 0, st, p, g);
         else if (p.vocab <= 512) hipLaunchKernelGGL((token_scores_short_kernel<E, 2>), grid, blk, 0, st, p, g);
-        else hipLaunchKernelGGL((token_scores_short_kernel<E, 4>), grid, blk, 0, st, p, g);
+        else if (p.vocab <= 1024) hipLaunchKernelGGL((token_scores_short_kernel<E, 4>), grid, blk, 0, st, p, g);
+        else hipLaunchKernelGGL((token_scores_short_kernel<E, 8>), grid, blk, 0, st, p, g);
     } else if (p.splits > 1) {
         hipLaunchKernelGGL((token_scores_long_kernel<E, 256, true>), dim3((unsigned)(p.rows * p.splits)), dim3(256), 0, st, p);
         hipLaunchKernelGGL((token_scores_join_kernel<E>), dim3((unsigned)p.rows), dim3(64), 0, st, p);
     } else {
-        hipLaunchKernelGGL((token_scores_long_kernel<E, 256, false>), dim3((unsigned)p.rows), dim3(256), 0, st, p);
+        // Few rows: wider work-groups keep the chip busier (256 x 32000: 8.5 against 10.0 us); many: narrower ones interleave
+        // better (8192 x 32000: 118 us with 256 threads, 138 with 512)
+        const dim3 grid((unsigned)p.rows);
+        if (p.rows < 768) hipLaunchKernelGGL((token_scores_long_kernel<E, 512, false>), grid, dim3(512), 0, st, p);
+        else hipLaunchKernelGGL((token_scores_long_kernel<E, 256, false>), grid, dim3(256), 0, st, p);
     }
 }
 

@@ -65,8 +65,8 @@ def check(r, z, tokens, k):
 
 
 SIZES = [(1, 1, 1), (3, 2, 4), (5, 31, 5), (9, 32, 4), (17, 33, 32), (130, 100, 8), (7, 255, 3), (6, 256, 32), (5, 257, 7),
-         (9, 511, 1), (4, 1000, 20), (3, 1024, 32), (3, 1025, 32), (5, 1030, 5), (2, 4095, 9), (300, 5001, 8), (1, 8192, 32),
-         (2, 16391, 20), (40, 32000, 5), (1, 50257, 20), (257, 20011, 32), (1, 131072, 8), (3, 200003, 20), (64, 70000, 0)]
+         (9, 511, 1), (4, 1000, 20), (3, 1024, 32), (3, 1025, 32), (5, 1030, 5), (70, 2000, 8), (5, 2047, 20), (4, 2048, 32), (3, 2049, 7), (33, 700, 3), (2, 4095, 9), (300, 5001, 8), (1, 8192, 32),
+         (2, 16391, 20), (40, 32000, 5), (1, 50257, 20), (257, 20011, 32), (1, 131072, 8), (3, 200003, 20), (64, 70000, 0), (5, 65537, 9), (128, 66000, 3), (2, 600001, 32)]
 
 
 @pytest.mark.parametrize("rows,vocab,k", SIZES)
@@ -85,7 +85,7 @@ def test_token_scores(rows, vocab, k, dtype):
     check(ops.token_scores(z, tokens, alternatives=k), z, tokens, k)
 
 
-@pytest.mark.parametrize("vocab", [1, 5, 32, 300, 1024, 1500, 9001, 40000, 140001])
+@pytest.mark.parametrize("vocab", [1, 5, 32, 300, 1024, 1500, 2500, 9001, 40000, 140001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_special_rows(vocab, dtype):
     """Rows that allow nothing, one token, the lowest value everywhere, NaN and infinities at the first, a middle and the
