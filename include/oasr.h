@@ -410,7 +410,7 @@ int oasr_quant_i8_rows(const uint16_t* x, int64_t ldx, int64_t rows, int64_t k, 
                        void* stream);
 
 /* LayerNorm (optionally followed by Swish) of float32 rows straight to int8 codes and scales: the codes are made from
- * the float32 result (rint(v * (127 / max|v|))).  oasr_layernorm2_i8 is the double form of a block boundary (x is
+ * the float32 result.  oasr_layernorm2_i8 is the double form of a block boundary (x is
  * overwritten with its first LayerNorm).  d as for oasr_layernorm_fp8; all pointers but scale 16-byte aligned. */
 int oasr_layernorm_i8(const float* x, const float* w, const float* b, int8_t* y, float* scale, int64_t rows, int32_t d,
                       float eps, int32_t swish, void* stream);
@@ -433,9 +433,9 @@ int oasr_gemm_i8(const int8_t* a, int64_t lda, const int8_t* w_packed, const flo
                  float alpha, int32_t epilogue, void* stream);
 
 /* Both steps: the bf16 rows x (ldx apart) are quantised and multiplied.  The same bits as oasr_quant_i8_rows followed by
- * oasr_gemm_i8.  workspace: device, oasr_linear_i8_workspace_bytes(m, k) (0 for a few rows, which are quantised
+ * oasr_gemm_i8.  workspace: device, oasr_linear_i8_workspace_bytes(m, n, k) (0 for a few rows, which are quantised
  * inside the product), 256-byte aligned, contents on entry do not matter; calls that may overlap need one each. */
-int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t k);
+int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const float* scale_w, const float* bias,
                    const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, float alpha,
                    int32_t epilogue, void* workspace, int64_t workspace_bytes, void* stream);

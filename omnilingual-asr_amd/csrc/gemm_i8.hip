@@ -654,26 +654,35 @@ __global__ __launch_bounds__(256) void quant_i8_rows_kernel(const uint16_t* __re
     }
 }
 
-// A few tokens: quantisation and product in one launch.  Every work-group (32 columns, eight waves that split K) quantises the
-// rows itself - they are a few KiB that all of them read from L2 - into LDS, while its first weight slices are on their way;
-// the codes and scales are bit for bit those of the quantiser.  Bound by the weights' way from HBM: 16384 x 4096 at one row
-// 64 MiB; small ones by latency (a second launch would cost more than the work).
-constexpr int kFewBytes = 16384;             // rows * k at most: beyond, quantising once is cheaper
+// A few tokens: quantisation and product in one launch.  Every work-group (16 MT rows x 32 columns, eight waves that split K)
+// quantises its rows itself - they are a few KiB that many of them read from L2 - into LDS, while its first weight slices are
+// on their way; the codes and scales are bit for bit those of the quantiser.  Bound by the weights' way from HBM: 16384 x 4096 at
+// one row (64 MiB) 12.8 us; small ones by latency (a second launch would cost more than the work).
 constexpr int kFewColumns = 32;              // 64 at a time are 5 - 25 % slower at every size tried (1 x 4096 x 4096: 8.4 against 10.2 us)
 constexpr int kFewDepth = 6;                 // slices on their way (4: up to 4 % slower; 8: faster on short n, slower on long)
-constexpr int kFewItems = kFewBytes / 8 / 512;
-constexpr int kFewLds = kFewBytes + 16 * 16;
 
-template <int EPI>
-__global__ __launch_bounds__(512) void linear_i8_few_kernel(const GemmArgs p, const uint16_t* __restrict__ x, int64_t ldx, int k) {
-    constexpr int D = kFewDepth, CT = kFewColumns / 16, kSums = 8 * CT * 1024;
-    __shared__ __attribute__((aligned(1024))) char lds[kSums + 2048 > kFewLds ? kSums + 2048 : kFewLds];
-    __shared__ uint32_t row_amax[16];
+template <int MT>
+struct FewShape {
+    static constexpr int kCodes = 16384 * MT;                      // rows * k (rounded up to 64) of a work-group at most
+    static constexpr int kItems = kCodes / 8 / 512;                // per thread, eight values each
+    static constexpr int kCodeBytes = kCodes + 16 * 16 * MT, kSums = 8 * MT * 2 * 1024, kAll = kSums + MT * 2048;
+    static constexpr int kLds = kAll > kCodeBytes ? kAll : kCodeBytes;
+};
+
+template <int EPI, int MT>
+__global__ __launch_bounds__(512) void linear_i8_few_kernel(const GemmArgs p, const uint16_t* __restrict__ x, int64_t ldx, int k,
+                                                            int tiles_m) {
+    typedef FewShape<MT> Shape;
+    constexpr int D = kFewDepth, CT = kFewColumns / 16;
+    __shared__ __attribute__((aligned(1024))) char lds[Shape::kLds];
+    __shared__ uint32_t row_amax[16 * MT];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (tid < 16) row_amax[tid] = 0;
-    const int64_t n0 = (int64_t)blockIdx.x * kFewColumns;
-    const int rows = (int)p.m, kp = p.ks * kSlice, pitch = kp + 16;        // 16 bytes apart: the rows' fragments in other banks
+    if (tid < 16 * MT) row_amax[tid] = 0;
+    const int64_t m0 = (int64_t)(blockIdx.x % tiles_m) * (16 * MT), n0 = (int64_t)(blockIdx.x / tiles_m) * kFewColumns;
+    const int rows = (int)min((int64_t)(16 * MT), p.m - m0), kp = p.ks * kSlice;
+    const int pitch = kp + 16;               // 16 bytes apart: the rows' fragments in other banks
+    x += m0 * ldx;
 
     const char* src_w[CT];
 #pragma unroll
@@ -694,60 +703,65 @@ __global__ __launch_bounds__(512) void linear_i8_few_kernel(const GemmArgs p, co
 #pragma unroll
     for (int d = 0; d < D - 1; ++d)
         if (d < count) request(wf[d]);
+    const int64_t mu = m0 + 16 * (wave % MT);
     Epilogue<EPI, 1, 2> out;
-    if (wave == 0) out.load(p, 0, n0, lane);
+    if (wave < MT) out.load(p, mu, n0, lane);
 
-    // the rows, eight values to an item and up to four items to a thread, all requested at once; a row is a multiple of eight
-    // items, so eight neighbouring lanes always share one
+    // the rows, eight values to an item, all requested at once; a row is a multiple of eight items, so eight neighbouring lanes
+    // always share one
     const int per_row = kp / 8, items = rows * per_row;
-    u32x4 v[kFewItems];
+    u32x4 v[Shape::kItems];
 #pragma unroll
-    for (int i = 0; i < kFewItems; ++i) {
+    for (int i = 0; i < Shape::kItems; ++i) {
         const int id = tid + 512 * i, r = id / per_row;
         v[i] = id < items ? load_row8(x + r * ldx, 8 * (id - r * per_row), k) : (u32x4){0, 0, 0, 0};
     }
     __syncthreads();                         // row_amax is clear
 #pragma unroll
-    for (int i = 0; i < kFewItems; ++i) {
+    for (int i = 0; i < Shape::kItems; ++i) {
         const int id = tid + 512 * i;
-        uint32_t amax = amax8(v[i], 0);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, o, 64));
+        const uint32_t amax = eight_umax(amax8(v[i], 0));
         if (id < items && (lane & 7) == 0) atomicMax(&row_amax[id / per_row], amax);
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kFewItems; ++i) {
+    for (int i = 0; i < Shape::kItems; ++i) {
         const int id = tid + 512 * i, r = id / per_row;
         if (id >= items) break;
         *reinterpret_cast<u32x2*>(lds + r * pitch + 8 * (id - r * per_row)) = codes8(v[i], row_scale(row_amax[r]));
     }
     __syncthreads();
-    const int row = min(lane & 15, rows - 1);
-    out.sa[0] = row_scale(row_amax[row]).scale;
-    const char* frag = lds + row * pitch + wave * kSlice + (lane >> 4) * 16;
-    i32x4 acc[CT] = {};
+    const char* frag[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) frag[i] = lds + min(16 * i + (lane & 15), rows - 1) * pitch + wave * kSlice + (lane >> 4) * 16;
+    out.sa[0] = row_scale(row_amax[min(16 * (wave % MT) + (lane & 15), rows - 1)]).scale;
+    i32x4 acc[MT][CT] = {};
     for (int t = 0; t < count; t += D) {
 #pragma unroll
         for (int d = 0; d < D; ++d) {
             if (t + d >= count) break;
             if (t + d + D - 1 < count) request(wf[(d + D - 1) % D]);
-            const i32x4 xf = *reinterpret_cast<const i32x4*>(frag + (t + d) * 8 * kSlice);
 #pragma unroll
-            for (int j = 0; j < CT; ++j) acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[d][j], xf, acc[j], 0, 0, 0);
+            for (int i = 0; i < MT; ++i) {
+                const i32x4 xf = *reinterpret_cast<const i32x4*>(frag[i] + (t + d) * 8 * kSlice);
+#pragma unroll
+                for (int j = 0; j < CT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[d][j], xf, acc[i][j], 0, 0, 0);
+            }
         }
     }
     __syncthreads();                         // the rows have been read
 #pragma unroll
-    for (int j = 0; j < CT; ++j) *reinterpret_cast<i32x4*>(lds + (wave * CT + j) * 1024 + lane * 16) = acc[j];
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) *reinterpret_cast<i32x4*>(lds + ((wave * MT + i) * CT + j) * 1024 + lane * 16) = acc[i][j];
     __syncthreads();
-    if (wave == 0) {
+    if (wave < MT) {
         i32x4 sum[1][2] = {};
 #pragma unroll
         for (int w = 0; w < 8; ++w)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) sum[0][j] += *reinterpret_cast<const i32x4*>(lds + (w * CT + j) * 1024 + lane * 16);
-        out.finish(p, sum, 0, n0, lane, lds + kSums);
+            for (int j = 0; j < 2; ++j) sum[0][j] += *reinterpret_cast<const i32x4*>(lds + ((w * MT + wave) * CT + j) * 1024 + lane * 16);
+        out.finish(p, sum, mu, n0, lane, lds + Shape::kSums + wave * 2048);
     }
 }
 
@@ -839,12 +853,25 @@ static void launch_form(int form, const GemmArgs& p, hipStream_t st) {
     }
 }
 
-// Whether a call quantises inside the product (and needs no workspace).
-static bool few_rows(int64_t m, int64_t k) { return m <= 16 && m * round_up(k, kSlice) <= kFewBytes; }
+// Whether a call quantises inside the product (and needs no workspace): the row tiles of 16 per work-group, or 0.  Up to 16
+// rows always where they fit; more rows (32 to a work-group) while the work-groups fit the CUs once: 99 x 2048 x 1024 8.5 us on
+// the device against 7.9 in two launches, but 8.4 against 12.4 per call made from a program (a launch costs the host 3.5).  Twice as
+// many work-groups take twice as long (99 x 4096 x 1024: 16.7 against 8.7).
+static int few_rows(int64_t m, int64_t n, int64_t k) {
+    const int64_t kp = round_up(k, kSlice);
+    if (m <= 16 && m * kp <= FewShape<1>::kCodes) return 1;
+    if (32 * kp <= FewShape<2>::kCodes && (m + 31) / 32 * ((n + kFewColumns - 1) / kFewColumns) <= 256) return 2;
+    return 0;
+}
 
-static int launch_few(const GemmArgs& p, const uint16_t* x, int64_t ldx, int64_t k, int32_t epilogue, hipStream_t st) {
-    const dim3 grid((unsigned)((p.n + kFewColumns - 1) / kFewColumns)), blk(512);
-#define OASR_FEW(E) hipLaunchKernelGGL((linear_i8_few_kernel<E>), grid, blk, 0, st, p, x, ldx, (int)k)
+static int launch_few(int mt, const GemmArgs& p, const uint16_t* x, int64_t ldx, int64_t k, int32_t epilogue, hipStream_t st) {
+    const int tm = (int)((p.m + 16 * mt - 1) / (16 * mt));
+    const dim3 grid((unsigned)(tm * ((p.n + kFewColumns - 1) / kFewColumns))), blk(512);
+#define OASR_FEW(E)                                                                                             \
+    do {                                                                                                        \
+        if (mt == 1) hipLaunchKernelGGL((linear_i8_few_kernel<E, 1>), grid, blk, 0, st, p, x, ldx, (int)k, tm); \
+        else hipLaunchKernelGGL((linear_i8_few_kernel<E, 2>), grid, blk, 0, st, p, x, ldx, (int)k, tm);         \
+    } while (0)
     switch (epilogue) {
         case OASR_EPI_BIAS_BF16: OASR_FEW(OASR_EPI_BIAS_BF16); break;
         case OASR_EPI_BIAS_SWISH_BF16: OASR_FEW(OASR_EPI_BIAS_SWISH_BF16); break;
@@ -965,8 +992,8 @@ int oasr_gemm_i8(const int8_t* a, int64_t lda, const int8_t* w_packed, const flo
                            (hipStream_t)stream);
 }
 
-int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t k) {
-    if (m <= 0 || k <= 0 || i8::few_rows(m, k)) return 0;
+int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (m <= 0 || n <= 0 || k <= 0 || i8::few_rows(m, n, k)) return 0;
     return round_up(m * round_up(k, i8::kSlice), 256) + round_up(m * 4, 256);
 }
 
@@ -979,12 +1006,12 @@ int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const
     if (m == 0) return OASR_OK;
     OASR_REQUIRE(x, "linear_i8: null pointer");
     OASR_REQUIRE(((uintptr_t)x & 1) == 0, "linear_i8: misaligned pointer");
-    if (i8::few_rows(m, k))
-        return i8::launch_few(i8::gemm_args(nullptr, 0, w_packed, nullptr, scale_w, bias, resid, ldr, c, ldc, m, n, k, alpha, epilogue), x,
+    if (const int mt = i8::few_rows(m, n, k))
+        return i8::launch_few(mt, i8::gemm_args(nullptr, 0, w_packed, nullptr, scale_w, bias, resid, ldr, c, ldc, m, n, k, alpha, epilogue), x,
                               ldx, k, epilogue, (hipStream_t)stream);
     OASR_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0, "linear_i8: workspace missing or not 256-byte aligned");
-    if (workspace_bytes < oasr_linear_i8_workspace_bytes(m, k)) {
-        set_error("linear_i8: workspace needs %lld bytes, got %lld", (long long)oasr_linear_i8_workspace_bytes(m, k),
+    if (workspace_bytes < oasr_linear_i8_workspace_bytes(m, n, k)) {
+        set_error("linear_i8: workspace needs %lld bytes, got %lld", (long long)oasr_linear_i8_workspace_bytes(m, n, k),
                   (long long)workspace_bytes);
         return OASR_ECAPACITY;
     }

@@ -110,7 +110,7 @@ _SIGNATURES = {
     "oasr_gemm_i8_packed_bytes": (c_i64, [c_i64, c_i64]),
     "oasr_gemm_pack_w_i8": (c_i32, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
     "oasr_gemm_i8": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_f32, c_i32, c_vp]),
-    "oasr_linear_i8_workspace_bytes": (c_i64, [c_i64, c_i64]),
+    "oasr_linear_i8_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
     "oasr_linear_i8": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_f32, c_i32, c_vp, c_i64, c_vp]),
     "oasr_attention_relkey": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp]),
     "oasr_dwconv_causal": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_i64, c_i32, c_i32, c_vp]),

@@ -153,7 +153,7 @@ class LinearI8:
             return out
         L = _hip.lib()
         with _on(self.device):
-            ws_bytes = int(L.oasr_linear_i8_workspace_bytes(m, k))
+            ws_bytes = int(L.oasr_linear_i8_workspace_bytes(m, self.out_features, k))
             ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=self.device) if ws_bytes else None
             _hip.check(L.oasr_linear_i8(x2.data_ptr(), ldx, self._packed_ptr, self._scale_ptr, self._bias_ptr,
                                         None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m,

@@ -69,7 +69,8 @@ SHAPES = [(1, 1, 1), (1, 33, 64), (1, 1024, 512), (2, 1000, 1000), (3, 64, 65), 
           (33, 4096, 256), (64, 512, 4096), (99, 2048, 1024), (127, 257, 191), (128, 128, 64), (129, 384, 320), (200, 777, 1000),
           (256, 256, 64), (300, 96, 16448), (513, 1024, 512), (1000, 4096, 64), (1504, 1024, 1024), (2100, 640, 192),
           (4096, 512, 512), (8200, 1056, 320), (2100, 4128, 128), (4500, 2080, 64), (2049, 4097, 65),
-          (48, 1000, 8192), (300, 2048, 4096), (400, 700, 4096), (1504, 1024, 4096), (1500, 1000, 4100), (2000, 2100, 4096), (64, 16400, 100)]
+          (48, 1000, 8192), (300, 2048, 4096), (400, 700, 4096), (1504, 1024, 4096), (1500, 1000, 4100), (2000, 2100, 4096), (64, 16400, 100),
+          (17, 500, 500), (40, 70, 1024), (256, 1000, 1000), (33, 4000, 960), (16, 2000, 1024), (15, 300, 1090), (5, 64, 3210), (3, 96, 16384)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)

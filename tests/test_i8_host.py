@@ -42,11 +42,11 @@ def test_operand_refusals():
     assert _gemm(lda=48) == -1 and b"lda" in L.oasr_last_error()
     assert _gemm(lda=72) == -1 and _gemm(k=65) == -1 and _gemm(a=None) == -1 and _gemm(a=A + 8) == -1 and _gemm(sa=None) == -1
     assert _linear(ldx=63) == -1 and b"ldx" in L.oasr_last_error()
-    many = dict(m=300)
+    many = dict(m=300, k=2000, ldx=2000)
     assert _linear(x=None) == -1 and _linear(ws=None, **many) == -1 and _linear(ws=A + 16, **many) == -1 and _linear(x=A + 1) == -1
-    need = L.oasr_linear_i8_workspace_bytes(300, 64)
-    assert need == 300 * 64 + 1280 and _linear(bytes=need - 1, **many) == -2 and b"workspace" in L.oasr_last_error()
-    assert L.oasr_linear_i8_workspace_bytes(1, 4096) == 0 and L.oasr_linear_i8_workspace_bytes(0, 64) == 0
+    need = L.oasr_linear_i8_workspace_bytes(300, 64, 2000)
+    assert need == 300 * 2048 + 1280 and _linear(bytes=need - 1, **many) == -2 and b"workspace" in L.oasr_last_error()
+    assert L.oasr_linear_i8_workspace_bytes(1, 64, 4096) == 0 and L.oasr_linear_i8_workspace_bytes(0, 64, 64) == 0
     assert _gemm(m=0, a=None, w=None, c=None) == 0 and _linear(m=0, x=None, ws=None) == 0     # nothing to do
     q = lambda x=A, ldx=64, rows=4, k=64, y=A, ldy=64, s=A: L.oasr_quant_i8_rows(x, ldx, rows, k, y, ldy, s, None)
     assert q(ldx=63) == -1 and q(ldy=56) == -1 and q(k=65, ldx=65) == -1 and q(k=0) == -1 and q(rows=-1) == -1
