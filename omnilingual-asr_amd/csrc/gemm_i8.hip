@@ -773,11 +773,19 @@ __global__ __launch_bounds__(256) void gemm_pack_w_i8_kernel(const int8_t* __res
     const int lane = (int)(idx & 63);
     const int64_t piece = idx >> 6, grp = piece / ks, t = piece - grp * ks;
     const int64_t row = grp * 16 + (lane & 15), col = t * kSlice + (lane >> 4) * 16;
-    uint32_t v[4] = {0, 0, 0, 0};
-    if (row < n)
-        for (int e = 0; e < 16; ++e)
-            if (col + e < k) v[e >> 2] |= (uint32_t)(uint8_t)w[row * ldw + col + e] << (8 * (e & 3));
-    *reinterpret_cast<u32x4*>(out + idx * 16) = (u32x4){v[0], v[1], v[2], v[3]};
+    struct __attribute__((packed, aligned(1))) Any {
+        uint32_t v[4];
+    } c = {{0, 0, 0, 0}};
+    const int8_t* src = w + row * ldw + col;
+    if (row < n) {
+        if (col + 16 <= k) {
+            c = *reinterpret_cast<const Any*>(src);
+        } else {
+            for (int e = 0; e < 16; ++e)
+                if (col + e < k) c.v[e >> 2] |= (uint32_t)(uint8_t)src[e] << (8 * (e & 3));
+        }
+    }
+    *reinterpret_cast<u32x4*>(out + idx * 16) = (u32x4){c.v[0], c.v[1], c.v[2], c.v[3]};
 }
 
 static int check_gemm(const char* what, const int8_t* w, const float* scale_w, const float* bias, const float* resid,

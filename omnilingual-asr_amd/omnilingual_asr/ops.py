@@ -8,7 +8,6 @@ No counterpart in the reference, whose projections and answers are made by a rem
 
 from __future__ import annotations
 
-import contextlib
 import math
 from typing import NamedTuple
 
@@ -21,12 +20,17 @@ EPILOGUES = {"bias": _hip.EPI_BIAS_BF16, "swish": _hip.EPI_BIAS_SWISH_BF16, "glu
              "residual": _hip.EPI_RESIDUAL_F32, "float": _hip.EPI_BIAS_F32}
 _INT8, _FLOAT32, _BFLOAT16, _LOGITS = (torch.int8,), (torch.float32,), (torch.bfloat16,), (torch.float32, torch.bfloat16)
 _NORM_WIDTHS = (256, 512, 1024, 2048, 4096)
-_NULL = contextlib.nullcontext()
 
 
-def _on(device: torch.device):
-    """The device's context, entered only where another one is current."""
-    return _NULL if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _call(name: str, device: torch.device, *args) -> None:
+    """One C call on `device`'s current stream; the device is made the current one where it is not."""
+    fn = getattr(_hip.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _hip.stream_ptr(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _hip.stream_ptr(device.index))
+    _hip.check(rc, name)
 
 
 def _rows(t, what: str, dtypes: tuple):
@@ -100,11 +104,8 @@ class LinearI8:
         if scale is None:
             raise ValueError("scale must be given")
         self.scale, self.bias = scale, bias
-        L = _hip.lib()
-        with _on(self.device):
-            self.packed = torch.empty((int(L.oasr_gemm_i8_packed_bytes(n, k)),), dtype=torch.int8, device=self.device)
-            _hip.check(L.oasr_gemm_pack_w_i8(codes.data_ptr(), ldw, n, k, self.packed.data_ptr(), _hip.current_stream_ptr()),
-                       "oasr_gemm_pack_w_i8")
+        self.packed = codes.new_empty((int(_hip.lib().oasr_gemm_i8_packed_bytes(n, k)),))
+        _call("oasr_gemm_pack_w_i8", self.device, codes.data_ptr(), ldw, n, k, self.packed.data_ptr())
         self._packed_ptr = self.packed.data_ptr()
 
     def _output(self, x, epilogue, resid, out):
@@ -151,14 +152,11 @@ class LinearI8:
         epi, out, ldc, resid, ldr = self._output(x, epilogue, resid, out)
         if m == 0:
             return out
-        L = _hip.lib()
-        with _on(self.device):
-            ws_bytes = int(L.oasr_linear_i8_workspace_bytes(m, self.out_features, k))
-            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=self.device) if ws_bytes else None
-            _hip.check(L.oasr_linear_i8(x2.data_ptr(), ldx, self._packed_ptr, self._scale_ptr, self._bias_ptr,
-                                        None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m,
-                                        self.out_features, k, alpha, epi, None if ws is None else ws.data_ptr(),
-                                        ws_bytes, _hip.current_stream_ptr()), "oasr_linear_i8")
+        ws_bytes = _hip.lib().oasr_linear_i8_workspace_bytes(m, self.out_features, k)
+        ws = x.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+        _call("oasr_linear_i8", self.device, x2.data_ptr(), ldx, self._packed_ptr, self._scale_ptr, self._bias_ptr,
+              None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m, self.out_features, k, alpha, epi,
+              None if ws is None else ws.data_ptr(), ws_bytes)
         return out
 
     def normed(self, x: torch.Tensor, gain: torch.Tensor, shift: torch.Tensor, *, eps: float = 1e-5, epilogue: str = "bias",
@@ -174,16 +172,10 @@ class LinearI8:
         epi, out, ldc, resid, ldr = self._output(x, epilogue, resid, out)
         if m == 0:
             return out
-        L = _hip.lib()
-        with _on(self.device):
-            st = _hip.current_stream_ptr()
-            codes = torch.empty((m, k), dtype=torch.int8, device=self.device)
-            scale = torch.empty((m,), dtype=torch.float32, device=self.device)
-            _hip.check(L.oasr_layernorm_i8(x2.data_ptr(), gain_ptr, shift_ptr, codes.data_ptr(), scale.data_ptr(), m, k, eps, 0, st),
-                       "oasr_layernorm_i8")
-            _hip.check(L.oasr_gemm_i8(codes.data_ptr(), k, self._packed_ptr, scale.data_ptr(), self._scale_ptr, self._bias_ptr,
-                                      None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m,
-                                      self.out_features, k, alpha, epi, st), "oasr_gemm_i8")
+        codes, scale = x.new_empty((m, k), dtype=torch.int8), x.new_empty((m,))
+        _call("oasr_layernorm_i8", self.device, x2.data_ptr(), gain_ptr, shift_ptr, codes.data_ptr(), scale.data_ptr(), m, k, eps, 0)
+        _call("oasr_gemm_i8", self.device, codes.data_ptr(), k, self._packed_ptr, scale.data_ptr(), self._scale_ptr, self._bias_ptr,
+              None if resid is None else resid.data_ptr(), ldr, out.data_ptr(), ldc, m, self.out_features, k, alpha, epi)
         return out
 
 
@@ -211,9 +203,13 @@ def _score_outputs(lead, given, alternatives, like):
     return TokenScores(new(given, dtype=f32), new(lead, dtype=f32), new(listed, dtype=torch.int32), new(listed, dtype=f32))
 
 
-def _score_workspace(rows, vocab, alternatives, device):
-    n = int(_hip.lib().oasr_token_scores_workspace_bytes(rows, vocab, alternatives))
-    return n, torch.empty((n,), dtype=torch.uint8, device=device) if n else None
+def _score(name, z, args, out, rows, vocab, alternatives):
+    """The call that both forms make: `args` between the logits' type and the outputs."""
+    ws_bytes = _hip.lib().oasr_token_scores_workspace_bytes(rows, vocab, alternatives)
+    ws = z.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    _call(name, z.device, z.data_ptr(), _hip.F32 if z.dtype == torch.float32 else _hip.BF16, *args, out.logprobs.data_ptr(),
+          out.entropy.data_ptr(), alternatives, out.ids.data_ptr(), out.best.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes)
+    return out
 
 
 def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, alternatives: int = 0) -> TokenScores:
@@ -231,14 +227,8 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, al
     out = _score_outputs(lead, given, alternatives, logits)
     if rows == 0:
         return out
-    with _on(device):
-        ws_bytes, ws = _score_workspace(rows, vocab, alternatives, device)
-        _hip.check(_hip.lib().oasr_token_scores(
-            z.data_ptr(), _hip.F32 if z.dtype == torch.float32 else _hip.BF16, ld, rows, vocab,
-            None if tokens is None else tokens.data_ptr(), n, out.logprobs.data_ptr(), out.entropy.data_ptr(), alternatives,
-            out.ids.data_ptr(), out.best.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes,
-            _hip.current_stream_ptr()), "oasr_token_scores")
-    return out
+    return _score("oasr_token_scores", z, (ld, rows, vocab, None if tokens is None else tokens.data_ptr(), n), out, rows, vocab,
+                  alternatives)
 
 
 def ctc_token_scores(logits: torch.Tensor, tokens: torch.Tensor, frames: torch.Tensor, *, vocab: int | None = None,
@@ -262,11 +252,5 @@ def ctc_token_scores(logits: torch.Tensor, tokens: torch.Tensor, frames: torch.T
     out = _score_outputs(shape, shape, alternatives, logits)
     if tokens.numel() == 0:
         return out
-    with _on(device):
-        ws_bytes, ws = _score_workspace(tokens.numel(), vocab, alternatives, device)
-        _hip.check(_hip.lib().oasr_ctc_token_scores(
-            logits.data_ptr(), _hip.F32 if logits.dtype == torch.float32 else _hip.BF16, ld, vocab, batch, t_pad,
-            tokens.data_ptr(), frames.data_ptr(), shape[1], out.logprobs.data_ptr(), out.entropy.data_ptr(), alternatives,
-            out.ids.data_ptr(), out.best.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes,
-            _hip.current_stream_ptr()), "oasr_ctc_token_scores")
-    return out
+    return _score("oasr_ctc_token_scores", logits, (ld, vocab, batch, t_pad, tokens.data_ptr(), frames.data_ptr(), shape[1]), out,
+                  tokens.numel(), vocab, alternatives)
