@@ -584,15 +584,15 @@ __global__ __launch_bounds__(512) void gemm_i8_split_kernel(const GemmArgs p, in
 // bytes per lane, all issued before the first use), or, for longer rows, in two sweeps of which the second reads from
 // cache.  HBM-bound: 2 bytes in, 1 byte out per element.  Row starts need no alignment; the codes' rows are whole
 // 64-byte slices, zero from k on.
-struct __attribute__((packed, aligned(2))) bf16x8_any {
-    uint32_t w[4];
-};
-
+// ONCE: read past the caches, for activations larger than they are (48128 x 4096 with its product 324 -> 315 us, since more
+// of the codes stay in the memory-side cache; at 12 MB it costs 4 %).
+template <bool ONCE = false>
 __device__ __forceinline__ u32x4 load_row8(const uint16_t* __restrict__ xr, int64_t c, int64_t k) {
+    typedef u32x4 __attribute__((aligned(2))) any;
     u32x4 v = {0, 0, 0, 0};
     if (c + 8 <= k) {
-        const bf16x8_any t = *reinterpret_cast<const bf16x8_any*>(xr + c);
-        v = (u32x4){t.w[0], t.w[1], t.w[2], t.w[3]};
+        const any* p = reinterpret_cast<const any*>(xr + c);
+        v = ONCE ? __builtin_nontemporal_load(p) : *p;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -621,7 +621,7 @@ __device__ __forceinline__ u32x2 codes8(u32x4 v, const RowScale& s) {
     return (u32x2){pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7])};
 }
 
-template <int NV>
+template <int NV, bool ONCE>
 __global__ __launch_bounds__(256) void quant_i8_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t rows,
                                                             int64_t k, int8_t* __restrict__ y, int64_t ldy,
                                                             float* __restrict__ scale) {
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(256) void quant_i8_rows_kernel(const uint16_t* __re
     u32x4 v[NV > 0 ? NV : 1];
     if (NV > 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = load_row8(xr, 8 * lane + 512 * i, k);
+        for (int i = 0; i < NV; ++i) v[i] = load_row8<ONCE>(xr, 8 * lane + 512 * i, k);
 #pragma unroll
         for (int i = 0; i < NV; ++i) amax = amax8(v[i], amax);
     } else {
@@ -934,7 +934,12 @@ static GemmArgs gemm_args(const int8_t* a, int64_t lda, const int8_t* w, const f
 static int quant_rows(const uint16_t* x, int64_t ldx, int64_t rows, int64_t k, int8_t* y, int64_t ldy, float* scale,
                       hipStream_t st) {
     const dim3 grid((unsigned)((rows + 3) / 4)), blk(256);
-#define OASR_QUANT_I8(NV) hipLaunchKernelGGL(quant_i8_rows_kernel<NV>, grid, blk, 0, st, x, ldx, rows, k, y, ldy, scale)
+    const bool once = rows * k >= ((int64_t)32 << 20);     // 64 MiB of activations
+#define OASR_QUANT_I8(NV)                                                                                              \
+    do {                                                                                                               \
+        if (once) hipLaunchKernelGGL((quant_i8_rows_kernel<NV, true>), grid, blk, 0, st, x, ldx, rows, k, y, ldy, scale); \
+        else hipLaunchKernelGGL((quant_i8_rows_kernel<NV, false>), grid, blk, 0, st, x, ldx, rows, k, y, ldy, scale);     \
+    } while (0)
     // the row in registers up to 16384 columns (32 loads per lane), the smallest form that covers it
     if (k <= 512) OASR_QUANT_I8(1);
     else if (k <= 1024) OASR_QUANT_I8(2);
@@ -942,7 +947,7 @@ static int quant_rows(const uint16_t* x, int64_t ldx, int64_t rows, int64_t k, i
     else if (k <= 4096) OASR_QUANT_I8(8);
     else if (k <= 8192) OASR_QUANT_I8(16);
     else if (k <= 16384) OASR_QUANT_I8(32);
-    else OASR_QUANT_I8(0);
+    else hipLaunchKernelGGL((quant_i8_rows_kernel<0, false>), grid, blk, 0, st, x, ldx, rows, k, y, ldy, scale);   // two sweeps: caches wanted
 #undef OASR_QUANT_I8
     OASR_CHECK_LAUNCH("quant_i8_rows");
     return OASR_OK;
