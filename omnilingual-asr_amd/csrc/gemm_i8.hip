@@ -80,19 +80,24 @@ __device__ __forceinline__ f32x4 load_cols(const float* __restrict__ p, int64_t 
 }
 
 // Four consecutive float32 values of a row, of which the first `count` exist.
-template <bool FULL>
+template <bool FULL, bool ONCE>
 __device__ __forceinline__ f32x4 load_f32(const float* p, int64_t count) {
-    if (FULL) return *reinterpret_cast<const f32x4*>(p);
+    if (FULL) {
+        const f32x4* q = reinterpret_cast<const f32x4*>(p);
+        return ONCE ? __builtin_nontemporal_load(q) : *q;
+    }
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (e < count) v[e] = p[e];
     return v;
 }
-template <bool FULL>
+template <bool FULL, bool ONCE>
 __device__ __forceinline__ void store_f32(float* p, f32x4 v, int64_t count) {
     if (FULL) {
-        *reinterpret_cast<f32x4*>(p) = v;
+        f32x4* q = reinterpret_cast<f32x4*>(p);
+        if (ONCE) __builtin_nontemporal_store(v, q);
+        else *q = v;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -100,10 +105,12 @@ __device__ __forceinline__ void store_f32(float* p, f32x4 v, int64_t count) {
     }
 }
 // Eight bf16 values of a row, of which the first `count` exist.
-template <bool FULL>
+template <bool FULL, bool ONCE>
 __device__ __forceinline__ void store_bf16x8(uint16_t* p, u32x4 v, int64_t count) {
     if (FULL) {
-        *reinterpret_cast<u32x4*>(p) = v;
+        u32x4* q = reinterpret_cast<u32x4*>(p);
+        if (ONCE) __builtin_nontemporal_store(v, q);
+        else *q = v;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -134,7 +141,9 @@ constexpr int kSlab = 4096;     // LDS per wave of the epilogue: 16 rows x 64 co
 // stored as it is costs a memory request per lane (measured: 16 bytes per clock and CU).  Each group of 16 rows therefore
 // crosses a wave-private slab, and leaves with the columns of a row in neighbouring lanes: whole 128-byte lines.  The slab's
 // 16-byte chunks are permuted by the row so that neither side has bank conflicts.
-template <int EPI, int MT, int NT>
+// ONCE: outputs and residual rows go past the caches (large problems, whose outputs the caches would not keep: products that end
+// in float32 gain 3 - 10 %, the others 2 %, the encoder's step is the same either way).
+template <int EPI, int MT, int NT, bool ONCE = false>
 struct Epilogue {
     static_assert(NT == 4 || NT == 2, "a wave owns 64 or 32 columns");
     static constexpr bool kResidual = EPI == OASR_EPI_RESIDUAL_F32, kFloat = kResidual || EPI == OASR_EPI_BIAS_F32,
@@ -159,7 +168,7 @@ struct Epilogue {
 #pragma unroll
         for (int q = 0; q < kStores; ++q) {
             const int64_t row = m0 + 16 * i + kRows * q + lane / kChunks;
-            if (FULL || row < p.m) resid[q] = load_f32<FULL>(p.resid + row * p.ldr + col, p.n - col);
+            if (FULL || row < p.m) resid[q] = load_f32<FULL, ONCE>(p.resid + row * p.ldr + col, p.n - col);
         }
     }
 
@@ -242,8 +251,8 @@ struct Epilogue {
             for (int q = 0; q < kStores; ++q) {
                 const int64_t row = m0 + 16 * i + kRows * q + out_row;
                 if (!storing || !(FULL || row < p.m)) continue;
-                if (kFloat) store_f32<FULL>(reinterpret_cast<float*>(p.c) + row * p.ldc + col, __builtin_bit_cast(f32x4, v[q]), left);
-                else store_bf16x8<FULL>(reinterpret_cast<uint16_t*>(p.c) + row * p.ldc + col, v[q], left);
+                if (kFloat) store_f32<FULL, ONCE>(reinterpret_cast<float*>(p.c) + row * p.ldc + col, __builtin_bit_cast(f32x4, v[q]), left);
+                else store_bf16x8<FULL, ONCE>(reinterpret_cast<uint16_t*>(p.c) + row * p.ldc + col, v[q], left);
             }
         }
     }
@@ -461,7 +470,7 @@ __global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int
             if (!(wm == 1 && t == nph - 1)) OASR_I8_BARRIER();
         }
         // (loading the scales during the last slice instead costs more in the loop than it saves here)
-        Epilogue<EPI, 8, 4>::run(p, acc, (int64_t)tm * kWide + wm * 128, (int64_t)tn * kWide + wn * 64, lane,
+        Epilogue<EPI, 8, 4, true>::run(p, acc, (int64_t)tm * kWide + wm * 128, (int64_t)tn * kWide + wn * 64, lane,
                                  ring + 2 * kWideRing * kWideSlice + wave * kSlab);
         if (wm == 1) OASR_I8_BARRIER();
     }
