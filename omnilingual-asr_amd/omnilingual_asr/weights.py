@@ -143,11 +143,12 @@ def quantize_rows_e4m3(w: torch.Tensor):
 
 def quantize_rows_i8(w: torch.Tensor):
     """Per-row 8-bit integer quantisation: (codes int8 [out, in], scale float32 [out]) with w ~= codes * scale,
-    scale = max|row| / 127 (1 for an all-zero row), codes = rint(127 w / max|row|)."""
+    scale = max|row| / 127 (1 for an all-zero row), codes = rint(127 w / max|row|).  A row that holds a NaN or an infinity
+    keeps it in its scale (codes 0)."""
     w = w.to(torch.float32)
     amax = w.abs().amax(dim=1)
-    amax = torch.where(amax > 0, amax, torch.full_like(amax, 127.0))
-    codes = (w.to(torch.float64) * 127.0 / amax[:, None]).round().to(torch.int8)
+    amax = torch.where(amax == 0, torch.full_like(amax, 127.0), amax)
+    codes = (w.to(torch.float64) * 127.0 / amax[:, None]).nan_to_num(0.0, 0.0, 0.0).round().to(torch.int8)
     return codes, amax / 127.0
 
 

@@ -91,6 +91,9 @@ def test_host_quantiser_is_the_definition():
     want, s = quantize64(w)
     assert codes.dtype == torch.int8 and torch.equal(codes.double(), want) and torch.equal(scale, s.float())
     assert scale[5] == 1.0 and int(codes.abs().max()) == 127
+    w[1, 3], w[2, 0] = float("nan"), float("inf")
+    codes, scale = quantize_rows_i8(w)
+    assert torch.isnan(scale[1]) and torch.isinf(scale[2]) and (codes[1:3] == 0).all() and torch.isfinite(scale[3:]).all()
 
 
 def test_pipeline_takes_one_kind_of_8_bit_weights():
