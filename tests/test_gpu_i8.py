@@ -26,7 +26,8 @@ def _quant(x, ldy=None, fill=77):
 
 
 @pytest.mark.parametrize("rows,k", [(1, 1), (3, 63), (5, 64), (7, 65), (4, 511), (9, 512), (6, 1000), (33, 1024), (5, 2047),
-                                    (17, 4096), (3, 8191), (5, 16384), (2, 16385), (3, 40001)])
+                                    (17, 4096), (3, 8191), (5, 16384), (2, 16385), (3, 40001),
+                                    (9000, 100), (9000, 1030), (9001, 4090), (8200, 4100), (700, 8192)])
 def test_quant_rows_bit_for_bit(rows, k):
     g = torch.Generator().manual_seed(rows * 7 + k)
     x = (torch.randn((rows, k), generator=g) * torch.rand((rows, 1), generator=g) * 4).to(torch.bfloat16)
