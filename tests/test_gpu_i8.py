@@ -92,6 +92,27 @@ def test_linear_i8(m, n, k, epilogue):
     assert_within(got, *finish64(p, bias, epilogue, resid, 0.5))
 
 
+@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("epilogue", ["bias", "swish", "glu", "residual", "float"])
+def test_epilogues_up_to_the_ends_of_float32(m, epilogue):
+    """Pre-activations as large as the type goes: a finite one gives a finite result, saturated gates are 0 and 1."""
+    g = torch.Generator().manual_seed(m)
+    ends = torch.tensor([3.3e38, 2.4e38, 1e38, 1e30, 1e4, 100.0, 89.0, 3.0])
+    bias = torch.cat([ends, -ends, torch.zeros(16)]).repeat(2)
+    bias[48:] = torch.cat([ends, -ends])                     # the second group's gates
+    bias[32:48] = torch.cat([-ends, ends]) * 0.5
+    codes, scale = weight_codes(64, 70, g)
+    x = torch.zeros((m, 70), dtype=torch.bfloat16)
+    x[0] = torch.randn(70, generator=g).to(torch.bfloat16)
+    resid = torch.randn((m, 64), generator=g) if epilogue == "residual" else None
+    layer = ops.LinearI8.from_codes(codes.cuda(), scale.cuda(), bias.cuda())
+    got = layer(x.cuda(), epilogue=epilogue, resid=None if resid is None else resid.cuda(), alpha=0.5)
+    qa, _ = quantize64(x)
+    sa = (x.float().abs().amax(1) / 127.0).masked_fill(x.abs().amax(1) == 0, 1.0)
+    assert torch.isfinite(got).all()
+    assert_within(got, *finish64(product64(qa, sa, codes, scale), bias, epilogue, resid, 0.5))
+
+
 def _norm64(x, w, b, swish=0):
     """LayerNorm (and Swish) in 64 bits, and how far a float32 evaluation may be.  With u = 2^-24: the mean is a tree of at
     most 24 additions deep, so it is within 24 u mean|x|, and mean|x| rstd <= sqrt(1 + mean^2 / var), below 1.1 for
