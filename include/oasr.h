@@ -405,7 +405,7 @@ int oasr_gemm_fp8_pw(const uint8_t* a, const uint8_t* w_packed, const float* sca
  * x: rows of k values, `ldx` apart (any k, any alignment of a row's start); y: rows `ldy` apart (a multiple of 16, at
  * least k rounded up to 64; y 16-byte aligned), columns k .. round_up(k, 64) - 1 are written as zeros, the rest of the
  * pitch is left alone.  A row that holds a NaN or an infinity gets a scale that is NaN or infinite, and every output
- * made from it is NaN.  rows may be 0. */
+ * made from it is NaN.  rows may be 0 and must be below 2^24. */
 int oasr_quant_i8_rows(const uint16_t* x, int64_t ldx, int64_t rows, int64_t k, int8_t* y, int64_t ldy, float* scale,
                        void* stream);
 
@@ -418,12 +418,12 @@ int oasr_layernorm2_i8(float* x, const float* w1, const float* b1, const float* 
                        float* scale, int64_t rows, int32_t d, float eps, void* stream);
 
 /* Weights of the 8-bit product, laid out once: int8 codes w[n][k] (rows `ldw` apart) to pieces of 16 rows x 64 k,
- * padded with zeros; out holds oasr_gemm_i8_packed_bytes(n, k) bytes and is 16-byte aligned.  Any n, k <= 131072. */
+ * padded with zeros; out holds oasr_gemm_i8_packed_bytes(n, k) bytes (below 64 GiB) and is 16-byte aligned.  Any n, k <= 131072. */
 int64_t oasr_gemm_i8_packed_bytes(int64_t n, int64_t k);
 int oasr_gemm_pack_w_i8(const int8_t* w, int64_t ldw, int64_t n, int64_t k, int8_t* out, void* stream);
 
 /* C[m][n] = epilogue(scale_a[m] * scale_w[n] * sum_k A8[m][k] * W8[n][k]): sums in 32-bit integers, exact (k <= 131072).
- * Any m (0: nothing is done), n, k; epilogues of oasr_epilogue, bias float32[n] or NULL with each of them
+ * Any m (0: nothing is done), n, k (a result past some 2^30 x 64 elements is refused); epilogues of oasr_epilogue, bias float32[n] or NULL with each of them
  * (OASR_EPI_GLU_BF16: n a multiple of 32, bias interleaved as the rows are, C of n / 2 columns).
  * a: rows `lda` apart as oasr_quant_i8_rows writes them - 16-byte aligned, lda a multiple of 16 and at least k rounded up to
  * 64, zeros from k up to there.  c, resid: rows `ldc`, `ldr` elements apart; resid may be c (with ldr = ldc), apart from
@@ -434,7 +434,8 @@ int oasr_gemm_i8(const int8_t* a, int64_t lda, const int8_t* w_packed, const flo
 
 /* Both steps: the bf16 rows x (ldx apart) are quantised and multiplied.  The same bits as oasr_quant_i8_rows followed by
  * oasr_gemm_i8.  workspace: device, oasr_linear_i8_workspace_bytes(m, n, k) (0 for a few rows, which are quantised
- * inside the product), 256-byte aligned, contents on entry do not matter; calls that may overlap need one each. */
+ * inside the product), 256-byte aligned, contents on entry do not matter; calls that may overlap need one each.
+ * m below 2^24. */
 int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const float* scale_w, const float* bias,
                    const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, float alpha,
@@ -536,7 +537,8 @@ int oasr_gather_chunks(const float* pcm, int64_t pcm_len, const int64_t* start, 
  *   ids, best [r][0 .. top-1] = the likeliest tokens and their log probabilities, best first, ties to the lower index
  * float32 results, sums in float32.  A logit of -inf is a token ruled out: probability 0, never among the likeliest (id -1,
  * log probability -inf where fewer than `top` remain).  A row that allows nothing: log probabilities -inf, entropy 0, no
- * likeliest.  A NaN or +inf in a row: NaN results, ids -1.  top 0 .. 32, given (tokens per row) and rows may be 0.
+ * likeliest.  A NaN or +inf in a row: NaN results, ids -1.  top 0 .. 32, given (tokens per row) and rows may be 0;
+ * rows below 2^24, vocab below 2^30.
  * workspace: device, oasr_token_scores_workspace_bytes(rows, vocab, top) bytes (0 for most sizes), 256-byte aligned,
  * contents on entry do not matter; calls that may overlap need one each. */
 typedef enum oasr_dtype { OASR_F32 = 0, OASR_BF16 = 1 } oasr_dtype;

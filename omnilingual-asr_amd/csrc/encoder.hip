@@ -128,6 +128,7 @@ int oasr_encoder_set_int8(oasr_encoder* enc, const oasr_layer_int8_weights* laye
         return OASR_OK;
     }
     OASR_REQUIRE(enc->fp8.empty(), "encoder_set_int8: the encoder has e4m3 weights");
+    OASR_REQUIRE(enc->cfg.d_model % 64 == 0 && enc->cfg.ffn_dim % 64 == 0, "encoder_set_int8: dimensions must be multiples of 64");
     for (int l = 0; l < enc->cfg.n_layers; ++l) {
         const oasr_layer_int8_weights& w = layers[l];
         OASR_REQUIRE(w.ffn1_w1_q && w.ffn1_w1_s && w.ffn1_w2_q && w.ffn1_w2_s && w.wqkv_q && w.wqkv_s && w.wo_q &&

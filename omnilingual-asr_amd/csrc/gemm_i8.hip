@@ -21,6 +21,9 @@ namespace i8 {
 constexpr int kSlice = 64;                 // k per slice: one MFMA step
 constexpr int kPiece = 16 * kSlice;        // bytes of 16 rows of a slice
 constexpr int64_t kMaxK = 131072;          // 128 * 127 * k < 2^31
+constexpr int64_t kMaxGroups = (int64_t)1 << 23;        // of 512 threads: a launch has fewer than 2^32 threads
+constexpr int64_t kMaxRows = (int64_t)1 << 24;          // one of 256 threads each at most
+constexpr int64_t kMaxWideTiles = (int64_t)1 << 30;     // walked by 256 work-groups, counted in 32 bits
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void gbl_void;
@@ -905,7 +908,9 @@ static int few_rows(int64_t m, int64_t n, int64_t k) {
 
 static int launch_few(int mt, const GemmArgs& p, const uint16_t* x, int64_t ldx, int64_t k, int32_t epilogue, hipStream_t st) {
     const int tm = (int)((p.m + 16 * mt - 1) / (16 * mt));
-    const dim3 grid((unsigned)(tm * ((p.n + kFewColumns - 1) / kFewColumns))), blk(512);
+    const int64_t groups = tm * ((p.n + kFewColumns - 1) / kFewColumns);
+    OASR_REQUIRE(groups < kMaxGroups, "linear_i8: m=%lld x n=%lld is too large a result", (long long)p.m, (long long)p.n);
+    const dim3 grid((unsigned)groups), blk(512);
 #define OASR_FEW(E)                                                                                             \
     do {                                                                                                        \
         if (mt == 1) hipLaunchKernelGGL((linear_i8_few_kernel<E, 1>), grid, blk, 0, st, p, x, ldx, (int)k, tm); \
@@ -926,7 +931,8 @@ static int launch_few(int mt, const GemmArgs& p, const uint16_t* x, int64_t ldx,
 static int launch_gemm(const GemmArgs& p, int32_t epilogue, hipStream_t st) {
     const int form = choose_form(p);
     const Form& t = kFormTable[form];
-    OASR_REQUIRE((p.m + t.bm - 1) / t.bm * ((p.n + t.bn - 1) / t.bn) < ((int64_t)1 << 30), "gemm_i8: too many tiles");
+    OASR_REQUIRE((p.m + t.bm - 1) / t.bm * ((p.n + t.bn - 1) / t.bn) < (form == kTile256 ? kMaxWideTiles : kMaxGroups),
+                 "gemm_i8: m=%lld x n=%lld is too large a result", (long long)p.m, (long long)p.n);
     switch (epilogue) {
         case OASR_EPI_BIAS_BF16: launch_form<OASR_EPI_BIAS_BF16>(form, p, st); break;
         case OASR_EPI_BIAS_SWISH_BF16: launch_form<OASR_EPI_BIAS_SWISH_BF16>(form, p, st); break;
@@ -1003,7 +1009,7 @@ extern "C" {
 int oasr_quant_i8_rows(const uint16_t* x, int64_t ldx, int64_t rows, int64_t k, int8_t* y, int64_t ldy, float* scale,
                        void* stream) {
     OASR_REQUIRE(rows >= 0 && k > 0, "quant_i8_rows: k must be positive and rows not negative");
-    OASR_REQUIRE(rows < ((int64_t)1 << 31), "quant_i8_rows: too many rows");
+    OASR_REQUIRE(rows < i8::kMaxRows, "quant_i8_rows: rows must be below 2^24");
     OASR_REQUIRE(ldx >= k && ldy % 16 == 0 && ldy >= round_up(k, i8::kSlice),
                  "quant_i8_rows: ldx must cover k, ldy must be a multiple of 16 and cover k rounded up to 64");
     if (rows == 0) return OASR_OK;
@@ -1025,7 +1031,7 @@ int oasr_gemm_pack_w_i8(const int8_t* w, int64_t ldw, int64_t n, int64_t k, int8
     OASR_REQUIRE(w && out && w != out, "gemm_pack_w_i8: null pointer or in-place call");
     OASR_REQUIRE(((uintptr_t)out & 15) == 0, "gemm_pack_w_i8: out must be 16-byte aligned");
     const int64_t chunks = oasr_gemm_i8_packed_bytes(n, k) / 16;
-    OASR_REQUIRE(chunks / 256 + 1 < ((int64_t)1 << 31), "gemm_pack_w_i8: matrix too large");
+    OASR_REQUIRE(chunks < ((int64_t)1 << 32) - 256, "gemm_pack_w_i8: the packed weights must be below 64 GiB");
     hipLaunchKernelGGL(i8::gemm_pack_w_i8_kernel, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, (hipStream_t)stream, w, ldw,
                        n, k, round_up(k, i8::kSlice) / i8::kSlice, chunks, out);
     OASR_CHECK_LAUNCH("gemm_pack_w_i8");
@@ -1068,6 +1074,7 @@ int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const
                   (long long)workspace_bytes);
         return OASR_ECAPACITY;
     }
+    OASR_REQUIRE(m < i8::kMaxRows, "linear_i8: m must be below 2^24");
     const int64_t kp = round_up(k, i8::kSlice);
     int8_t* q = static_cast<int8_t*>(workspace);
     float* s = reinterpret_cast<float*>(q + round_up(m * kp, 256));

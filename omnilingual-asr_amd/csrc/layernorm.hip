@@ -273,7 +273,7 @@ static int launch_ln(const float* x, const float* w, const float* b, void* y, in
 template <bool SWISH, bool TWO>
 static int launch_ln_i8(const char* what, float* x, const float* w1, const float* b1, const float* w2, const float* b2, int8_t* y,
                         float* scale, int64_t rows, int32_t d, float eps, hipStream_t st) {
-    OASR_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 33), "%s: bad row count", what);
+    OASR_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 26) - 4, "%s: rows must lie in [0, 2^26 - 4)", what);      // 64 threads each
     OASR_REQUIRE(d == 256 || d == 512 || d == 1024 || d == 2048 || d == 4096, "%s: unsupported width %d (256, 512, 1024, 2048, 4096)",
                  what, d);
     if (rows == 0) return OASR_OK;

@@ -634,7 +634,7 @@ static void launch(const Args& p, hipStream_t st) {
 
 static int run(const char* what, Args& p, int32_t dtype, void* workspace, int64_t bytes, hipStream_t st) {
     OASR_REQUIRE(dtype == OASR_F32 || dtype == OASR_BF16, "%s: dtype must be OASR_F32 or OASR_BF16", what);
-    OASR_REQUIRE(p.rows >= 0 && p.rows < ((int64_t)1 << 31) / kMaxSplits, "%s: rows must lie in [0, 2^25)", what);
+    OASR_REQUIRE(p.rows >= 0 && p.rows < ((int64_t)1 << 24), "%s: rows must lie in [0, 2^24)", what);      // 256 threads each at most
     OASR_REQUIRE(p.vocab > 0 && p.vocab < (1 << 30), "%s: vocab must lie in [1, 2^30)", what);
     OASR_REQUIRE(p.ld >= p.vocab, "%s: ld=%lld does not cover the vocabulary", what, (long long)p.ld);
     OASR_REQUIRE(p.given >= 0, "%s: the count of given tokens is negative", what);

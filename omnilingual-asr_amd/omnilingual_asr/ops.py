@@ -67,7 +67,7 @@ def _overlap(a, b) -> bool:
 def _vector(t, n: int, what: str, device) -> int | None:
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{what} must be a contiguous float32 vector of {n} on {device}")
     return t.data_ptr()
 
@@ -78,13 +78,17 @@ class LinearI8:
 
     `epilogue`: "bias" -> bf16, "swish" -> bf16, "glu" -> bf16 of half the width (rows of W interleaved as
     `weights.glu_interleave` does, a multiple of 32), "float" -> float32, "residual" -> resid + alpha * (...) in float32.
-    The packed weights belong to the object and must not be in use by another stream when it is dropped."""
+    Forward only: results carry no gradient.  The weights are packed on the stream that is current when the object is made; a
+    call on another stream has to wait for that one, as for any tensor made there.  The packed weights belong to the object
+    and must not be in use by another stream when it is dropped."""
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None):
         """`weight`: float [out, in] on a HIP device; quantised per output row."""
         if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_floating_point():
             raise ValueError("weight must be a float tensor [out, in]")
-        self._lay_out(*quantize_rows_i8(weight), bias)
+        if weight.shape[1] < 1:
+            raise ValueError("weight must have at least one column")
+        self._lay_out(*quantize_rows_i8(weight.detach()), bias)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None) -> "LinearI8":
@@ -94,7 +98,7 @@ class LinearI8:
         return self
 
     def _lay_out(self, codes, scale, bias):
-        if codes.dim() != 2:
+        if not isinstance(codes, torch.Tensor) or codes.dim() != 2:
             raise ValueError("codes must be [out, in]")
         codes, n, k, ldw = _rows(codes, "codes", _INT8)
         if n < 1 or not 1 <= k <= 131072:
@@ -125,7 +129,7 @@ class LinearI8:
             out = x.new_empty(shape, dtype=dtype)
             if epi != _hip.EPI_RESIDUAL_F32 and resid is None:
                 return epi, out, n, None, 0
-        elif out.shape != shape or out.device != self.device:
+        elif not isinstance(out, torch.Tensor) or out.shape != shape or out.device != self.device:
             raise ValueError(f"out must be of shape {shape} on {self.device}")
         flat, _, _, ldc = _rows(out, "out", (dtype,))
         if given and flat.data_ptr() != out.data_ptr():
@@ -136,7 +140,7 @@ class LinearI8:
             if resid is not None:
                 raise ValueError("resid goes with the residual epilogue only")
             return epi, out, ldc, None, 0
-        if resid is None or resid.shape != shape or resid.device != self.device:
+        if not isinstance(resid, torch.Tensor) or resid.shape != shape or resid.device != self.device:
             raise ValueError(f"the residual epilogue needs resid of shape {shape} on {self.device}")
         r, _, _, ldr = _rows(resid, "resid", _FLOAT32)
         if given and _overlap(flat, r) and (r.data_ptr() != flat.data_ptr() or ldr != ldc):
@@ -169,6 +173,8 @@ class LinearI8:
         if k not in _NORM_WIDTHS or ldx != k or x2.data_ptr() % 16:
             raise ValueError(f"normed takes contiguous, 16-byte aligned rows of {', '.join(map(str, _NORM_WIDTHS))} columns")
         gain_ptr, shift_ptr = _vector(gain, k, "gain", self.device), _vector(shift, k, "shift", self.device)
+        if gain_ptr is None or shift_ptr is None or (gain_ptr | shift_ptr) % 16:
+            raise ValueError("gain and shift must be given, 16-byte aligned")
         epi, out, ldc, resid, ldr = self._output(x, epilogue, resid, out)
         if m == 0:
             return out

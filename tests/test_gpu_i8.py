@@ -265,6 +265,15 @@ def test_largest_sums_are_exact():
         ops.LinearI8.from_codes(torch.zeros((1, k + 1), dtype=torch.int8, device="cuda"), torch.ones((1,), device="cuda"))
 
 
+def test_parameters_of_a_module():
+    """Weights and biases that a module holds (they require gradients) make a layer that keeps no graph of them."""
+    lin = torch.nn.Linear(96, 40, device="cuda")
+    layer = ops.LinearI8(lin.weight, lin.bias)
+    x = torch.randn((7, 96), device="cuda").to(torch.bfloat16)
+    assert not layer.scale.requires_grad
+    assert torch.equal(layer(x), ops.LinearI8(lin.weight.detach().clone(), lin.bias.detach().clone())(x))
+
+
 def test_offsets_past_32_bits():
     m, n, k = 66000, 33000, 64
     g = torch.Generator().manual_seed(9)
@@ -289,6 +298,7 @@ def test_refusals_on_the_device():
     x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
     y = x.clone()
     z = torch.zeros((5, 48), device="cuda")
+    wide, f, v = ops.LinearI8(torch.ones((16, 512), device="cuda")), torch.zeros((4, 512), device="cuda"), torch.ones(520, device="cuda")
     bad = [
         (lambda: layer(x[:, :63]), "64 columns"), (lambda: layer(x.float()), "bfloat16"), (lambda: layer(x, epilogue="gelu"), "epilogue"),
         (lambda: layer(x, epilogue="glu"), "multiple of 32"), (lambda: layer(x, epilogue="residual"), "resid"),
@@ -302,6 +312,9 @@ def test_refusals_on_the_device():
         (lambda: layer(x.t()[:, :1].expand(64, 64)[:4]), "contiguous rows"),
         (lambda: layer(torch.zeros((1, 64), dtype=torch.bfloat16, device="cuda").expand(4, 64)), "overlap"),
         (lambda: layer.normed(x.float(), s, s), "normed"), (lambda: layer.normed(x, s, s), "float32"),
+        (lambda: layer(x, out=[0.0]), "out must be"), (lambda: layer(x, epilogue="residual", resid=1.0), "resid"),
+        (lambda: wide.normed(f, v[:512], v[1:513]), "aligned"), (lambda: wide.normed(f, v[:512], None), "given"),
+        (lambda: ops.LinearI8.from_codes(c, 1.0), "scale"),
         (lambda: ops.LinearI8.from_codes(c, s[:4]), "scale"), (lambda: ops.LinearI8.from_codes(c, None), "scale"),
         (lambda: ops.LinearI8.from_codes(c, s, s.double()), "bias"), (lambda: ops.LinearI8.from_codes(c.t(), s), "contiguous rows"),
     ]

@@ -60,6 +60,18 @@ def test_operand_refusals():
     assert pack(k=131073, ldw=131073) == -1
 
 
+def test_sizes_beyond_a_launch_are_refused():
+    """A launch has fewer than 2^32 threads: what would need more is refused, not cut short."""
+    L = _hip.lib()
+    text = lambda: L.oasr_last_error().decode()
+    assert L.oasr_quant_i8_rows(A, 16, 1 << 24, 16, A, 64, A, None) == -1 and "2^24" in text()
+    assert L.oasr_layernorm_i8(A, A, A, A, A, (1 << 26) - 4, 256, 1e-5, 0, None) == -1 and "2^26" in text()
+    assert L.oasr_gemm_pack_w_i8(A, 64, (1 << 30) + 1, 64, 2 * A, None) == -1 and "64 GiB" in text()
+    assert _gemm(m=(1 << 31) - 1, n=(1 << 31) - 1, ldc=1 << 31) == -1 and "too large" in text()
+    assert _linear(m=1, n=1 << 28, ldc=1 << 28) == -1 and "too large" in text()
+    assert _linear(m=1 << 24, ldx=2048, k=2048, bytes=1 << 50) == -1 and "2^24" in text()
+
+
 def test_packed_bytes():
     f = _hip.lib().oasr_gemm_i8_packed_bytes
     assert f(1, 1) == 1024 and f(16, 64) == 1024 and f(17, 64) == 2048 and f(16, 65) == 2048 and f(0, 4) == 0 and f(4, -1) == 0
@@ -75,6 +87,10 @@ def test_tensor_refusals_without_a_device():
         ops.LinearI8.from_codes(torch.zeros((4,), dtype=torch.int8), torch.ones((4,)))
     with pytest.raises(ValueError, match="int8"):
         ops.LinearI8.from_codes(w, torch.ones((32,)))
+    with pytest.raises(ValueError, match="one column"):
+        ops.LinearI8(torch.zeros((32, 0)))
+    with pytest.raises(ValueError, match=r"\[out, in\]"):
+        ops.LinearI8.from_codes(None, None)
     layer = ops.LinearI8.__new__(ops.LinearI8)
     layer.device, layer.in_features, layer.out_features = torch.device("cpu"), 64, 32
     with pytest.raises(ValueError, match="HIP device"):

@@ -16,7 +16,7 @@ def _scores(**kw):
 
 
 @pytest.mark.parametrize("kw,text", [
-    (dict(dtype=2), "dtype"), (dict(rows=-1), "rows"), (dict(rows=1 << 25), "rows"), (dict(vocab=0), "vocab"),
+    (dict(dtype=2), "dtype"), (dict(rows=-1), "rows"), (dict(rows=1 << 25), "rows"), (dict(rows=1 << 24), "rows"), (dict(vocab=0), "vocab"),
     (dict(vocab=1 << 30, ld=1 << 30), "vocab"), (dict(ld=59), "ld"), (dict(given=-1), "given"), (dict(top=-1), "top"),
     (dict(top=33), "top"), (dict(z=None), "null"), (dict(tok=None), "null"), (dict(lp=None), "null"), (dict(ids=None), "null"),
     (dict(best=None), "null"), (dict(z=A + 2), "misaligned"), (dict(dtype=1, z=A + 1), "misaligned"), (dict(ent=A + 2), "misaligned"),
