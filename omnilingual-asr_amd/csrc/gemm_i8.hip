@@ -21,7 +21,7 @@ namespace i8 {
 constexpr int kSlice = 64;                 // k per slice: one MFMA step
 constexpr int kPiece = 16 * kSlice;        // bytes of 16 rows of a slice
 constexpr int64_t kMaxK = 131072;          // 128 * 127 * k < 2^31
-constexpr int64_t kMaxGroups = (int64_t)1 << 23;        // of 512 threads: a launch has fewer than 2^32 threads
+constexpr int64_t kMaxGroups = (int64_t)7 << 20;        // of 512 threads, and an eighth more: a launch has fewer than 2^32 threads
 constexpr int64_t kMaxRows = (int64_t)1 << 24;          // one of 256 threads each at most
 constexpr int64_t kMaxWideTiles = (int64_t)1 << 30;     // walked by 256 work-groups, counted in 32 bits
 
@@ -53,6 +53,41 @@ __device__ __forceinline__ uint32_t cvt_pk_bf16(float a, float b) {
     v[1] = (__bf16)b;
     return __builtin_bit_cast(uint32_t, v);
 }
+
+// Division of numbers below 2^32 by one that the host knows: a product with floor((2^32 - 1) / d), which is at most one too small,
+// and a correction (the division itself takes some hundred cycles, and a kernel's first addresses wait for it).
+// (Tiles of the 256 x 256 form found this way: 12032 x 16384 x 4096 669 -> 658 us, 48128 x 2048 x 1024 gated 123.9 -> 121.5.)
+struct Divisor {
+    uint32_t d, inv;
+
+    Divisor() = default;
+    __host__ __device__ explicit Divisor(int64_t by) : d((uint32_t)by), inv(0xffffffffu / d) {}
+    __device__ __forceinline__ void split(int v, int& quotient, int& rest) const {
+        uint32_t q = __umulhi((uint32_t)v, inv), r = (uint32_t)v - q * d;
+        if (r >= d) ++q, r -= d;
+        quotient = (int)q;
+        rest = (int)r;
+    }
+};
+
+// Which tile a work-group computes.  Work-groups with equal blockIdx % 8 share an XCD and its L2 (used for locality only): each
+// XCD gets a block of `rows` x `cols` tiles, so that it fetches few rows of A and few of W.  cols = 0: column by column.
+struct TileMap {
+    int tiles_m, tiles_n, across, cols;         // 2^across blocks side by side along m
+    Divisor rows;
+
+    __device__ __forceinline__ bool tile(int& tm, int& tn) const {
+        if (cols == 0) {
+            rows.split((int)blockIdx.x, tn, tm);
+            return true;
+        }
+        rows.split((int)(blockIdx.x >> 3), tn, tm);
+        const int xcd = blockIdx.x & 7;
+        tm += (xcd & ((1 << across) - 1)) * (int)rows.d;
+        tn += (xcd >> across) * cols;
+        return tm < tiles_m && tn < tiles_n;
+    }
+};
 
 #define OASR_I8_BARRIER()                     \
     do {                                      \
@@ -274,7 +309,7 @@ struct Epilogue {
 // has seen its own copies of slice p land and has read slice p - 1, so the slot of p - 1 may be filled again.
 // Rows of A past m repeat row m - 1 and row groups of W past the last repeat the last: read, multiplied, never stored.
 template <int EPI, int WM, int WN, int MT, int NT, int RING>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmArgs p, int tiles_n) {
+__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmArgs p, const TileMap map) {
     constexpr int kWaves = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
     constexpr int kPieces = (BM + BN) / 16, kCopies = kPieces / kWaves, kSlot = kPieces * kPiece;
     static_assert(kPieces % kWaves == 0, "every wave issues the same number of copies");
@@ -282,7 +317,9 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmAr
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * BM, n0 = (int64_t)(blockIdx.x % tiles_n) * BN;
+    int tm, tn;
+    if (!map.tile(tm, tn)) return;           // the whole work-group
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
 
     const char* src[kCopies];
     int step[kCopies];
@@ -369,16 +406,23 @@ __global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int
     const int local = banded ? m_cnt * tiles_n : (int)((int64_t)n_tiles * (xcd + 1) / 8) - flat_lo;
     if (first >= local) return;
     const int mine = (local - first + stride - 1) / stride;
+    const Divisor by_band(banded ? m_cnt * 4 : tiles_n), by_rest(max(tiles_n & 3, 1));
     auto tile_at = [&](int i, int& tm, int& tn) {
         const int l = first + i * stride;
         if (!banded) {
-            tm = (flat_lo + l) / tiles_n;
-            tn = (flat_lo + l) % tiles_n;
+            by_band.split(flat_lo + l, tm, tn);
             return;
         }
-        const int band = l / (m_cnt * 4), width = min(4, tiles_n - 4 * band), in = l - band * m_cnt * 4;
-        tm = m_lo + in / width;
-        tn = 4 * band + in % width;
+        int band, in;
+        by_band.split(l, band, in);
+        if (4 * band + 4 <= tiles_n) {
+            tm = in >> 2;
+            tn = in & 3;
+        } else {
+            by_rest.split(in, tm, tn);
+        }
+        tm += m_lo;
+        tn += 4 * band;
     };
 
     i32x4 acc[8][4];
@@ -491,13 +535,15 @@ struct SplitShape {
 };
 
 template <int EPI, int MT>
-__global__ __launch_bounds__(512) void gemm_i8_split_kernel(const GemmArgs p, int tiles_m) {
+__global__ __launch_bounds__(512) void gemm_i8_split_kernel(const GemmArgs p, const TileMap map) {
     typedef SplitShape<MT> Shape;
     constexpr int D = Shape::kDepth;
     __shared__ __attribute__((aligned(1024))) char lds[Shape::kLds];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t m0 = (int64_t)(blockIdx.x % tiles_m) * (16 * MT), n0 = (int64_t)(blockIdx.x / tiles_m) * 64;
+    int tm, tn;
+    if (!map.tile(tm, tn)) return;           // the whole work-group
+    const int64_t m0 = (int64_t)tm * (16 * MT), n0 = (int64_t)tn * 64;
 
     char* const ring = lds + wave * Shape::kRingBytes;
     const char* src_a[MT];
@@ -849,15 +895,15 @@ static int check_gemm(const char* what, const int8_t* w, const float* scale_w, c
 // k 512 .. 16384) and pick within 1.4 % of the fastest form on average: e.g. 1504 x 1024 x 4096: 96 rows split 14.8 us, 128 x 128
 // tiles 25.8, 256 x 256 43.4; 1504 x 4096 x 1024: 23.2 (32 rows split), 14.4, 20.1; 512 x 1024 x 512: 4.5, 6.2, 10.0.
 // 16 rows split re-read the weights once per row tile: with more than 128 work-groups of them 32 rows are faster
-// (99 x 2048 x 4096: 8.9 against 11.6 us).
+// (300 x 4096 x 4096: 17.4 against 22.3 us).
 struct Form {
     int bm, bn, slices;         // tile, slices per step
     double begin, step, share;
 };
 enum { kSplit16, kSplit32, kSplit64, kSplit96, kSplit128, kTile128, kTile256, kForms };
 static const Form kFormTable[kForms] = {
-    {16, 64, 8, 1.50, 0.57, 0.7}, {32, 64, 8, 1.64, 0.68, 0.8},  {64, 64, 8, 2.40, 0.84, 1.0},  {96, 64, 8, 4.05, 1.10, 1.0},
-    {128, 64, 8, 4.35, 1.38, 1.0}, {128, 128, 1, 4.10, 0.33, 0.68}, {256, 256, 1, 11.3, 0.51, 1.0}};
+    {16, 64, 8, 1.31, 0.50, 0.7}, {32, 64, 8, 1.69, 0.62, 0.8},  {64, 64, 8, 2.44, 0.79, 1.0},  {96, 64, 8, 3.93, 1.06, 1.0},
+    {128, 64, 8, 4.49, 1.31, 1.0}, {128, 128, 1, 4.23, 0.32, 0.7}, {256, 256, 1, 10.4, 0.54, 1.0}};
 
 static int choose_form(const GemmArgs& p) {
     int best = kTile128;
@@ -877,19 +923,40 @@ static int choose_form(const GemmArgs& p) {
     return best;
 }
 
+// The map of a launch of tm x tn tiles of bm x bn, and its work-groups (a few of which may have no tile).  Of the ways to deal
+// the tiles to the eight XCDs as 1 x 8, 2 x 4, 4 x 2 or 8 x 1 blocks, the one that fetches least; rows of A count six times (they
+// come in half lines, 64 bytes per slice: with a weight of one 1504 x 1024 x 4096 takes 22.1 us instead of 20.2, with four
+// 1000 x 1000 x 4096 18.1 instead of 16.6).  A way that leaves an XCD more than an eighth above the average, or needs another
+// round of work-groups, is out.  Against tiles dealt column by column, calls with their quantiser: 50 x 8192 x 8192 29.3 -> 18.3 us,
+// 100 x 4096 x 16384 54.4 -> 26.0, 900 x 1024 x 8192 29.4 -> 24.6, 1504 x 4096 x 1024 19.5 -> 18.1; 2000 x 1024 x 4096 23.4 -> 24.0.
+static int64_t map_tiles(int tm, int tn, int bm, int bn, TileMap& map) {
+    const int64_t tiles = (int64_t)tm * tn;
+    map = {tm, tn, 0, 0, Divisor(tm)};
+    int64_t least = INT64_MAX;
+    for (int a = 0; a < 4; ++a) {
+        const int rows = (tm + (1 << a) - 1) >> a, cols = (tn + (8 >> a) - 1) / (8 >> a);
+        const int64_t cost = 6 * (int64_t)rows * bm + (int64_t)cols * bn, most = (int64_t)rows * cols;
+        if (64 * most > 9 * tiles || (most + 31) / 32 > (tiles + 255) / 256 || cost >= least) continue;
+        least = cost;
+        map = {tm, tn, a, cols, Divisor(rows)};
+    }
+    return map.cols ? 8 * (int64_t)map.rows.d * map.cols : tiles;
+}
+
 template <int EPI>
 static void launch_form(int form, const GemmArgs& p, hipStream_t st) {
     const Form& t = kFormTable[form];
     const int tm = (int)((p.m + t.bm - 1) / t.bm), tn = (int)((p.n + t.bn - 1) / t.bn);
     const int64_t tiles = (int64_t)tm * tn;
-    const dim3 grid((unsigned)tiles), split(512);
+    TileMap map;
+    const dim3 grid((unsigned)map_tiles(tm, tn, t.bm, t.bn, map)), split(512);
     switch (form) {
-        case kSplit16: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 1>), grid, split, 0, st, p, tm); break;
-        case kSplit32: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 2>), grid, split, 0, st, p, tm); break;
-        case kSplit64: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 4>), grid, split, 0, st, p, tm); break;
-        case kSplit96: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 6>), grid, split, 0, st, p, tm); break;
-        case kSplit128: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 8>), grid, split, 0, st, p, tm); break;
-        case kTile128: hipLaunchKernelGGL((gemm_i8_tile_kernel<EPI, 2, 2, 4, 4, 4>), grid, dim3(256), 0, st, p, tn); break;
+        case kSplit16: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 1>), grid, split, 0, st, p, map); break;
+        case kSplit32: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 2>), grid, split, 0, st, p, map); break;
+        case kSplit64: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 4>), grid, split, 0, st, p, map); break;
+        case kSplit96: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 6>), grid, split, 0, st, p, map); break;
+        case kSplit128: hipLaunchKernelGGL((gemm_i8_split_kernel<EPI, 8>), grid, split, 0, st, p, map); break;
+        case kTile128: hipLaunchKernelGGL((gemm_i8_tile_kernel<EPI, 2, 2, 4, 4, 4>), grid, dim3(256), 0, st, p, map); break;
         default:
             hipLaunchKernelGGL((gemm_i8_wide_kernel<EPI>), dim3((unsigned)(tiles < 256 ? (tiles + 7) / 8 * 8 : 256)), dim3(512), 0, st, p, tm, tn);
     }
@@ -908,9 +975,9 @@ static int few_rows(int64_t m, int64_t n, int64_t k) {
 
 static int launch_few(int mt, const GemmArgs& p, const uint16_t* x, int64_t ldx, int64_t k, int32_t epilogue, hipStream_t st) {
     const int tm = (int)((p.m + 16 * mt - 1) / (16 * mt));
-    const int64_t groups = tm * ((p.n + kFewColumns - 1) / kFewColumns);
-    OASR_REQUIRE(groups < kMaxGroups, "linear_i8: m=%lld x n=%lld is too large a result", (long long)p.m, (long long)p.n);
-    const dim3 grid((unsigned)groups), blk(512);
+    const int64_t tn = (p.n + kFewColumns - 1) / kFewColumns;
+    OASR_REQUIRE(tm * tn < kMaxGroups, "linear_i8: m=%lld x n=%lld is too large a result", (long long)p.m, (long long)p.n);
+    const dim3 grid((unsigned)(tm * tn)), blk(512);
 #define OASR_FEW(E)                                                                                             \
     do {                                                                                                        \
         if (mt == 1) hipLaunchKernelGGL((linear_i8_few_kernel<E, 1>), grid, blk, 0, st, p, x, ldx, (int)k, tm); \

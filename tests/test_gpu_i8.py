@@ -449,3 +449,18 @@ def test_int8_transcription_with_scores():
             assert (s.ids == top.numpy()).all() and (s.ids[:, 0] == ids).all()
     with pytest.raises(ValueError, match="decode"):
         eng.score(torch.zeros((5, 7), dtype=torch.int32, device="cuda"), torch.zeros((5, 7), dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("m,n,k", [(100, 4096, 4160), (50, 8192, 1088), (300, 4100, 2050), (900, 1024, 2048), (1000, 1000, 1100), (130, 1030, 1030),
+                                   (800, 3000, 700), (2500, 1000, 500), (1037, 2081, 1025)])
+def test_every_tile_is_computed_once(m, n, k):
+    """Tiles dealt to the chip's parts as blocks, ragged ones among them: every output is there and exact."""
+    g = torch.Generator().manual_seed(m + n + k)
+    a = torch.randint(-3, 4, (m, k), generator=g).to(torch.bfloat16)
+    a[:, 0] = 127                                       # every row's scale is 1, its codes are its values
+    codes = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8)
+    layer = ops.LinearI8.from_codes(codes.cuda(), torch.ones((n,), device="cuda"))
+    out = torch.full((m, n), float("nan"), device="cuda")
+    layer(a.cuda(), epilogue="float", out=out)
+    want = a.cuda().float() @ codes.cuda().float().t()  # below 2^24: exact in float32
+    assert (want.abs() < 2 ** 24).all() and torch.equal(out, want)
