@@ -8,8 +8,8 @@
 // rows and k padded with zeros; a piece holds its 16-byte chunks in the order in which the lanes of a fragment take them
 // (lane = (row lane & 15, chunk lane >> 4)), so a fragment is one contiguous KiB, in memory as in LDS.  A's rows stay
 // row-major: a copy brings 16 rows x 64 k with four neighbouring lanes per row (whole 64-byte segments) and its source
-// addresses put chunk c of row r at place c ^ ((r >> 2) & 3) of the row, which keeps the fragment reads free of bank
-// conflicts.
+// addresses put chunk c of row r at place c ^ (-(r >> 2) & 3) of the row, which keeps the fragment reads free of bank
+// conflicts (with (r >> 2) & 3 they take twice as long: a read's groups of sixteen lanes are not lanes 0 .. 15).
 // The weight fragment is the matrix instruction's A operand (v_mfma_i32_16x16x64_i8), so a lane ends up with four
 // consecutive n of one row m: C[m = lane & 15][n = 4 (lane >> 4) + e].
 #include "oasr_common.h"
@@ -53,6 +53,8 @@ __device__ __forceinline__ uint32_t cvt_pk_bf16(float a, float b) {
     v[1] = (__bf16)b;
     return __builtin_bit_cast(uint32_t, v);
 }
+
+__device__ __forceinline__ int turned(int row) { return (4 - (row >> 2)) & 3; }      // of a piece's rows 0 .. 15
 
 // Division of numbers below 2^32 by one that the host knows: a product with floor((2^32 - 1) / d), which is at most one too small,
 // and a correction (the division itself takes some hundred cycles, and a kernel's first addresses wait for it).
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmAr
         if (q < BM / 16) {
             int64_t row = m0 + 16 * q + (lane >> 2);
             row = row < p.m ? row : p.m - 1;
-            src[i] = reinterpret_cast<const char*>(p.a) + row * p.lda + (((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+            src[i] = reinterpret_cast<const char*>(p.a) + row * p.lda + (((lane & 3) ^ turned(lane >> 2)) << 4);
             step[i] = kSlice;
         } else {
             int64_t grp = n0 / 16 + (q - BM / 16);
@@ -352,7 +354,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmAr
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
-    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ ((fr >> 2) & 3)) << 4);
+    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ turned(fr)) << 4);
 
     for (int t = 0; t < RING - 1 && t < p.ks; ++t) copy_next(t);
     int slot = 0, fill = RING - 1;
@@ -428,9 +430,9 @@ __global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int
 
     i32x4 acc[8][4];
     const int nph = p.ks, total = mine * nph;
-    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ ((fr >> 2) & 3)) << 4);
+    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ turned(fr)) << 4);
     // Copies: wave w brings rows 32 w .. 32 w + 31 of both operands' slices, two pieces each.  Rows past the last repeat it.
-    const uint32_t chunk = (uint32_t)(((lane & 3) ^ ((lane >> 4) & 3)) << 4);
+    const uint32_t chunk = (uint32_t)(((lane & 3) ^ turned(lane >> 2)) << 4);
     const char *src_a, *src_w0, *src_w1;
     uint32_t off0, off1;
     int st_i = 0, st_t = 0;
@@ -552,7 +554,7 @@ __global__ __launch_bounds__(512) void gemm_i8_split_kernel(const GemmArgs p, co
     for (int i = 0; i < MT; ++i) {
         int64_t row = m0 + 16 * i + (lane >> 2);
         row = row < p.m ? row : p.m - 1;
-        src_a[i] = reinterpret_cast<const char*>(p.a) + row * p.lda + (((lane & 3) ^ ((lane >> 4) & 3)) << 4) + wave * kSlice;
+        src_a[i] = reinterpret_cast<const char*>(p.a) + row * p.lda + (((lane & 3) ^ turned(lane >> 2)) << 4) + wave * kSlice;
     }
     const char* src_w[4];
 #pragma unroll
@@ -579,7 +581,7 @@ __global__ __launch_bounds__(512) void gemm_i8_split_kernel(const GemmArgs p, co
             src_w[j] += 8 * kPiece;
         }
     };
-    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ ((fr >> 2) & 3)) << 4);
+    const int fr = lane & 15, frag = fr * 64 + (((lane >> 4) ^ turned(fr)) << 4);
 #pragma unroll
     for (int d = 0; d < D - 1; ++d)
         if (d < count) request(d, wf[d]);
