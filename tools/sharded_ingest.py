@@ -70,8 +70,10 @@ for kind in kinds:
     limit = total * (1.0 / world) + (total / max(len(want.segments), 1)) + 2000
     ok = same and 0 < share <= limit and any(s.text for s in got.segments)
     ok_all = ok_all and ok
-    print("rank %d of %d, %s: %d segments, equal to the unsharded result: %s, read %d of %d source samples (%.0f %%)"
-          % (rank, world, kind, len(got.segments), same, share, total, 100.0 * share / total), flush=True)
+    # one write with its newline: an unbuffered print makes two, and the ranks' lines could run into each other
+    sys.stdout.write("rank %d of %d, %s: %d segments, equal to the unsharded result: %s, read %d of %d source samples (%.0f %%)\n"
+                     % (rank, world, kind, len(got.segments), same, share, total, 100.0 * share / total))
+    sys.stdout.flush()
     dist.barrier()
     if kind in ("wav", "ogg") and rank == 0:
         path.unlink()
