@@ -319,12 +319,20 @@ struct Sums {
     float m, s, t;
 };
 
+// A lane's largest value, the chunk at which the step that held it began, and the largest of its other steps.
+struct Tops {
+    float first, second;
+    int where;
+};
+
 template <int N>
-__device__ __forceinline__ void add_values(Sums& a, float& top, const float (&z)[N]) {
+__device__ __forceinline__ void add_values(Sums& a, Tops& top, int at, const float (&z)[N]) {
     float b = z[0];
 #pragma unroll
     for (int j = 1; j < N; ++j) b = fmaxf(b, z[j]);
-    top = fmaxf(top, b);
+    top.second = fmaxf(top.second, fminf(top.first, b));
+    top.where = b > top.first ? at : top.where;
+    top.first = fmaxf(top.first, b);
     if (__any(b > a.m)) {
         const float m = fmaxf(a.m, group_reduce(b, 64, larger));
         const float d = fminf(m - a.m, kLargest), f = __builtin_amdgcn_exp2f(d * -kLog2e);
@@ -358,8 +366,9 @@ template <typename E, int T, bool SPLIT>
 __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
     constexpr int N = Chunk<E>::N, W = T / 64, U = 16 / N;      // U chunks = 16 values per lane and step
     __shared__ Sums wave_sums[W];
-    __shared__ uint32_t wave_bound[W], found, holding;
+    __shared__ uint32_t wave_bound[W], found, holding, single;
     __shared__ uint16_t holders[T];
+    __shared__ int steps[T];
     __shared__ uint2 cand[kCandidates];
     __shared__ uint2 wave_pick[W];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -383,7 +392,7 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
     const int tail = !SPLIT || split == p.splits - 1 ? p.vocab - chunks * N : 0;
 
     Sums a = {kLowest, 0.f, 0.f};
-    float top = -INFINITY;
+    Tops top = {-INFINITY, -INFINITY, hi};
     int base = lo;
     for (; base + U * T <= hi; base += U * T) {
         float z[16];
@@ -394,7 +403,7 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
 #pragma unroll
             for (int e = 0; e < N; ++e) z[u * N + e] = some[e];
         }
-        add_values(a, top, z);
+        add_values(a, top, base, z);
     }
     for (; base < hi; base += T) {
         float some[N];
@@ -404,22 +413,22 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
 #pragma unroll
             for (int e = 0; e < N; ++e) some[e] = -INFINITY;
         }
-        add_values(a, top, some);
+        add_values(a, top, base, some);
     }
     if (tail) {                                                 // uniform
         const float last[1] = {tid < tail ? Chunk<E>::one(row + (int64_t)chunks * N + tid) : -INFINITY};
-        add_values(a, top, last);
+        add_values(a, top, hi, last);                       // no chunk: offered below by itself
     }
     a.s = group_reduce(a.s, 64, sum_of);
     a.t = group_reduce(a.t, 64, sum_of);
     // A bound that at least `top` values reach: the least over the waves of each wave's ceil(top / W)-th largest lane.
-    const uint32_t mine = ordered(top);
+    const uint32_t mine = ordered(top.first);
     const uint32_t reach = p.top > 0 ? wave_nth_largest(mine, (p.top + W - 1) / W) : 0;
     if (lane == 0) {
         wave_sums[wave] = a;
         wave_bound[wave] = reach;
     }
-    if (tid == 0) found = holding = 0;
+    if (tid == 0) found = holding = single = 0;
     __syncthreads();
     a = wave_sums[0];
     uint32_t bound = wave_bound[0];
@@ -456,8 +465,10 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
         if (tid < p.top) emit_none(tid);
         return;
     }
-    // Every value at or above the bound becomes a candidate.  Only lanes whose own largest reaches it hold any; their shares
-    // (`each` chunks, T apart) are read again by the whole work-group, a chunk per thread, so that it costs one latency.
+    // Every value at or above the bound becomes a candidate.  Only lanes whose own largest reaches it hold any, and as a rule in
+    // one step only: that step's U chunks are read again; where a second step reaches the bound too, all of the lane's (`each`
+    // chunks, T apart).  The whole work-group reads, a chunk per thread, so that it costs one latency.  (Reading all chunks of every
+    // such lane touches nearly every line of a row a second time: 8192 x 32000 with 20 alternatives 131 us, this way 112.)
     auto offer = [&](float z, uint32_t index) {
         const uint32_t u = ordered(z);
         if (u >= bound) {
@@ -465,12 +476,20 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
             if (at < kCandidates) cand[at] = make_uint2(u, index);
         }
     };
-    if (mine >= bound) holders[atomicAdd(&holding, 1u)] = (uint16_t)tid;
+    if (mine >= bound) {
+        if (ordered(top.second) >= bound) holders[atomicAdd(&holding, 1u)] = (uint16_t)tid;
+        else steps[atomicAdd(&single, 1u)] = top.where + tid;
+    }
     __syncthreads();
-    const uint32_t each = (uint32_t)(hi - lo + T - 1) / T, reads = holding * each;
+    const uint32_t ones = single * U, each = (uint32_t)(hi - lo + T - 1) / T, reads = ones + holding * each;
     for (uint32_t i = tid; i < reads; i += T) {
-        const uint32_t q = i / each;
-        const int c = lo + holders[q] + (int)(i - q * each) * T;
+        int c;
+        if (i < ones) {
+            c = steps[i / U] + (int)(i % U) * T;                // past a last, single chunk: another of the lane's, below the bound
+        } else {
+            const uint32_t q = (i - ones) / each;
+            c = lo + holders[q] + (int)(i - ones - q * each) * T;
+        }
         if (c < hi) {
             float some[N];
             Chunk<E>::load(row + (int64_t)c * N, some);

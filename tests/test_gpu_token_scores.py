@@ -244,3 +244,26 @@ def test_streams_and_repeated_graph_replays():
             for _, out in graphs:
                 assert all(torch.equal(x, y) for x, y in zip(out, want[rep & 1]))
             assert all(torch.equal(x, y) for x, y in zip(eager, want[1]))
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 50257), (3, 33001), (800, 20011), (2, 131075), (5, 2049)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_likeliest_wherever_they_lie(rows, vocab, dtype):
+    """The likeliest values next to each other, at strides that meet in one thread's share (in one step and in several), in the
+    last chunks and behind them: every one is found, once."""
+    strides = [1, 4, 8, 1024, 2048, 4096, 8192, 16384, 7, vocab // 32]
+    g = torch.Generator().manual_seed(vocab)
+    for stride in strides:
+        z = torch.rand((rows, vocab), generator=g) * 2
+        places = []
+        for r in range(rows):
+            start = int(torch.randint(0, vocab, (1,), generator=g)) if r else vocab - 1 - 31 * (stride if 31 * stride < vocab else 1)
+            at = torch.unique((start + stride * torch.arange(32)) % vocab)
+            at = at[torch.randperm(at.numel(), generator=g)]
+            z[r, at] = 8.0 + torch.arange(at.numel(), 0, -1) * 0.25       # exact in bfloat16, all different
+            places.append(at)
+        s = ops.token_scores(z.to(dtype).cuda(), alternatives=32)
+        ids = s.ids.cpu()
+        for r in range(rows):
+            assert ids[r, :places[r].numel()].tolist() == places[r].tolist(), (stride, r)
+            assert ids[r].unique().numel() == 32
