@@ -613,8 +613,8 @@ __global__ __launch_bounds__(64) void token_scores_join_kernel(const Args p) {
 }
 
 // Work-groups per row.  Cutting a row costs a second launch (some 4 us), which pays for few and very long rows only: parts of
-// 8192 tokens (one row of 131072: 9.7 against 14.7 us, 64 rows 14.3
-// against 18.0; one row of 32000: 9.1 against 7.6, 200 rows of 131072 bf16 21.9 against 20.9).
+// 8192 tokens (one row of 131072: 9.7 against 14.7 us, 64 rows 14.3 against 18.0; one row of 32000: 9.1 against 7.6, 200 rows of
+// 131072 bf16 21.9 against 20.9).
 static int splits_for(int64_t rows, int64_t vocab) {
     if (vocab <= 65536 || rows > 128) return 1;
     int64_t s = (vocab + 8191) / 8192;
@@ -643,10 +643,12 @@ static void launch(const Args& p, hipStream_t st) {
         hipLaunchKernelGGL((token_scores_long_kernel<E, 256, true>), dim3((unsigned)(p.rows * p.splits)), dim3(256), 0, st, p);
         hipLaunchKernelGGL((token_scores_join_kernel<E>), dim3((unsigned)p.rows), dim3(64), 0, st, p);
     } else {
-        // Few rows: wider work-groups keep the chip busier (256 x 32000: 8.5 against 10.0 us); many: narrower ones interleave
-        // better (8192 x 32000: 118 us with 256 threads, 138 with 512)
+        // Few long rows: wider work-groups keep the chip busier (1 x 65536 float32: 9.6 against 12.0 us, 256 x 50257 float32: 14.5 against
+        // 18.3).  Many or shorter ones: narrower work-groups interleave better and have fewer lanes to rank (8192 x 32000: 104 us
+        // with 256 threads, 134 with 512; 513 x 50257 float32: 21.4 and 23.4; 400 x 10000: 7.2 and 8.5).
         const dim3 grid((unsigned)p.rows);
-        if (p.rows < 768) hipLaunchKernelGGL((token_scores_long_kernel<E, 512, false>), grid, dim3(512), 0, st, p);
+        const bool wide = p.rows <= 400 && (int64_t)p.vocab * (int64_t)sizeof(E) >= 61440;
+        if (wide) hipLaunchKernelGGL((token_scores_long_kernel<E, 512, false>), grid, dim3(512), 0, st, p);
         else hipLaunchKernelGGL((token_scores_long_kernel<E, 256, false>), grid, dim3(256), 0, st, p);
     }
 }
