@@ -66,7 +66,7 @@ def check(r, z, tokens, k):
 
 SIZES = [(1, 1, 1), (3, 2, 4), (5, 31, 5), (9, 32, 4), (17, 33, 32), (130, 100, 8), (7, 255, 3), (6, 256, 32), (5, 257, 7),
          (9, 511, 1), (4, 1000, 20), (3, 1024, 32), (3, 1025, 32), (5, 1030, 5), (70, 2000, 8), (5, 2047, 20), (4, 2048, 32), (3, 2049, 7), (33, 700, 3), (2, 4095, 9), (300, 5001, 8), (1, 8192, 32),
-         (2, 16391, 20), (40, 32000, 5), (1, 50257, 20), (257, 20011, 32), (1, 131072, 8), (3, 200003, 20), (64, 70000, 0), (5, 65537, 9), (128, 66000, 3), (2, 600001, 32)]
+         (2, 16391, 20), (40, 32000, 5), (1, 50257, 20), (257, 20011, 32), (1, 131072, 8), (3, 200003, 20), (64, 70000, 0), (5, 65537, 9), (128, 66000, 3), (2, 600001, 32), (4100, 2111, 32), (4200, 9000, 5), (1030, 9001, 20), (401, 31000, 8), (600, 4999, 12)]
 
 
 @pytest.mark.parametrize("rows,vocab,k", SIZES)
@@ -246,7 +246,7 @@ def test_streams_and_repeated_graph_replays():
             assert all(torch.equal(x, y) for x, y in zip(eager, want[1]))
 
 
-@pytest.mark.parametrize("rows,vocab", [(3, 50257), (3, 33001), (800, 20011), (2, 131075), (5, 2049)])
+@pytest.mark.parametrize("rows,vocab", [(3, 50257), (3, 33001), (800, 20011), (2, 131075), (5, 2049), (4100, 2111), (1030, 9001), (401, 20000)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_likeliest_wherever_they_lie(rows, vocab, dtype):
     """The likeliest values next to each other, at strides that meet in one thread's share (in one step and in several), in the
@@ -267,3 +267,22 @@ def test_likeliest_wherever_they_lie(rows, vocab, dtype):
         for r in range(rows):
             assert ids[r, :places[r].numel()].tolist() == places[r].tolist(), (stride, r)
             assert ids[r].unique().numel() == 32
+
+
+@pytest.mark.parametrize("vocab", [2049, 2500, 9001])
+def test_special_rows_among_many(vocab):
+    """The special rows within thousands of others: each row's results depend on that row alone."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    z = torch.randn((4111, vocab), generator=g, device="cuda") * 3
+    z[5] = -INF
+    z[6] = -INF
+    z[6, vocab - 1] = 2.0
+    z[7] = torch.finfo(torch.float32).min
+    z[8, 0], z[9, vocab // 2], z[10, vocab - 1] = math.nan, INF, -INF
+    z[11] = 1.5
+    z[12, ::2] = -INF
+    z[13, vocab - 1] = 90.0
+    tokens = torch.randint(0, vocab, (4111, 1), generator=g, device="cuda", dtype=torch.int32)
+    at = torch.cat([torch.arange(0, 20), torch.tensor([4096, 4110])])
+    many = ops.token_scores(z, tokens, alternatives=32)
+    check(ops.TokenScores(*(v[at.cuda()] for v in many)), z[at.cuda()], tokens[at.cuda()], 32)
