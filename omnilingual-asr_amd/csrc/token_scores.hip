@@ -10,7 +10,7 @@
 // Ties go to the lower index: candidates are ranked by (value, index), never by the order in which they were found.
 //
 // Bandwidth-bound for rows that number in the hundreds (2 or 4 bytes per logit against about ten issue slots), bound by
-// latency below.  Rows up to 2048 tokens stay in the registers of a group of lanes; longer ones are streamed by a
+// latency below.  Rows up to 1024 tokens stay in the registers of a group of lanes; longer ones are streamed by a
 // work-group each, or by several where rows are few, whose results a second launch joins.
 #include "oasr_common.h"
 
@@ -22,7 +22,7 @@ constexpr float kLargest = 3.402823466e38f;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxTop = 32;
 constexpr int kMaxSplits = 64;
-constexpr int kShort = 2048;                      // tokens that a wave holds in registers
+constexpr int kShort = 1024;                      // tokens that a wave holds in registers
 constexpr int kCandidates = 512;                  // kept in LDS per row before ranking
 
 struct Args {
@@ -637,8 +637,7 @@ static void launch(const Args& p, hipStream_t st) {
         const dim3 grid((unsigned)((p.rows + per_wg - 1) / per_wg)), blk(256);
         if (p.vocab <= 256) hipLaunchKernelGGL((token_scores_short_kernel<E, 1>), grid, blk, 0, st, p, g);
         else if (p.vocab <= 512) hipLaunchKernelGGL((token_scores_short_kernel<E, 2>), grid, blk, 0, st, p, g);
-        else if (p.vocab <= 1024) hipLaunchKernelGGL((token_scores_short_kernel<E, 4>), grid, blk, 0, st, p, g);
-        else hipLaunchKernelGGL((token_scores_short_kernel<E, 8>), grid, blk, 0, st, p, g);
+        else hipLaunchKernelGGL((token_scores_short_kernel<E, 4>), grid, blk, 0, st, p, g);     // (eight: 20000 x 2000 bf16 41 us, streamed 25)
     } else if (p.splits > 1) {
         hipLaunchKernelGGL((token_scores_long_kernel<E, 256, true>), dim3((unsigned)(p.rows * p.splits)), dim3(256), 0, st, p);
         hipLaunchKernelGGL((token_scores_join_kernel<E>), dim3((unsigned)p.rows), dim3(64), 0, st, p);
