@@ -291,33 +291,29 @@ __global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, i
         }
         return;
     }
-    uint32_t least = kOrderedLowest;
-    {
-        // a whole wave per row: the values that reach the top-th largest of the lanes' own largest go to a list, and are
-        // ranked there; a list that overflows (ties) is left, and the rounds below take its place
-        const uint32_t bound = max(wave_nth_largest(ordered(own), p.top), kOrderedLowest);
-        int n = 0;
+    // a whole wave per row: the values that reach the top-th largest of the lanes' own largest go to a list, and are
+    // ranked there; a list that overflows (ties) is left, and the rounds below take its place
+    const uint32_t bound = max(wave_nth_largest(ordered(own), p.top), kOrderedLowest);
+    int n = 0;
 #pragma unroll
-        for (int j = 0; j < 4 * C; ++j) {
-            const uint32_t u = ordered(z[j]);
-            const uint64_t hits = __ballot(usable && u >= bound);
-            const int at = n + __popcll(hits & ((1ull << lane) - 1));
-            if ((hits >> lane & 1) && at < kList) lists[wave_in][at] = {u, (uint32_t)(4 * (sub + (j >> 2) * group) + (j & 3))};
-            n += __popcll(hits);
+    for (int j = 0; j < 4 * C; ++j) {
+        const uint32_t u = ordered(z[j]);
+        const uint64_t hits = __ballot(usable && u >= bound);
+        const int at = n + __popcll(hits & ((1ull << lane) - 1));
+        if ((hits >> lane & 1) && at < kList) lists[wave_in][at] = {u, (uint32_t)(4 * (sub + (j >> 2) * group) + (j & 3))};
+        n += __popcll(hits);
+    }
+    if (n <= kList) {
+        OASR_SCORES_WAVE_LDS();
+        if (!live) return;
+        if (lane < n) {
+            const Pick me = lists[wave_in][lane];
+            int rank = 0;
+            for (int o = 0; o < n; ++o) rank += before(lists[wave_in][o].value, lists[wave_in][o].index, me.value, me.index);
+            if (rank < p.top) write_best(p, r, rank, me.value, me.index, m, log_s);
         }
-        if (n <= kList) {
-            OASR_SCORES_WAVE_LDS();
-            if (!live) return;
-            if (lane < n) {
-                const Pick me = lists[wave_in][lane];
-                int rank = 0;
-                for (int o = 0; o < n; ++o) rank += before(lists[wave_in][o].value, lists[wave_in][o].index, me.value, me.index);
-                if (rank < p.top) write_best(p, r, rank, me.value, me.index, m, log_s);
-            }
-            if (lane >= n && lane < p.top) write_none(p, r, lane, absent);
-            return;
-        }
-        least = bound;
+        if (lane >= n && lane < p.top) write_none(p, r, lane, absent);
+        return;
     }
     uint32_t taken = 0;                               // this lane's values that are out already
     for (int k = 0; k < p.top; ++k) {
@@ -325,7 +321,7 @@ __global__ __launch_bounds__(256) void token_scores_short_kernel(const Args p, i
 #pragma unroll
         for (int j = 0; j < 4 * C; ++j) {
             const uint32_t u = ordered(z[j]), at = 4 * (sub + (j >> 2) * group) + (j & 3);
-            if (!(taken >> j & 1) && u >= least) best = better(best, {u, at});
+            if (!(taken >> j & 1) && u >= bound) best = better(best, {u, at});
         }
         best = group_reduce(best, group, better);
 #pragma unroll
