@@ -663,14 +663,16 @@ static void launch(const Args& p, hipStream_t st) {
         hipLaunchKernelGGL((token_scores_long_kernel<E, 256, true>), dim3((unsigned)(p.rows * p.splits)), dim3(256), 0, st, p);
         hipLaunchKernelGGL((token_scores_join_kernel<E>), dim3((unsigned)p.rows), dim3(64), 0, st, p);
     } else {
-        // Few long rows: wider work-groups keep the chip busier (1 x 65536 float32: 512 threads 9.6 us, 256 threads 12.0; 256 x 50257
-        // float32: 14.5 and 18.3).  Many or shorter ones: narrower work-groups interleave better and have fewer lanes to rank
-        // (8192 x 32000: 512 threads 134 us, 256 threads 104; 16000 x 5000 bf16: 256 threads 54, 128 threads 38, one wave 34;
-        // 1024 x 4000 float32: 7.7, 7.1 and 7.4; 1024 x 20000 bf16: 13.8, 14.1 and 18.0).
+        // Few long rows: wider work-groups keep the chip busier (256 x 65536 bf16: 512 threads 14.7 us, 256 threads 18.9; 400 x 50257
+        // float32: 20.8 and 24.5; but 513 x 50257 bf16: 21.4 and 20.6).  Many or shorter ones: narrower work-groups interleave better
+        // and have fewer lanes to rank (8192 x 32000 bf16: 512 threads 131 us, 256 threads 103; 16000 x 5000: 256 threads 61,
+        // 128 threads 45, one wave 41; 2048 x 5000: 13.7, 10.6 and 11.1; 1024 x 32000: 19.6, 22.7 and 33.3).  Rows from memory, not
+        // from a cache that an earlier call filled.
         const dim3 grid((unsigned)p.rows);
         const int64_t bytes = (int64_t)p.vocab * (int64_t)sizeof(E);
         const bool brief = p.vocab <= 10240;
-        if (p.rows <= 400 && bytes >= 61440) hipLaunchKernelGGL((token_scores_long_kernel<E, 512, false>), grid, dim3(512), 0, st, p);
+        const bool wide = (p.rows <= 400 && bytes >= 61440) || (p.rows <= 640 && bytes >= 131072);
+        if (wide) hipLaunchKernelGGL((token_scores_long_kernel<E, 512, false>), grid, dim3(512), 0, st, p);
         else if (brief && p.rows >= 4096) hipLaunchKernelGGL((token_scores_long_kernel<E, 64, false>), grid, dim3(64), 0, st, p);
         else if (p.vocab <= 5120 || (brief && p.rows >= 1024)) hipLaunchKernelGGL((token_scores_long_kernel<E, 128, false>), grid, dim3(128), 0, st, p);
         else hipLaunchKernelGGL((token_scores_long_kernel<E, 256, false>), grid, dim3(256), 0, st, p);
