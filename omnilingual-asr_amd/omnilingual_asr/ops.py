@@ -78,9 +78,10 @@ class LinearI8:
 
     `epilogue`: "bias" -> bf16, "swish" -> bf16, "glu" -> bf16 of half the width (rows of W interleaved as
     `weights.glu_interleave` does, a multiple of 32), "float" -> float32, "residual" -> resid + alpha * (...) in float32.
-    Forward only: results carry no gradient.  The weights are packed on the stream that is current when the object is made; a
-    call on another stream has to wait for that one, as for any tensor made there.  The packed weights belong to the object
-    and must not be in use by another stream when it is dropped."""
+    Forward only: results carry no gradient.  The layer owns what it reads: the weights are packed and scale and bias copied on
+    the stream that is current when the object is made, so a module they came from may be moved, changed or dropped afterwards.
+    A call on another stream has to wait for that one, as for any tensor made there, and the object must not be in use by
+    another stream when it is dropped.  `scale`, `bias` and `packed` give the layer's own memory and cannot be assigned."""
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None):
         """`weight`: float [out, in] on a HIP device; quantised per output row."""
@@ -104,13 +105,31 @@ class LinearI8:
         if n < 1 or not 1 <= k <= 131072:
             raise ValueError("a weight has at least one row and 1 to 131072 columns")
         self.device, self.out_features, self.in_features = codes.device, n, k
-        self._scale_ptr, self._bias_ptr = _vector(scale, n, "scale", codes.device), _vector(bias, n, "bias", codes.device)
+        _vector(scale, n, "scale", codes.device), _vector(bias, n, "bias", codes.device)
         if scale is None:
             raise ValueError("scale must be given")
-        self.scale, self.bias = scale, bias
-        self.packed = codes.new_empty((int(_hip.lib().oasr_gemm_i8_packed_bytes(n, k)),))
-        _call("oasr_gemm_pack_w_i8", self.device, codes.data_ptr(), ldw, n, k, self.packed.data_ptr())
-        self._packed_ptr = self.packed.data_ptr()
+        packed = codes.new_empty((int(_hip.lib().oasr_gemm_i8_packed_bytes(n, k)),))
+        _call("oasr_gemm_pack_w_i8", self.device, codes.data_ptr(), ldw, n, k, packed.data_ptr())
+        self._own(packed, scale.detach().clone(), None if bias is None else bias.detach().clone())
+
+    def _own(self, packed, scale, bias):
+        """The layer's own buffers and their addresses, which hold as long as nobody else can replace a buffer's storage: a
+        Parameter's is replaced in place by Module.to() and the like, the tensor object staying the same."""
+        self._packed, self._scale, self._bias = packed, scale, bias
+        self._packed_ptr, self._scale_ptr = packed.data_ptr(), scale.data_ptr()
+        self._bias_ptr = None if bias is None else bias.data_ptr()
+
+    @property
+    def packed(self) -> torch.Tensor:
+        return self._packed.detach()
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self._scale.detach()
+
+    @property
+    def bias(self) -> torch.Tensor | None:
+        return None if self._bias is None else self._bias.detach()
 
     def _output(self, x, epilogue, resid, out):
         """(epilogue code, output, its row pitch, residual's pointer, its row pitch) for input x."""

@@ -464,3 +464,18 @@ def test_every_tile_is_computed_once(m, n, k):
     layer(a.cuda(), epilogue="float", out=out)
     want = a.cuda().float() @ codes.cuda().float().t()  # below 2^24: exact in float32
     assert (want.abs() < 2 ** 24).all() and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("change", [lambda lin: lin.cpu(), lambda lin: lin.double(), lambda lin: lin.half(), lambda lin: lin.bias.data.fill_(9.0)],
+                         ids=["cpu", "double", "half", "in place"])
+def test_layer_outlives_changes_of_the_module_it_came_from(change):
+    """The module leaves the device or changes its type after quantisation, what it freed is allocated again and overwritten:
+    the layer's results stay."""
+    lin = torch.nn.Linear(512, 4096, device="cuda")
+    layer = ops.LinearI8(lin.weight, lin.bias)
+    x = torch.randn((5, 512), device="cuda").to(torch.bfloat16)
+    want = layer(x)
+    torch.cuda.synchronize()
+    change(lin)
+    over = [torch.full((4096,), float("nan"), device="cuda") for _ in range(64)]
+    assert torch.equal(layer(x), want) and len(over) == 64

@@ -140,3 +140,51 @@ def test_encoder_takes_one_kind_of_8_bit_weights():
         assert L.oasr_encoder_set_int8(handle, (_hip.LayerInt8Weights * 1)(_hip.LayerInt8Weights(**full))) == -1
     finally:
         L.oasr_encoder_destroy(handle)
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """Layers on host tensors: what a call would hand to the library, as (name, arguments), instead of the call."""
+    calls = []
+    monkeypatch.setattr(ops, "_rows", lambda t, what, dtypes: (t, t.numel() // t.shape[-1], t.shape[-1], t.shape[-1]))
+    monkeypatch.setattr(ops, "_call", lambda name, device, *args: calls.append((name, args)))
+    return calls
+
+
+def _handed_over(layer, calls):
+    """The addresses of weights, scale and bias that a call on `layer` passes."""
+    del calls[:]
+    layer(torch.zeros((1, layer.in_features), dtype=torch.bfloat16))
+    (name, args), = calls
+    assert name == "oasr_linear_i8"
+    return args[2:5]
+
+
+def test_layer_reads_its_own_memory_when_a_module_moves(recorded):
+    """Module.to() and the like put new storage under the same Parameter object and free the old one: a layer made from a
+    module's Parameters reads memory of its own, whatever happens to them."""
+    lin = torch.nn.Linear(64, 32)
+    layer = ops.LinearI8(lin.weight, lin.bias)
+    scale = torch.rand(32)
+    other = ops.LinearI8.from_codes(torch.ones((32, 64), dtype=torch.int8), scale, lin.bias)
+    kept = lin.bias.detach().clone()
+    before = _handed_over(layer, recorded)
+    foreign = {lin.bias.data_ptr(), scale.data_ptr()}
+    lin.double()
+    for it in (layer, other):
+        own = _handed_over(it, recorded)
+        assert own == (it.packed.data_ptr(), it.scale.data_ptr(), it.bias.data_ptr())
+        assert not foreign & set(own) and lin.bias.data_ptr() not in own
+        assert torch.equal(it.bias, kept) and it.bias.dtype == torch.float32 and not it.bias.requires_grad
+    assert _handed_over(layer, recorded) == before and torch.equal(other.scale, scale)
+
+
+@pytest.mark.parametrize("name", ["scale", "bias", "packed"])
+def test_buffers_of_a_layer_cannot_be_assigned(recorded, name):
+    """An assigned tensor would not be what the kernels read."""
+    layer = ops.LinearI8(torch.ones((32, 64)), torch.ones(32))
+    before = _handed_over(layer, recorded)
+    with pytest.raises(AttributeError):
+        setattr(layer, name, torch.zeros(32))
+    getattr(layer, name).data = torch.zeros(32)          # of the alias: the layer keeps its own
+    assert _handed_over(layer, recorded) == before == (layer.packed.data_ptr(), layer.scale.data_ptr(), layer.bias.data_ptr())
