@@ -81,7 +81,8 @@ class LinearI8:
     Forward only: results carry no gradient.  The layer owns what it reads: the weights are packed and scale and bias copied on
     the stream that is current when the object is made, so a module they came from may be moved, changed or dropped afterwards.
     A call on another stream has to wait for that one, as for any tensor made there, and the object must not be in use by
-    another stream when it is dropped.  `scale`, `bias` and `packed` give the layer's own memory and cannot be assigned."""
+    another stream when it is dropped.  `scale`, `bias` and `packed` give the layer's own memory and cannot be assigned.
+    A layer can be copied (copy.deepcopy) and pickled; it has to be on a HIP device when it is loaded."""
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None):
         """`weight`: float [out, in] on a HIP device; quantised per output row."""
@@ -118,6 +119,19 @@ class LinearI8:
         self._packed, self._scale, self._bias = packed, scale, bias
         self._packed_ptr, self._scale_ptr = packed.data_ptr(), scale.data_ptr()
         self._bias_ptr = None if bias is None else bias.data_ptr()
+
+    def __getstate__(self):
+        return {"packed": self._packed, "scale": self._scale, "bias": self._bias, "shape": (self.out_features, self.in_features)}
+
+    def __setstate__(self, state):
+        """A copy or an unpickled layer reads its own buffers, on the device on which they are now."""
+        (n, k), packed, scale, bias = state["shape"], state["packed"], state["scale"], state["bias"]
+        _rows(packed, "packed weights", _INT8)
+        if packed.shape != (int(_hip.lib().oasr_gemm_i8_packed_bytes(n, k)),):
+            raise ValueError(f"packed weights are not those of a layer [{n}, {k}]")
+        self.device, self.out_features, self.in_features = packed.device, n, k
+        _vector(scale, n, "scale", packed.device), _vector(bias, n, "bias", packed.device)
+        self._own(packed, scale, bias)
 
     @property
     def packed(self) -> torch.Tensor:

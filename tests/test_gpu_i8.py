@@ -479,3 +479,20 @@ def test_layer_outlives_changes_of_the_module_it_came_from(change):
     change(lin)
     over = [torch.full((4096,), float("nan"), device="cuda") for _ in range(64)]
     assert torch.equal(layer(x), want) and len(over) == 64
+
+
+def test_copied_and_saved_layers():
+    """A deep copy and a saved layer give the layer's bits after the original is gone and its memory overwritten."""
+    import copy
+    import io
+    g = torch.Generator(device="cuda").manual_seed(12)
+    layer = ops.LinearI8(torch.randn((700, 900), generator=g, device="cuda"), torch.randn((700,), generator=g, device="cuda"))
+    x = torch.randn((40, 900), generator=g, device="cuda").to(torch.bfloat16)
+    want, file = layer(x), io.BytesIO()
+    torch.save(layer, file)
+    again = copy.deepcopy(layer)
+    layer._packed.zero_(), layer._scale.zero_(), layer._bias.zero_()
+    del layer
+    file.seek(0)
+    for it in (again, torch.load(file, weights_only=False)):
+        assert torch.equal(it(x), want)

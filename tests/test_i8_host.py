@@ -188,3 +188,33 @@ def test_buffers_of_a_layer_cannot_be_assigned(recorded, name):
         setattr(layer, name, torch.zeros(32))
     getattr(layer, name).data = torch.zeros(32)          # of the alias: the layer keeps its own
     assert _handed_over(layer, recorded) == before == (layer.packed.data_ptr(), layer.scale.data_ptr(), layer.bias.data_ptr())
+
+
+@pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle"])
+def test_copies_of_a_layer_read_their_own_memory(recorded, how):
+    """A copy passes the addresses of its own buffers, not those of the layer that it was made from."""
+    import copy
+    import pickle
+    again = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda t: pickle.loads(pickle.dumps(t))}[how]
+    for bias in (torch.rand(32), None):
+        layer = ops.LinearI8(torch.rand((32, 64)), bias)
+        layer._packed.copy_(torch.arange(2048) % 127)
+        it = again(layer)
+        got, mine = _handed_over(it, recorded), _handed_over(layer, recorded)
+        assert got == (it.packed.data_ptr(), it.scale.data_ptr(), None if bias is None else it.bias.data_ptr())
+        assert (got == mine) == (how == "copy")
+        assert torch.equal(it.packed, layer.packed) and torch.equal(it.scale, layer.scale)
+        assert (it.device, it.out_features, it.in_features) == (layer.device, 32, 64)
+
+
+def test_a_loaded_layer_has_to_be_on_a_device_and_whole(monkeypatch, recorded):
+    import pickle
+    layer = ops.LinearI8(torch.rand((32, 64)), torch.rand(32))
+    state = layer.__getstate__()
+    for change in (dict(shape=(32, 65)), dict(shape=(33, 64)), dict(scale=state["scale"][:31]), dict(bias=state["bias"].double())):
+        with pytest.raises(ValueError):
+            ops.LinearI8.__new__(ops.LinearI8).__setstate__({**state, **change})
+    saved = pickle.dumps(layer)
+    monkeypatch.undo()                                   # host tensors again, as loading onto the host makes them
+    with pytest.raises(ValueError, match="HIP device"):
+        pickle.loads(saved)
