@@ -423,7 +423,8 @@ int64_t oasr_gemm_i8_packed_bytes(int64_t n, int64_t k);
 int oasr_gemm_pack_w_i8(const int8_t* w, int64_t ldw, int64_t n, int64_t k, int8_t* out, void* stream);
 
 /* C[m][n] = epilogue(scale_a[m] * scale_w[n] * sum_k A8[m][k] * W8[n][k]): sums in 32-bit integers, exact (k <= 131072).
- * Any m (0: nothing is done), n, k (a result past some 2^30 x 64 elements is refused); epilogues of oasr_epilogue, bias float32[n] or NULL with each of them
+ * Any m (0: nothing is done) and n below 2^31 with fewer than 2^30 tiles of 256 x 256 (lda of 2^26 and more: fewer than
+ * 7 * 2^20 tiles of 128 x 128), any k up to 131072; epilogues of oasr_epilogue, bias float32[n] or NULL with each of them
  * (OASR_EPI_GLU_BF16: n a multiple of 32, bias interleaved as the rows are, C of n / 2 columns).
  * a: rows `lda` apart as oasr_quant_i8_rows writes them - 16-byte aligned, lda a multiple of 16 and at least k rounded up to
  * 64, zeros from k up to there.  c, resid: rows `ldc`, `ldr` elements apart; resid may be c (with ldr = ldc), apart from
@@ -435,7 +436,7 @@ int oasr_gemm_i8(const int8_t* a, int64_t lda, const int8_t* w_packed, const flo
 /* Both steps: the bf16 rows x (ldx apart) are quantised and multiplied.  The same bits as oasr_quant_i8_rows followed by
  * oasr_gemm_i8.  workspace: device, oasr_linear_i8_workspace_bytes(m, n, k) (0 for a few rows, which are quantised
  * inside the product), 256-byte aligned, contents on entry do not matter; calls that may overlap need one each.
- * m below 2^24. */
+ * m below 2^24; n as for oasr_gemm_i8, but below 7 * 2^25 - 31 where the workspace is 0. */
 int64_t oasr_linear_i8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int oasr_linear_i8(const uint16_t* x, int64_t ldx, const int8_t* w_packed, const float* scale_w, const float* bias,
                    const float* resid, int64_t ldr, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, float alpha,

@@ -941,6 +941,7 @@ static int choose_form(const GemmArgs& p) {
     for (int f = 0; f < kForms; ++f) {
         const Form& t = kFormTable[f];
         const int64_t groups = ((p.m + t.bm - 1) / t.bm) * ((p.n + t.bn - 1) / t.bn);
+        if (groups >= (f == kTile256 ? kMaxWideTiles : kMaxGroups)) continue;       // more than a launch has: a form of larger tiles
         if (f == kSplit16 && p.m > 16 && groups > 128) continue;
         if (f == kTile256 && p.lda >= (1 << 26)) continue;       // 32 row pitches have to fit its 32-bit offsets
         const double rounds = (double)((groups + 255) / 256) * t.share;

@@ -496,3 +496,20 @@ def test_copied_and_saved_layers():
     file.seek(0)
     for it in (again, torch.load(file, weights_only=False)):
         assert torch.equal(it(x), want)
+
+
+def test_more_columns_than_a_launch_has_tiles_of_64():
+    """A few rows by so many columns that the forms of 64 columns would need more threads than a launch has: a form of larger
+    tiles takes them.  Every output is checked (a power of two as scale: exact)."""
+    n, m = (7 << 26) + 70, 3
+    codes = torch.randint(-128, 128, (n, 1), dtype=torch.int8, device="cuda")
+    layer = ops.LinearI8.from_codes(codes, torch.full((n,), 0.5, device="cuda"))
+    a = torch.zeros((m, 64), dtype=torch.int8, device="cuda")
+    a[:, 0] = torch.tensor([1, -127, 3])
+    sa, out = torch.tensor([1.0, 2.0, 0.25], device="cuda"), torch.full((m, n), float("nan"), device="cuda")
+    H.check(H.lib().oasr_gemm_i8(a.data_ptr(), 64, layer.packed.data_ptr(), sa.data_ptr(), layer.scale.data_ptr(), None, None, 0,
+                                 out.data_ptr(), n, m, n, 1, 1.0, H.EPI_BIAS_F32, H.current_stream_ptr()))
+    for r in range(m):
+        assert torch.equal(out[r], codes[:, 0].float() * float(a[r, 0]) * float(sa[r]) * 0.5)
+    del layer, out, codes
+    torch.cuda.empty_cache()
