@@ -235,9 +235,13 @@ def _int32(t, shape, what: str, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _score_outputs(lead, given, alternatives, like):
+def _score_outputs(lead, given, alternatives, like, rows, vocab, n):
+    """The outputs of `rows` rows with `n` given tokens each, after the checks of sizes (the C call takes vocab, n and a batch as
+    32-bit integers)."""
     if not 0 <= alternatives <= MAX_ALTERNATIVES:
         raise ValueError(f"alternatives must lie in [0, {MAX_ALTERNATIVES}]")
+    if rows >= 1 << 24 or vocab >= 1 << 30 or n >= 1 << 31:
+        raise ValueError("token scores take fewer than 2^24 rows, 2^30 columns and 2^31 given tokens a row")
     new, f32, listed = like.new_empty, torch.float32, (*lead, alternatives)
     return TokenScores(new(given, dtype=f32), new(lead, dtype=f32), new(listed, dtype=torch.int32), new(listed, dtype=f32))
 
@@ -263,7 +267,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, al
         if given != lead and given[:-1] != lead:
             raise ValueError(f"tokens must be of shape {tuple(lead)} or {tuple(lead)} and one more dimension")
         tokens, n = _int32(tokens, given, "tokens", device), 1 if given == lead else given[-1]
-    out = _score_outputs(lead, given, alternatives, logits)
+    out = _score_outputs(lead, given, alternatives, logits, rows, vocab, n)
     if rows == 0:
         return out
     return _score("oasr_token_scores", z, (ld, rows, vocab, None if tokens is None else tokens.data_ptr(), n), out, rows, vocab,
@@ -288,7 +292,7 @@ def ctc_token_scores(logits: torch.Tensor, tokens: torch.Tensor, frames: torch.T
     tokens, frames = _int32(tokens, shape, "tokens", device), _int32(frames, shape, "frames", device)
     if t_pad == 0 and tokens.numel():
         raise ValueError("logits have no frames")
-    out = _score_outputs(shape, shape, alternatives, logits)
+    out = _score_outputs(shape, shape, alternatives, logits, tokens.numel(), vocab, 1)
     if tokens.numel() == 0:
         return out
     return _score("oasr_ctc_token_scores", logits, (ld, vocab, batch, t_pad, tokens.data_ptr(), frames.data_ptr(), shape[1]), out,

@@ -60,3 +60,23 @@ def test_tensor_refusals_without_a_device():
         ops.token_scores(z.half())
     with pytest.raises(ValueError, match="contiguous tensor"):
         ops.ctc_token_scores(z, torch.zeros((3, 4), dtype=torch.int32), torch.zeros((3, 4), dtype=torch.int32))
+
+
+def test_sizes_past_the_calls_32_bits_are_refused(monkeypatch):
+    """A vocabulary or a batch past 2^32 must not reach the library as its low 32 bits (shapes alone: no memory behind them)."""
+    monkeypatch.setattr(ops, "_rows", lambda t, what, dtypes: (t, t.numel() // t.shape[-1], t.shape[-1], t.shape[-1]))
+    reached = []
+    monkeypatch.setattr(ops, "_call", lambda name, device, *args: reached.append((name, args)))
+    meta = lambda *shape, dtype=torch.bfloat16: torch.empty(shape, dtype=dtype, device="meta")  # noqa: E731
+    i32 = lambda *shape: meta(*shape, dtype=torch.int32)  # noqa: E731
+    for call in (lambda: ops.token_scores(meta(1, (1 << 32) + 5)), lambda: ops.token_scores(meta(2, 1 << 30)),
+                 lambda: ops.token_scores(meta(1 << 24, 3)), lambda: ops.token_scores(meta(1, 5), i32(1, (1 << 32) + 1)),
+                 lambda: ops.ctc_token_scores(meta((1 << 32) + 1, 1, 1), i32((1 << 32) + 1, 1), i32((1 << 32) + 1, 1)),
+                 lambda: ops.ctc_token_scores(meta(1, 2, (1 << 32) + 5), i32(1, 2), i32(1, 2)),
+                 lambda: ops.ctc_token_scores(meta(2, 4, 5), i32(2, 1 << 23), i32(2, 1 << 23))):
+        with pytest.raises(ValueError, match="fewer than"):
+            call()
+    assert not reached
+    ops.token_scores(meta(3, (1 << 30) - 1), i32(3, 7))
+    ops.ctc_token_scores(meta(2, 4, (1 << 32) + 5), i32(2, 3), i32(2, 3), vocab=100)      # a pitch is 64 bits wide
+    assert [name for name, _ in reached] == ["oasr_token_scores", "oasr_ctc_token_scores"]
