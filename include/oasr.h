@@ -536,7 +536,9 @@ int oasr_gather_chunks(const float* pcm, int64_t pcm_len, const int64_t* start, 
  *   logprobs[r][i] = log softmax(z)[tokens[r][i]]; a token below 0 means none (0), one at or past vocab gives NaN
  *   entropy[r]     = -sum p log p, natural units; may be NULL
  *   ids, best [r][0 .. top-1] = the likeliest tokens and their log probabilities, best first, ties to the lower index
- * float32 results, sums in float32.  A logit of -inf is a token ruled out: probability 0, never among the likeliest (id -1,
+ * float32 results, compensated sums in float32: a log probability is within 2^-17 + 2^-22 |log p|, an entropy within
+ * 2^-16 (1 + H).  (Past 2^20 tokens, a row whose values rise from its first token to its last may lose another 2^-23 per 4096
+ * tokens, since each rise of the running maximum rescales the sums.)  A logit of -inf is a token ruled out: probability 0, never among the likeliest (id -1,
  * log probability -inf where fewer than `top` remain).  A row that allows nothing: log probabilities -inf, entropy 0, no
  * likeliest.  A NaN or +inf in a row: NaN results, ids -1.  top 0 .. 32, given (tokens per row) and rows may be 0;
  * rows below 2^24, vocab below 2^30.

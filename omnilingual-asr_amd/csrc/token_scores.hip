@@ -1,7 +1,8 @@
 // Log probabilities of given tokens under rows of logits, the rows' entropies and their k likeliest tokens, one pass over
 // the logits.  For a row z with reference m (its maximum when the pass ends):
 //   S = sum exp(z - m),  T = sum exp(z - m) (m - z):   log p(t) = (z_t - m) - log S,   entropy = log S + T / S
-// (every term of T is >= 0, so the entropy loses nothing by cancellation; natural units).  S, T and m are float32.
+// (every term of T is >= 0, so the entropy loses nothing by cancellation; natural units).  S, T and m are float32; over long rows
+// S and T are summed with compensation.
 // Partial results over different references join by f = exp(m' - m): S = S + f S', T = T + f (T' + (m - m') S').
 //
 // What is masked: -inf has probability 0 and is never among the likeliest (id -1, log p -inf where fewer than k tokens
@@ -340,6 +341,18 @@ struct Sums {
     float m, s, t;
 };
 
+// A lane's running sums with what their additions rounded away (cs, ct: what the sums hold too much), so that the error of
+// a sum does not grow with the row: one of 2^26 tokens gives a lane 4096 terms, and with terms that all round the same way the plain
+// sum of 4096 is off by 2^-14.6 of itself, of 65536 by 2^-10.6.
+struct LaneSums {
+    float m, s, t, cs, ct;
+};
+__device__ __forceinline__ void add_compensated(float& sum, float& excess, float v) {
+    const float y = v - excess, next = sum + y;
+    excess = (next - sum) - y;
+    sum = next;
+}
+
 // A lane's largest value, the chunk at which the step that held it began, and the largest of its other steps.
 struct Tops {
     float first, second;
@@ -347,7 +360,7 @@ struct Tops {
 };
 
 template <int N>
-__device__ __forceinline__ void add_values(Sums& a, Tops& top, int at, const float (&z)[N]) {
+__device__ __forceinline__ void add_values(LaneSums& a, Tops& top, int at, const float (&z)[N]) {
     float b = z[0];
 #pragma unroll
     for (int j = 1; j < N; ++j) b = fmaxf(b, z[j]);
@@ -358,15 +371,21 @@ __device__ __forceinline__ void add_values(Sums& a, Tops& top, int at, const flo
         const float m = fmaxf(a.m, group_reduce(b, 64, larger));
         const float d = fminf(m - a.m, kLargest), f = __builtin_amdgcn_exp2f(d * -kLog2e);
         a.t = f > 0.f ? f * fmaf(d, a.s, a.t) : 0.f * a.s;     // NaN stays NaN
+        a.ct = f > 0.f ? f * fmaf(d, a.cs, a.ct) : 0.f;
         a.s *= f;
+        a.cs *= f;
         a.m = m;
     }
+    // the step's own sums first: sixteen terms are too few to matter, and one compensated addition per step costs little
+    float s = 0.f, t = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         const float x = a.m - z[j], e = __builtin_amdgcn_exp2f(x * -kLog2e);
-        a.s += e;
-        a.t = fmaf(e, fminf(x, kLargest), a.t);
+        s = j ? s + e : e;
+        t = j ? fmaf(e, fminf(x, kLargest), t) : e * fminf(x, kLargest);
     }
+    add_compensated(a.s, a.cs, s);
+    add_compensated(a.t, a.ct, t);
 }
 
 // Joins sums over another reference.
@@ -412,7 +431,7 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
     const int hi = SPLIT ? (int)((int64_t)chunks * (split + 1) / p.splits) : chunks;
     const int tail = !SPLIT || split == p.splits - 1 ? p.vocab - chunks * N : 0;
 
-    Sums a = {kLowest, 0.f, 0.f};
+    LaneSums own = {kLowest, 0.f, 0.f, 0.f, 0.f};
     Tops top = {-INFINITY, -INFINITY, hi};
     int base = lo;
     for (; base + U * T <= hi; base += U * T) {
@@ -424,7 +443,7 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
 #pragma unroll
             for (int e = 0; e < N; ++e) z[u * N + e] = some[e];
         }
-        add_values(a, top, base, z);
+        add_values(own, top, base, z);
     }
     for (; base < hi; base += T) {
         float some[N];
@@ -434,14 +453,13 @@ __global__ __launch_bounds__(T) void token_scores_long_kernel(const Args p) {
 #pragma unroll
             for (int e = 0; e < N; ++e) some[e] = -INFINITY;
         }
-        add_values(a, top, base, some);
+        add_values(own, top, base, some);
     }
     if (tail) {                                                 // uniform
         const float last[1] = {tid < tail ? Chunk<E>::one(row + (int64_t)chunks * N + tid) : -INFINITY};
-        add_values(a, top, hi, last);                       // no chunk: offered below by itself
+        add_values(own, top, hi, last);                       // no chunk: offered below by itself
     }
-    a.s = group_reduce(a.s, 64, sum_of);
-    a.t = group_reduce(a.t, 64, sum_of);
+    Sums a = {own.m, group_reduce(own.s - own.cs, 64, sum_of), group_reduce(own.t - own.ct, 64, sum_of)};
     // A bound that at least `top` values reach: the least over the waves of each wave's ceil(top / W)-th largest lane.
     const uint32_t mine = ordered(top.first);
     const uint32_t reach = p.top > 0 ? wave_nth_largest(mine, (p.top + W - 1) / W) : 0;

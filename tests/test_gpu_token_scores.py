@@ -286,3 +286,28 @@ def test_special_rows_among_many(vocab):
     at = torch.cat([torch.arange(0, 20), torch.tensor([4096, 4110])])
     many = ops.token_scores(z, tokens, alternatives=32)
     check(ops.TokenScores(*(v[at.cuda()] for v in many)), z[at.cuda()], tokens[at.cuda()], 32)
+
+
+@pytest.mark.parametrize("rows,vocab", [(6, 1 << 26), (140, 1 << 20), (140, 300007), (4200, 10001), (1100, 10001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_sums_of_long_rows_do_not_drift(rows, vocab, dtype):
+    """Rows of one value (z < 0) with a 0 at every 509th place (each wave then sums terms exp(z), which all round the same way):
+    S = n + (V - n) exp(z), T = (V - n) exp(z) (-z).  In units of u = 2^-24, for |z| <= 5: a term is within 12, a step's sixteen
+    terms add 15, the compensated sum 3, the joins over lanes, waves and parts at most 48: S and T within 78 u of themselves, 2^-17.7;
+    the logarithm and the last difference add 2^-22 |log p|.  A plain sum of the 4096 terms of a lane is off by up to 2^-14.6."""
+    values = [math.log(0.7), math.log(0.3), math.log(0.999), -5.0, -2.2, -0.1]
+    z = torch.empty((rows, vocab), dtype=dtype, device="cuda")
+    for r in range(rows):
+        z[r] = values[r % 6]
+    z[:, 3::509] = 0
+    n = len(range(3, vocab, 509))
+    at = torch.tensor([[3, 0]] * rows, dtype=torch.int32, device="cuda")
+    got = ops.token_scores(z, at, alternatives=1)
+    low = z[:, 0].double().cpu()
+    t = (vocab - n) * torch.exp(low) * -low
+    total = n + (vocab - n) * torch.exp(low)
+    want = -torch.log(total)
+    close(got.logprobs, torch.stack([want, low + want], 1), lambda w: 2.0 ** -17 + 2.0 ** -22 * w.abs())
+    entropy = torch.log(total) + t / total
+    assert ((got.entropy.double().cpu() - entropy).abs() <= 2.0 ** -17 * (1 + t / total) + 2.0 ** -22 * entropy).all()
+    assert (got.ids == 3).all()
