@@ -9,6 +9,8 @@ No counterpart in the reference, whose projections and answers are made by a rem
 from __future__ import annotations
 
 import math
+import numbers
+import operator
 from typing import NamedTuple
 
 import torch
@@ -20,6 +22,7 @@ EPILOGUES = {"bias": _hip.EPI_BIAS_BF16, "swish": _hip.EPI_BIAS_SWISH_BF16, "glu
              "residual": _hip.EPI_RESIDUAL_F32, "float": _hip.EPI_BIAS_F32}
 _INT8, _FLOAT32, _BFLOAT16, _LOGITS = (torch.int8,), (torch.float32,), (torch.bfloat16,), (torch.float32, torch.bfloat16)
 _NORM_WIDTHS = (256, 512, 1024, 2048, 4096)
+_EINVAL = -1                                             # OASR_EINVAL: refused before a launch
 
 
 def _call(name: str, device: torch.device, *args) -> None:
@@ -30,7 +33,25 @@ def _call(name: str, device: torch.device, *args) -> None:
     else:
         with torch.cuda.device(device):
             rc = fn(*args, _hip.stream_ptr(device.index))
+    if rc == _EINVAL:
+        raise ValueError(_hip.lib().oasr_last_error().decode("utf-8", "replace"))
     _hip.check(rc, name)
+
+
+def _number(v, what: str) -> float:
+    if type(v) is float:
+        return v
+    if not isinstance(v, numbers.Real):                  # a tensor among them: its value is on the device
+        raise ValueError(f"{what} must be a number")
+    return float(v)
+
+
+def _integer(v, what: str) -> int:
+    if type(v) is int:
+        return v
+    if isinstance(v, torch.Tensor) or not hasattr(v, "__index__"):
+        raise ValueError(f"{what} must be an integer")
+    return operator.index(v)
 
 
 def _rows(t, what: str, dtypes: tuple):
@@ -147,7 +168,7 @@ class LinearI8:
 
     def _output(self, x, epilogue, resid, out):
         """(epilogue code, output, its row pitch, residual's pointer, its row pitch) for input x."""
-        epi = EPILOGUES.get(epilogue)
+        epi = EPILOGUES.get(epilogue) if isinstance(epilogue, str) else None
         if epi is None:
             raise ValueError(f"epilogue must be one of {', '.join(EPILOGUES)}")
         n = self.out_features
@@ -186,6 +207,7 @@ class LinearI8:
         x2, m, k, ldx = _rows(x, "x", _BFLOAT16)
         if k != self.in_features or x.device != self.device:
             raise ValueError(f"x must have {self.in_features} columns on {self.device}")
+        alpha = _number(alpha, "alpha")
         epi, out, ldc, resid, ldr = self._output(x, epilogue, resid, out)
         if m == 0:
             return out
@@ -208,6 +230,7 @@ class LinearI8:
         gain_ptr, shift_ptr = _vector(gain, k, "gain", self.device), _vector(shift, k, "shift", self.device)
         if gain_ptr is None or shift_ptr is None or (gain_ptr | shift_ptr) % 16:
             raise ValueError("gain and shift must be given, 16-byte aligned")
+        alpha, eps = _number(alpha, "alpha"), _number(eps, "eps")
         epi, out, ldc, resid, ldr = self._output(x, epilogue, resid, out)
         if m == 0:
             return out
@@ -260,6 +283,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, al
     every row's entropy and its `alternatives` likeliest tokens.  `tokens`: int32 [...] or [..., n]; a negative one means
     none (0).  Masked logits (-inf) have probability 0 and are no alternatives; include/oasr.h says what else rows hold."""
     z, rows, vocab, ld = _rows(logits, "logits", _LOGITS)
+    alternatives = _integer(alternatives, "alternatives")
     lead, device = logits.shape[:-1], logits.device
     given, n = (*lead, 0), 0
     if tokens is not None:
@@ -283,7 +307,7 @@ def ctc_token_scores(logits: torch.Tensor, tokens: torch.Tensor, frames: torch.T
         raise ValueError("logits must be a contiguous tensor [batch, frames, pitch]")
     batch, t_pad, ld = logits.shape
     _rows(logits, "logits", _LOGITS)
-    vocab = ld if vocab is None else int(vocab)
+    vocab, alternatives = ld if vocab is None else _integer(vocab, "vocab"), _integer(alternatives, "alternatives")
     if not 1 <= vocab <= ld:
         raise ValueError(f"vocab must lie in [1, {ld}]")
     if not isinstance(tokens, torch.Tensor) or tokens.dim() != 2 or tokens.shape[0] != batch:

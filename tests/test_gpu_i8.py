@@ -513,3 +513,10 @@ def test_more_columns_than_a_launch_has_tiles_of_64():
         assert torch.equal(out[r], codes[:, 0].float() * float(a[r, 0]) * float(sa[r]) * 0.5)
     del layer, out, codes
     torch.cuda.empty_cache()
+
+
+def test_too_many_rows_are_a_value_error():
+    layer = ops.LinearI8(torch.ones((1, 1), device="cuda"))
+    with pytest.raises(ValueError, match="m must be below 2.24"):
+        layer(torch.zeros((1 << 24, 1), dtype=torch.bfloat16, device="cuda"))
+    torch.cuda.empty_cache()

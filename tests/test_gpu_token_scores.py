@@ -311,3 +311,11 @@ def test_sums_of_long_rows_do_not_drift(rows, vocab, dtype):
     entropy = torch.log(total) + t / total
     assert ((got.entropy.double().cpu() - entropy).abs() <= 2.0 ** -17 * (1 + t / total) + 2.0 ** -22 * entropy).all()
     assert (got.ids == 3).all()
+
+
+def test_sizes_past_the_limits_are_refused_as_value_errors():
+    with pytest.raises(ValueError, match="2.24 rows"):
+        ops.token_scores(torch.zeros((1 << 24, 1), device="cuda"))
+    with pytest.raises(ValueError, match="2.30 columns"):
+        ops.token_scores(torch.empty((1, (1 << 32) + 5), dtype=torch.bfloat16, device="cuda"), alternatives=2)
+    torch.cuda.empty_cache()

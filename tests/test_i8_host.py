@@ -1,5 +1,6 @@
 """Refusals of the 8-bit integer operators, made before anything is launched (no GPU needed), and the host-side quantiser."""
 
+import numpy
 import pytest
 import torch
 
@@ -218,3 +219,35 @@ def test_a_loaded_layer_has_to_be_on_a_device_and_whole(monkeypatch, recorded):
     monkeypatch.undo()                                   # host tensors again, as loading onto the host makes them
     with pytest.raises(ValueError, match="HIP device"):
         pickle.loads(saved)
+
+
+def test_arguments_of_other_types_are_value_errors(recorded):
+    """Before anything is launched, in the normalising call too."""
+    layer = ops.LinearI8(torch.rand((32, 256)), torch.rand(32))
+    x, v = torch.zeros((2, 256), dtype=torch.bfloat16), torch.ones(256)
+    del recorded[:]
+    for bad in ("0.5", None, [1.0], 1j, torch.tensor(0.5)):
+        for call in (lambda: layer(x, alpha=bad), lambda: layer.normed(x.float(), v, v, alpha=bad),
+                     lambda: layer.normed(x.float(), v, v, eps=bad)):
+            with pytest.raises(ValueError, match="must be a number"):
+                call()
+    for bad in (["bias"], None, 0, {}):
+        with pytest.raises(ValueError, match="epilogue must be"):
+            layer(x, epilogue=bad)
+    assert not recorded
+    for good in (1, 0.5, numpy.float32(2)):
+        layer(x, alpha=good)
+    assert len(recorded) == 3
+
+
+def test_sizes_that_the_library_refuses_are_value_errors(monkeypatch):
+    """What only the C call knows to be too large arrives as the refusal it is; a failing launch stays an OasrError."""
+    lib = _hip.lib()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(_hip, "stream_ptr", lambda index: None)
+    monkeypatch.setattr(lib, "oasr_linear_i8", lambda stream: lib.oasr_quant_i8_rows(A, 16, 1 << 24, 16, A, 64, A, stream))
+    with pytest.raises(ValueError, match="rows must be below"):
+        ops._call("oasr_linear_i8", torch.device("cuda", 0))
+    monkeypatch.setattr(lib, "oasr_linear_i8", lambda stream: -3)
+    with pytest.raises(_hip.OasrError):
+        ops._call("oasr_linear_i8", torch.device("cuda", 0))

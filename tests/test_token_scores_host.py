@@ -1,5 +1,6 @@
 """Refusals of the token scores, made before anything is launched (no GPU needed)."""
 
+import numpy
 import pytest
 import torch
 
@@ -80,3 +81,19 @@ def test_sizes_past_the_calls_32_bits_are_refused(monkeypatch):
     ops.token_scores(meta(3, (1 << 30) - 1), i32(3, 7))
     ops.ctc_token_scores(meta(2, 4, (1 << 32) + 5), i32(2, 3), i32(2, 3), vocab=100)      # a pitch is 64 bits wide
     assert [name for name, _ in reached] == ["oasr_token_scores", "oasr_ctc_token_scores"]
+
+
+def test_counts_of_other_types_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_rows", lambda t, what, dtypes: (t, t.numel() // t.shape[-1], t.shape[-1], t.shape[-1]))
+    reached = []
+    monkeypatch.setattr(ops, "_call", lambda name, device, *args: reached.append(args))
+    z, t = torch.zeros((1, 4, 9)), torch.zeros((1, 4), dtype=torch.int32)
+    for bad in (2.0, "2", None, [2], torch.tensor(2)):
+        for call in (lambda: ops.token_scores(z, alternatives=bad), lambda: ops.ctc_token_scores(z, t, t, alternatives=bad)):
+            with pytest.raises(ValueError, match="integer"):
+                call()
+    for bad in (3.7, "9"):
+        with pytest.raises(ValueError, match="integer"):
+            ops.ctc_token_scores(z, t, t, vocab=bad)
+    assert not reached
+    assert ops.ctc_token_scores(z, t, t, vocab=numpy.int64(5), alternatives=numpy.int32(2)).ids.shape == (1, 4, 2) and len(reached) == 1
