@@ -1,11 +1,11 @@
 """Per-block distance of the device encoder from the CPU oracle, through the whole depth of a geometry.
 
-    python tools/depth_parity.py [G7B|G300|GTINY] [--fp8] [--samples 33000,21000] [--layers N]
+    python tools/depth_parity.py [G7B|G300|GTINY] [--fp8 | --int8] [--samples 33000,21000] [--layers N]
 
 For every k = 0 .. n_layers the first k blocks run on the device (`oasr_encoder_forward` with
 `n_layers_run = k`) and are compared, per utterance, with the oracle's state after k blocks: the
 float32 forward (never quantised), and the forward that rounds where the device rounds
-(`device_rounding=True`; with --fp8 it also quantises the eight projections to e4m3).  Prints relative L2 and max abs per block.
+(`device_rounding=True`; with --fp8 it also quantises the eight projections to e4m3, with --int8 to 8-bit integers).  Prints relative L2 and max abs per block.
 Weights are drawn on the device (a 7 B-parameter set takes ~40 s from the CPU generator) and copied
 to the host for the oracle.
 """
@@ -68,7 +68,7 @@ def device_drawn_weights(g, seed: int) -> dict:
     return w
 
 
-def depth_curves(g, n_list, fp8: bool, seed: int = 31, weights: dict | None = None):
+def depth_curves(g, n_list, fp8: bool, seed: int = 31, weights: dict | None = None, int8: bool = False):
     """[(k, rel_f32, max_f32, rel_emu, max_emu)] per block k and the worst utterance, device vs the two oracles."""
     from omnilingual_asr.engine_hip import HipEngine
     from oracle import conformer as OC
@@ -85,8 +85,8 @@ def depth_curves(g, n_list, fp8: bool, seed: int = 31, weights: dict | None = No
     og = OC.Geometry(name=g.name, d_model=g.d_model, ffn_dim=g.ffn_dim, n_heads=g.n_heads, n_layers=g.n_layers)
     ft, lt = torch.from_numpy(feats), torch.from_numpy(lens)
     _, ref = OC.forward(ft, lt, w, og, per_layer=True)
-    _, emu = OC.forward(ft, lt, w, og, per_layer=True, fp8=fp8, device_rounding=True)
-    eng = HipEngine(g, weights=w, fp8=fp8)
+    _, emu = OC.forward(ft, lt, w, og, per_layer=True, fp8=fp8, int8=int8, device_rounding=True)
+    eng = HipEngine(g, weights=w, fp8=fp8, int8=int8)
     dev = torch.device("cuda")
     nv = torch.tensor(n_list, dtype=torch.int32, device=dev)
     f_dev, l_dev = eng.features(pcm.to(dev), nv)
@@ -110,6 +110,7 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("model", nargs="?", default="G7B")
     ap.add_argument("--fp8", action="store_true")
+    ap.add_argument("--int8", action="store_true")
     ap.add_argument("--samples", default="33000,21000")
     ap.add_argument("--layers", type=int, default=-1)
     a = ap.parse_args()
@@ -119,8 +120,8 @@ def main():
         g = dataclasses.replace(g, n_layers=a.layers)
     n_list = [int(s) for s in a.samples.split(",")]
     t0 = time.time()
-    rows = depth_curves(g, n_list, a.fp8)
-    print("%s %s, samples %s, %d blocks (%.0f s)" % (g.name, "fp8" if a.fp8 else "bf16", n_list, g.n_layers, time.time() - t0))
+    rows = depth_curves(g, n_list, a.fp8, int8=a.int8)
+    print("%s %s, samples %s, %d blocks (%.0f s)" % (g.name, "fp8" if a.fp8 else "int8" if a.int8 else "bf16", n_list, g.n_layers, time.time() - t0))
     print("blocks  rel-L2 vs float32  max abs   rel-L2 vs device-rounding oracle  max abs")
     for k, rf, mf, re, me in rows:
         print("%4d    %.3e         %.4f    %.3e                        %.4f" % (k, rf, mf, re, me))
