@@ -29,7 +29,7 @@ import torch.distributed as dist
 
 HBM_PEAK_GBS = 8000.0         # MI355X HBM3E spec
 MFMA_BF16_PEAK_TFLOPS = 2500.0  # dense bf16
-MFMA_FP8_PEAK_TFLOPS = 5000.0   # dense fp8
+MFMA_FP8_PEAK_TFLOPS = 5000.0   # dense fp8, and dense int8
 
 
 def synth_batch(batch: int, n: int, seed: int) -> torch.Tensor:
@@ -118,23 +118,24 @@ def kernel_rooflines(engine, batch: int, t_pad: int, pcm, nv, hidden) -> dict:
     rows = int(L.oasr_encoder_rows(batch, t_pad))
     dev = engine.device
     lw = engine._packed["layers"][0]
-    fp8 = engine.fp8
-    peak = MFMA_FP8_PEAK_TFLOPS if fp8 else MFMA_BF16_PEAK_TFLOPS
+    fp8, int8 = engine.fp8, engine.int8
+    peak = MFMA_FP8_PEAK_TFLOPS if fp8 or int8 else MFMA_BF16_PEAK_TFLOPS
     d, f = g.d_model, g.ffn_dim
     x = torch.zeros((rows, d), dtype=torch.float32, device=dev)
     x[:hidden.numel() // d] = hidden.reshape(-1, d)
     st = _hip.current_stream_ptr()
     bf = lambda r, c: torch.empty((r, c), dtype=torch.bfloat16, device=dev)
     xn, big, ctx = bf(rows, d), bf(rows, max(f, 3 * d)), bf(rows, d)
-    a8 = torch.empty((rows, max(f, d)), dtype=torch.uint8, device=dev) if fp8 else None
-    sa = torch.empty((rows,), dtype=torch.float32, device=dev) if fp8 else None
+    a8 = torch.empty((rows, max(f, d)), dtype=torch.uint8, device=dev) if fp8 or int8 else None
+    sa = torch.empty((rows,), dtype=torch.float32, device=dev) if fp8 or int8 else None
     resid = torch.zeros((rows, d), dtype=torch.float32, device=dev)
     lengths = torch.full((batch,), min(t_pad, int(_hip.num_stacked(pcm.shape[1]))), dtype=torch.int32, device=dev)
 
-    def ln():          # LayerNorm -> A operand of the up-projection (bf16 rows, or e4m3 rows + scales)
-        if fp8:
-            _hip.check(L.oasr_layernorm_fp8(x.data_ptr(), lw["ffn1_ln_w"].data_ptr(), lw["ffn1_ln_b"].data_ptr(),
-                                            a8.data_ptr(), sa.data_ptr(), rows, d, 1e-5, 0, st))
+    def ln():          # LayerNorm -> A operand of the up-projection (bf16 rows, or 8-bit rows + scales)
+        if fp8 or int8:
+            norm8 = L.oasr_layernorm_fp8 if fp8 else L.oasr_layernorm_i8
+            _hip.check(norm8(x.data_ptr(), lw["ffn1_ln_w"].data_ptr(), lw["ffn1_ln_b"].data_ptr(),
+                             a8.data_ptr(), sa.data_ptr(), rows, d, 1e-5, 0, st))
         else:
             _hip.check(L.oasr_layernorm(x.data_ptr(), lw["ffn1_ln_w"].data_ptr(), lw["ffn1_ln_b"].data_ptr(),
                                         xn.data_ptr(), rows, d, d, 1e-5, 1, 0, st))
@@ -151,15 +152,20 @@ def kernel_rooflines(engine, batch: int, t_pad: int, pcm, nv, hidden) -> dict:
                 fn8 = L.oasr_gemm_fp8_pw if w_packed else L.oasr_gemm_fp8
                 _hip.check(fn8(a8.data_ptr(), lw[wname + "_q"].data_ptr(), sa.data_ptr(),
                                lw[wname + "_s"].data_ptr(), bias, res, c.data_ptr(), rows, n, k, alpha, epi, st))
+            elif int8:
+                _hip.check(L.oasr_gemm_i8(a8.data_ptr(), k, lw[wname + "_q"].data_ptr(), sa.data_ptr(), lw[wname + "_s"].data_ptr(),
+                                          bias, res, n, c.data_ptr(), n, rows, n, k, alpha, epi, st))
             else:
                 _hip.check(L.oasr_gemm_bf16_ex(a.data_ptr(), lw[wname].data_ptr(), bias, res, c.data_ptr(), rows, n, k,
                                                alpha, epi, flags, st))
         return run
 
-    def quant(a, k):   # fp8: the row quantiser that feeds a projection whose input a GEMM / attention produced
+    def quant(a, k):   # 8-bit: the row quantiser that feeds a projection whose input a GEMM / attention produced
         def run():
             if fp8:
                 _hip.check(L.oasr_quant_fp8_rows(a.data_ptr(), rows, k, a8.data_ptr(), sa.data_ptr(), st))
+            elif int8:
+                _hip.check(L.oasr_quant_i8_rows(a.data_ptr(), k, rows, k, a8.data_ptr(), k, sa.data_ptr(), st))
         return run
 
     def entry(name, ms, flops, shape):
@@ -167,7 +173,7 @@ def kernel_rooflines(engine, batch: int, t_pad: int, pcm, nv, hidden) -> dict:
         return {"kernel": name + " " + shape, "bound": "mfma", "achieved": round(tf, 1), "peak": peak,
                 "unit": "TFLOP/s", "frac": round(tf / peak, 4), "flop_per_launch": flops, "avg_launch_ms": round(ms, 4)}
 
-    kern = "gemm_fp8_kernel" if fp8 else "gemm_bf16_kernel"
+    kern = "gemm_fp8_kernel" if fp8 else "gemm_i8_*_kernel" if int8 else "gemm_bf16_kernel"
     up = gemm(xn, "ffn1_w1", lw["ffn1_b1"].data_ptr(), None, big, f, d, 1.0, _hip.EPI_BIAS_SWISH_BF16, _hip.GEMM_C_PACKED)
     ms_up = _time_launches(ln, up)
     down = gemm(big, "ffn1_w2", lw["ffn1_b2"].data_ptr(), resid.data_ptr(), resid, d, f, 0.5, _hip.EPI_RESIDUAL_F32,
@@ -199,7 +205,7 @@ def kernel_rooflines(engine, batch: int, t_pad: int, pcm, nv, hidden) -> dict:
     up_shape = "%dx%dx%d" % (rows, f, d)
     lm_shape = "%dx%d" % (batch, pcm.shape[1])
     main = entry(kern + "<BIAS_SWISH>", ms_up, 2.0 * rows * f * d, up_shape)
-    main["traffic"] = measured_traffic("gemm_fp8_kernel<1>" if fp8 else "gemm_bf16_kernel<1>", up_shape)
+    main["traffic"] = None if int8 else measured_traffic("gemm_fp8_kernel<1>" if fp8 else "gemm_bf16_kernel<1>", up_shape)
     attn_e = entry("attention_relkey_kernel<%d>" % g.head_dim, ms_attn, attn_flops,
                    "%dx%dx%dx%d" % (batch, g.n_heads, t_valid, g.head_dim))
     attn_e["peak"], attn_e["frac"] = MFMA_BF16_PEAK_TFLOPS, round(attn_e["achieved"] / MFMA_BF16_PEAK_TFLOPS, 4)
@@ -217,13 +223,13 @@ def kernel_rooflines(engine, batch: int, t_pad: int, pcm, nv, hidden) -> dict:
     }
 
 
-# Tolerances of the parity tests (tests/test_gpu_encoder.py, tests/test_gpu_fp8.py): per utterance, relative
-# L2 and largest absolute difference of the encoder states against the CPU oracle.
-PARITY_TOL = {"bf16": (2e-2, 0.15), "fp8": (3e-2, None)}     # the fp8 test states no absolute bound
+# Tolerances of the parity tests (tests/test_gpu_encoder.py, tests/test_gpu_fp8.py, tests/test_gpu_i8_stages.py): per
+# utterance, relative L2 and largest absolute difference of the encoder states against the CPU oracle.
+PARITY_TOL = {"bf16": (2e-2, 0.15), "fp8": (3e-2, None), "int8": (3e-2, None)}     # the 8-bit tests state no absolute bound
 
 
 def cpu_baseline(engine, weights, pcm_rows: np.ndarray, seconds: float, hip_hidden, n_layers: int, runs: int) -> dict:
-    """The CPU oracle (float32 PyTorch restatement of the same geometry; with --fp8 its emulation of the
+    """The CPU oracle (float32 PyTorch restatement of the same geometry; with --fp8 or --int8 its emulation of the
     device's quantisation) on this host's cores, on a bounded sample of the benchmarked batch: the rows
     `pcm_rows` copied back from the device tensor the step ran on, through the first `n_layers` blocks.
     One warm-up on a single row, then the median of `runs` timed passes.  The oracle's output is then
@@ -241,7 +247,8 @@ def cpu_baseline(engine, weights, pcm_rows: np.ndarray, seconds: float, hip_hidd
     def one_pass(x):
         t0 = time.perf_counter()
         feats, lens = OL.features_batch(x, None)
-        out["hidden"] = OC.forward(torch.from_numpy(feats), torch.from_numpy(lens), w, og, fp8=engine.fp8)
+        out["hidden"] = OC.forward(torch.from_numpy(feats), torch.from_numpy(lens), w, og, fp8=engine.fp8,
+                                   int8=engine.int8)
         out["lens"] = lens
         return time.perf_counter() - t0
 
@@ -255,7 +262,7 @@ def cpu_baseline(engine, weights, pcm_rows: np.ndarray, seconds: float, hip_hidd
         a, b = hip_hidden[i, : lens[i]].double(), want[i, : lens[i]].double()
         rel = max(rel, float((a - b).norm() / b.norm()))
         mx = max(mx, float((a - b).abs().max()))
-    tol = PARITY_TOL["fp8" if engine.fp8 else "bf16"]
+    tol = PARITY_TOL["fp8" if engine.fp8 else "int8" if engine.int8 else "bf16"]
     depth = "all %d blocks" % n_layers if n_layers == g.n_layers else         "the first %d of %d blocks, time scaled by %d/%d" % (n_layers, g.n_layers, g.n_layers, n_layers)
     return {"value": round(pcm_rows.shape[0] * seconds / dt, 3), "unit": "x real time (audio-s/wall-s)",
             "cores": threads, "kind": "port",
@@ -263,6 +270,10 @@ def cpu_baseline(engine, weights, pcm_rows: np.ndarray, seconds: float, hip_hidd
                       "pass(es), %.1f s of CPU work in all" % (pcm_rows.shape[0] - 1, seconds, depth, runs, sum(times)),
             "parity": {"rows": int(pcm_rows.shape[0]), "blocks": n_layers, "rel_l2": round(rel, 5), "max_abs": round(mx, 4),
                        "tol_rel_l2": tol[0], "tol_max_abs": tol[1], "ok": bool(rel <= tol[0] and (tol[1] is None or mx <= tol[1]))}}
+
+
+def compute_dtype(args) -> str:
+    return "fp8 (e4m3) projections, bf16 elsewhere" if args.fp8 else "int8 projections, bf16 elsewhere" if args.int8 else "bf16"
 
 
 def run_long_audio(args, world: int, rank: int) -> None:
@@ -284,7 +295,7 @@ def run_long_audio(args, world: int, rank: int) -> None:
         s, e = int(bounds[i][0]) - base, int(bounds[i][1]) - base
         pcm[s:e] = synth_batch(1, e - s, 1234 + i)[0].numpy()
     mine = bounds[lo:hi] - base
-    pipe = GeminiASRPipeline(model=args.model, batch_size=args.batch, fp8=args.fp8)
+    pipe = GeminiASRPipeline(model=args.model, batch_size=args.batch, fp8=args.fp8, int8=args.int8)
     # warm-up: both slots of the full-batch shape, three batches each (the first replays of a freshly captured
     # graph carry one-off launch costs), and the tail shape (buffers, graphs, clocks)
     full = min(len(mine), 6 * args.batch)
@@ -324,7 +335,7 @@ def run_long_audio(args, world: int, rank: int) -> None:
             "value": round(total / 16000.0 / elapsed, 1), "unit": "x real time", "n_gpus": world,
             "steps": batches, "warmup": -(-full // args.batch) + (1 if tail else 0), "ms_per_step": round(elapsed / batches * 1e3, 3),
             "higher_is_better": True, "scaling": "strong", "vs_baseline": None,
-            "dtype": "fp8 (e4m3) projections, bf16 elsewhere" if args.fp8 else "bf16",
+            "dtype": compute_dtype(args),
             "data": "synthetic (seeded noise + 440 Hz tone per chunk, seed 1234 + chunk index), random-init weights seed 0",
             "config": {"workload": "BASELINE configs[3]: %.2f h of 16 kHz audio -> %d chunks of %.0f s, host chunk loop "
                                    "(page-locked assembly, upload, log-mel + %s encoder + CTC stage per batch of %d), "
@@ -344,6 +355,7 @@ def main() -> None:
     ap.add_argument("--seconds", type=float, default=30.0)
     ap.add_argument("--model", default="G300")
     ap.add_argument("--fp8", action="store_true", help="e4m3 weights and activations in the large projections")
+    ap.add_argument("--int8", action="store_true", help="8-bit integer weights and activations in the large projections")
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-kernel-timing", action="store_true")
@@ -383,7 +395,7 @@ def main() -> None:
 
     from omnilingual_asr.weights import init_random_weights, resolve_geometry
     weights = init_random_weights(resolve_geometry(args.model), 0)
-    engine = HipEngine(args.model, weights=weights, fp8=args.fp8)
+    engine = HipEngine(args.model, weights=weights, fp8=args.fp8, int8=args.int8)
     g = engine.geometry
     n = int(args.seconds * 16000)
     dev = engine.device
@@ -435,13 +447,13 @@ def main() -> None:
             "higher_is_better": True,
             "scaling": "weak",
             "vs_baseline": None,
-            "dtype": "fp8 (e4m3) projections, bf16 elsewhere" if args.fp8 else "bf16",
+            "dtype": compute_dtype(args),
             "data": "synthetic (seeded noise + 440 Hz tone), random-init weights seed 0",
             "config": {"workload": (("BASELINE configs[1]" if args.batch == 1 else "BASELINE configs[2]" if args.batch == 32
                                      else "geometry of BASELINE configs[2] at another batch size") if g.name == "G300"
                                     else "BASELINE configs[4]" if args.fp8 and args.batch == 8 else
-                                    "geometry of BASELINE configs[4]" + ("" if args.fp8 else " in bf16")) +
-                                   (" fp8" if args.fp8 and g.name == "G300" else "") +
+                                    "geometry of BASELINE configs[4]" + ("" if args.fp8 else " in int8" if args.int8 else " in bf16")) +
+                                   (" fp8" if args.fp8 and g.name == "G300" else " int8" if args.int8 and g.name == "G300" else "") +
                                    ": batch=%d x %.0f s chunks @16 kHz, log-mel + %s encoder "
                                    "(%d blocks, d=%d, %.0fM params), %s" %
                                    (args.batch, args.seconds, g.name, g.n_layers, g.d_model, g.n_params() / 1e6,
@@ -450,8 +462,8 @@ def main() -> None:
                        "parallelism": "chunks sharded over %d rank(s), one all-gather of records" % world},
             "encoder_tflops": round(flops_step / (elapsed / args.steps) / 1e12, 1),
             "encoder_mfma_frac": round(flops_step / (elapsed / args.steps) / 1e12 /
-                                       (MFMA_FP8_PEAK_TFLOPS if args.fp8 else MFMA_BF16_PEAK_TFLOPS), 4),
-            "encoder_mfma_peak": MFMA_FP8_PEAK_TFLOPS if args.fp8 else MFMA_BF16_PEAK_TFLOPS,
+                                       (MFMA_FP8_PEAK_TFLOPS if args.fp8 or args.int8 else MFMA_BF16_PEAK_TFLOPS), 4),
+            "encoder_mfma_peak": MFMA_FP8_PEAK_TFLOPS if args.fp8 or args.int8 else MFMA_BF16_PEAK_TFLOPS,
         }
         # The headline value is the resident-batch step.  Beside it: the same batch through the host chunk loop's
         # two-deep path (page-locked assembly is skipped, but the upload over PCIe, the step, the CTC stage and the
