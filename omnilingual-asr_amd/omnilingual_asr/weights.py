@@ -156,8 +156,10 @@ def pack_for_device(weights: dict, g: Geometry, device, fp8: bool = False, int8:
     """Device tensors in the layout of `oasr_layer_weights` / `oasr_top_weights` (include/oasr.h);
     with `fp8`, also the e4m3 codes and row scales of `oasr_layer_fp8_weights`, with `int8` the int8 codes (row-major
     still) and row scales of `oasr_layer_int8_weights`."""
-    bf = lambda t: t.to(device=device, dtype=torch.bfloat16).contiguous()
-    f32 = lambda t: t.to(device=device, dtype=torch.float32).contiguous()
+    # detached: a Parameter that already has the wanted type and device would come back as the object itself, whose storage
+    # Module.to() replaces, while the library keeps its address
+    bf = lambda t: t.detach().to(device=device, dtype=torch.bfloat16).contiguous()
+    f32 = lambda t: t.detach().to(device=device, dtype=torch.float32).contiguous()
     fp_w = torch.zeros((g.d_model, 192), dtype=torch.float32)
     fp_w[:, : g.feat_dim] = weights["fp_w"]
     top = {"fp_ln_w": f32(weights["fp_ln_w"]), "fp_ln_b": f32(weights["fp_ln_b"]),

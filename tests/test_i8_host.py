@@ -251,3 +251,19 @@ def test_sizes_that_the_library_refuses_are_value_errors(monkeypatch):
     monkeypatch.setattr(lib, "oasr_linear_i8", lambda stream: -3)
     with pytest.raises(_hip.OasrError):
         ops._call("oasr_linear_i8", torch.device("cuda", 0))
+
+
+def test_packed_weights_survive_a_module_that_moves():
+    """Weights that are Parameters of the wanted type are packed without a copy: their memory has to stay when the module they
+    belong to changes its type, since the encoder keeps addresses."""
+    from omnilingual_asr.weights import GEOMETRIES, init_random_weights, pack_for_device
+    g = GEOMETRIES["GTINY"]
+    w = init_random_weights(g, 1)
+    held = torch.nn.ParameterDict({"fp_b": w["fp_b"], "bo": w["layers"][0]["bo"]})
+    w["fp_b"], w["layers"][0]["bo"] = held["fp_b"], held["bo"]
+    packed = pack_for_device(w, g, "cpu", int8=True)
+    tensors = [packed["top"]["fp_b"], packed["layers"][0]["bo"]]
+    before = [(t.data_ptr(), t.clone()) for t in tensors]
+    held.double()
+    for t, (address, values) in zip(tensors, before):
+        assert t.data_ptr() == address and t.dtype == torch.float32 and torch.equal(t, values) and not t.requires_grad
