@@ -33,9 +33,10 @@ def _call(name: str, device: torch.device, *args) -> None:
     else:
         with torch.cuda.device(device):
             rc = fn(*args, _hip.stream_ptr(device.index))
-    if rc == _EINVAL:
-        raise ValueError(_hip.lib().oasr_last_error().decode("utf-8", "replace"))
-    _hip.check(rc, name)
+    if rc:
+        if rc == _EINVAL:
+            raise ValueError(_hip.lib().oasr_last_error().decode("utf-8", "replace"))
+        _hip.check(rc, name)
 
 
 def _number(v, what: str) -> float:
