@@ -418,7 +418,10 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmAr
 // grid is one work-group per CU; each walks its tiles in one continuous pipeline, the next tile's first slices being in
 // flight during the epilogue.  A ring of four slices of 64 k (16 KiB per operand), copied two slices ahead.
 // Work-groups with equal blockIdx % 8 share an XCD (used for locality only): an XCD owns a contiguous range of row tiles and
-// walks it in bands of four column tiles, so that a band's weights stay in that XCD's L2.
+// walks it in bands of four column tiles, so that a band's weights stay in that XCD's L2.  From 16 row tiles on the ranges are whole
+// row tiles, so some XCDs have one more than others, and with few rounds of tiles that is a round more than an even split would
+// take: 9216 x 1024 x 4096 has 144 tiles, 16 or 20 to an XCD of 18 work-groups, two rounds instead of one.
+// The residual form takes all 256 registers and spills nine (40 bytes of scratch, outside the loop over K).
 constexpr int kWide = 256, kWideRing = 4, kWideSlice = kWide * kSlice;
 
 template <int EPI>
@@ -550,8 +553,10 @@ __global__ __launch_bounds__(512) void gemm_i8_wide_kernel(const GemmArgs p, int
 // Problems with few tiles (single tokens, one utterance): a work-group of eight waves owns 16 MT x 64 outputs, and the
 // waves split K among them, slice by slice in turn.  Exact sums make the split free of consequences, and it is what keeps
 // enough bytes in flight: no wave waits for another before the end.  A wave brings its A rows through an LDS ring of its own
-// (DEPTH slices, no barriers) and its weight fragments straight to registers, both DEPTH - 1 slices ahead: about 200 KiB per
-// CU on their way, where the ring shared by the waves of a tile holds 48 (1504 x 1024 x 4096: 15.2 against 25.4 us).  At the end the partial
+// (DEPTH slices, no barriers) and its weight fragments straight to registers, both requested DEPTH - 1 slices ahead: up to
+// 200 KiB per CU, where the ring shared by the waves of a tile holds 48 (1504 x 1024 x 4096: 15.2 against 25.4 us).  They are not on
+// their way all the time: the weights are ordinary loads behind a condition, so at the loop's start the compiler waits for all that is
+// in flight, the slice just requested included, once in DEPTH slices (matrix pipe busy 12 % there, waits 40 %).  At the end the partial
 // sums cross LDS, and every wave finishes its share of the 16 x 32 outputs.
 template <int MT>
 struct SplitShape {
@@ -740,7 +745,8 @@ __global__ __launch_bounds__(256) void quant_i8_rows_kernel(const uint16_t* __re
 // on their way; the codes and scales are bit for bit those of the quantiser.  Bound by the weights' way from HBM: 16384 x 4096 at
 // one row (64 MiB) 12.8 us; small ones by latency (a second launch would cost more than the work).
 constexpr int kFewColumns = 32;              // 64 at a time are 5 - 25 % slower at every size tried (1 x 4096 x 4096: 8.4 against 10.2 us)
-constexpr int kFewDepth = 6;                 // slices on their way (4: up to 4 % slower; 8: faster on short n, slower on long)
+constexpr int kFewDepth = 6;                 // slices requested ahead (4: up to 4 % slower; 8: faster on short n, slower on long)
+                                             // (the first and last of six wait for all that is in flight, as above)
 
 template <int MT>
 struct FewShape {
@@ -922,7 +928,9 @@ static int check_gemm(const char* what, const int8_t* w, const float* scale_w, c
 // Which kernel runs a product: the one with the least estimated time, rounds * (begin + steps * step) microseconds.  A round is
 // 256 work-groups (one per CU; where several share a CU a further round costs `share` of one), a step one slice (64 k), or
 // for the splitting kernel eight.  The figures are fitted to times of all forms over 364 sizes (m 17 .. 4096, n 512 .. 16384,
-// k 512 .. 16384) and pick within 1.4 % of the fastest form on average: e.g. 1504 x 1024 x 4096: 96 rows split 14.8 us, 128 x 128
+// k 512 .. 16384) and pick within 1.4 % of the fastest form on average over those; larger m and smaller n are extrapolated, and the
+// 256 x 256 form, which takes most of the large ones, is priced at ceil(tiles / 256) rounds although its whole row tiles per XCD
+// may need one more (about a quarter of the sizes that it is picked for, up to twice the estimate).  E.g. 1504 x 1024 x 4096: 96 rows split 14.8 us, 128 x 128
 // tiles 25.8, 256 x 256 43.4; 1504 x 4096 x 1024: 23.2 (32 rows split), 14.4, 20.1; 512 x 1024 x 512: 4.5, 6.2, 10.0.
 // 16 rows split re-read the weights once per row tile: with more than 128 work-groups of them 32 rows are faster
 // (300 x 4096 x 4096: 17.4 against 22.3 us).
